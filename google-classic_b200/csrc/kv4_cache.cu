@@ -1,0 +1,361 @@
+// kv4_cache.cu -- the paged 4-bit KV cache: sizes and argument checks, rows of
+// keys and values quantised into their pages, and read back.
+//
+// Eight lanes hold a group of 32 values (four each) of one row, head and side:
+// the group's value of largest magnitude is found over them with shuffles, and
+// each lane writes the halfword of its four codes.  Both kernels move each
+// byte once and are bound by memory traffic.
+#include "kv4.cuh"
+
+#include <mutex>
+
+namespace {
+
+constexpr int ROW_THREADS = 256;
+
+size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
+size_t counter_bytes(const holo_kv4 *c) {
+    return round256(sizeof(int) * (size_t)c->max_seqs * c->n_kv_heads * (KV4_MAX_GROUP / KV4_HEADS));
+}
+size_t plan_bytes(const holo_kv4 *c) { return round256(sizeof(int) * (16 + 3 * (size_t)c->n_pages + 2 * (size_t)c->max_seqs)); }
+size_t partial_bytes(const holo_kv4 *c) {
+    return sizeof(float) * (size_t)KV4_MAX_CTAS * 2 * KV4_HEADS * (c->head_dim + 2);
+}
+
+std::mutex g_work_mu;
+
+// the library's own workspace on the current device, zero when it is made
+void *own_work(size_t bytes) {
+    HoloDevice *D = holo_dev();
+    if (!D) return nullptr;
+    std::lock_guard<std::mutex> lk(g_work_mu);
+    if (D->kv4_work_bytes < bytes) {
+        cudaDeviceSynchronize();   // calls that use the old one
+        if (D->kv4_work) cudaFree(D->kv4_work);
+        D->kv4_work = nullptr;
+        D->kv4_work_bytes = 0;
+        if (cudaMalloc(&D->kv4_work, bytes) != cudaSuccess || cudaMemset(D->kv4_work, 0, bytes) != cudaSuccess ||
+            cudaDeviceSynchronize() != cudaSuccess) {
+            cudaGetLastError();
+            holo_set_status(HOLO_E_NOMEM, "kv4 workspace");
+            return nullptr;
+        }
+        D->kv4_work_bytes = bytes;
+    }
+    return D->kv4_work;
+}
+
+// the sequence i with cu[i] <= row < cu[i + 1]: the last i with cu[i] <= row
+__device__ __forceinline__ int seq_of_row(const int *__restrict__ cu, int n, int row) {
+    int lo = 0, hi = n;   // cu[lo] <= row < cu[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (__ldg(cu + mid) <= row) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// where row `row` of the packed rows lies: its block and place; false where it
+// has none (rows outside cu, a sequence left out, a missing page)
+__device__ __forceinline__ bool row_place(const Kv4View &c, const int *cu, const int *start, const int *seqs, int n,
+                                          int row, int &page, int &block, int &slot) {
+    const int i = seq_of_row(cu, n, row);
+    const int first = __ldg(cu + i), at0 = __ldg(start + i), s = seqs ? __ldg(seqs + i) : i;
+    if (row < first || row >= __ldg(cu + i + 1) || at0 < 0) return false;
+    if (s < 0 || s >= c.max_seqs) {
+        kv4_report(c.status, HOLO_E_ARG);
+        return false;
+    }
+    const long long pos = (long long)at0 + (row - first);
+    const long long col = pos / c.page_tokens;
+    if (col >= c.max_pages) {
+        kv4_report(c.status, HOLO_E_ARG);
+        return false;
+    }
+    page = __ldg(c.tables + (size_t)s * c.max_pages + col);
+    if (page < 0 || page >= c.n_pages) {
+        kv4_report(c.status, HOLO_E_ARG);
+        return false;
+    }
+    const int in_page = (int)(pos - col * c.page_tokens);
+    block = in_page / KV4_BLOCK;
+    slot = in_page % KV4_BLOCK;
+    return true;
+}
+
+template <typename T> struct Four { T v[4]; };
+
+template <typename T>
+__device__ __forceinline__ void load4(const T *p, bool wide, float (&x)[4]) {
+    if (wide) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 w = __ldg(reinterpret_cast<const float4 *>(p));
+            x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w;
+        } else {
+            const uint2 w = __ldg(reinterpret_cast<const uint2 *>(p));
+            const T *h = reinterpret_cast<const T *>(&w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = kv4_to_float<T>(h[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = kv4_to_float<T>(p[i]);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T *p, bool wide, const float (&x)[4]) {
+    if (wide) {
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
+        } else {
+            uint2 w;
+            T *h = reinterpret_cast<T *>(&w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) h[i] = kv4_from_float<T>(x[i]);
+            *reinterpret_cast<uint2 *>(p) = w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = kv4_from_float<T>(x[i]);
+    }
+}
+
+// four codes of a lane and the scale of its group, over the eight lanes that
+// hold it: d = fp16(m / -8), code = rint(x / d) + 8 in 0..15 (fp32 arithmetic,
+// each operation rounded once), NaN as the scale where a value is not finite
+__device__ __forceinline__ uint32_t quantise4(const float (&x)[4], __half &d) {
+    float m = x[0];
+    bool finite = isfinite(x[0]);
+#pragma unroll
+    for (int i = 1; i < 4; ++i) {
+        if (fabsf(x[i]) > fabsf(m)) m = x[i];
+        finite = finite && isfinite(x[i]);
+    }
+    // of two equal magnitudes the lower lane's stays
+    const int lane = threadIdx.x & 7;
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+        const float other = __shfl_xor_sync(0xffffffffu, m, o, 8);
+        const bool lower = (lane & o) != 0;   // the other lane is the lower one
+        if (fabsf(other) > fabsf(m) || (lower && fabsf(other) == fabsf(m))) m = other;
+    }
+    const unsigned all = __ballot_sync(0xffffffffu, finite);
+    const unsigned mine = 0xffu << (threadIdx.x & 24);
+    d = (all & mine) == mine ? __float2half_rn(m * -0.125f) : __ushort_as_half(0x7e00);
+    const float w = __half2float(d);
+    uint32_t codes = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int q = w == 0.0f ? 0 : __float2int_rn(__fdiv_rn(x[i], w));
+        codes |= (uint32_t)max(0, min(15, q + 8)) << (4 * i);
+    }
+    return codes;
+}
+
+// Thread = (row, head, group b, four values g).  blockIdx.x strides the rows'
+// fours; whole groups of eight threads stay together (the shuffles), past the
+// end too.
+template <typename T, int HD>
+__global__ void __launch_bounds__(ROW_THREADS)
+append_kernel(const __grid_constant__ Kv4View c, const T *__restrict__ k, const T *__restrict__ v, long long k_row,
+              long long v_row, int rows, const int *__restrict__ cu, const int *__restrict__ start,
+              const int *__restrict__ seqs, int n, bool wide) {
+    constexpr int NB = HD / KV4_GROUP, FOURS = HD / 4;
+    const long long per_row = (long long)c.n_kv * FOURS, total = (long long)rows * per_row;
+    const long long step = (long long)gridDim.x * ROW_THREADS;
+    for (long long e0 = (long long)blockIdx.x * ROW_THREADS; e0 < total; e0 += step) {
+        const long long e = e0 + threadIdx.x;
+        const bool in = e < total;
+        const int row = in ? (int)(e / per_row) : 0, in_row = in ? (int)(e - (long long)row * per_row) : 0;
+        const int kvh = in_row / FOURS, four = in_row % FOURS, b = four >> 3, g = four & 7;
+        int page = 0, block = 0, slot = 0;
+        const bool ok = in && row_place(c, cu, start, seqs, n, row, page, block, slot);
+        float xk[4] = {0.0f, 0.0f, 0.0f, 0.0f}, xv[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (ok) {
+            load4(k + (size_t)row * k_row + (size_t)kvh * HD + 4 * four, wide, xk);
+            load4(v + (size_t)row * v_row + (size_t)kvh * HD + 4 * four, wide, xv);
+        }
+        __half dk, dv;
+        const uint32_t ck = quantise4(xk, dk), cv = quantise4(xv, dv);
+        if (ok) {
+            uint8_t *blk = kv4_block(c, HD, page, kvh, block);
+            *reinterpret_cast<uint16_t *>(blk + kv4_k_half(HD, slot, g, b)) = (uint16_t)ck;
+            *reinterpret_cast<uint16_t *>(blk + kv4_off_v(HD) + kv4_v_half(HD, slot, g, b)) = (uint16_t)cv;
+            if (g == 0) {
+                *reinterpret_cast<__half *>(blk + kv4_off_dk(HD) + 2 * (slot * NB + b)) = dk;
+                *reinterpret_cast<__half *>(blk + kv4_off_dv(HD) + 2 * (slot * NB + b)) = dv;
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ void dequantise4(uint32_t codes, __half d, float (&x)[4]) {
+    const float w = __half2float(d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = w * (float)((int)((codes >> (4 * i)) & 15u) - 8);
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(ROW_THREADS)
+read_kernel(const __grid_constant__ Kv4View c, T *__restrict__ k, T *__restrict__ v, long long k_row, long long v_row,
+            int rows, const int *__restrict__ cu, const int *__restrict__ start, const int *__restrict__ seqs, int n,
+            bool wide) {
+    constexpr int NB = HD / KV4_GROUP, FOURS = HD / 4;
+    const long long per_row = (long long)c.n_kv * FOURS, total = (long long)rows * per_row;
+    const long long step = (long long)gridDim.x * ROW_THREADS;
+    for (long long e = (long long)blockIdx.x * ROW_THREADS + threadIdx.x; e < total; e += step) {
+        const int row = (int)(e / per_row), in_row = (int)(e - (long long)row * per_row);
+        const int kvh = in_row / FOURS, four = in_row % FOURS, b = four >> 3, g = four & 7;
+        int page, block, slot;
+        float xk[4] = {0.0f, 0.0f, 0.0f, 0.0f}, xv[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (row_place(c, cu, start, seqs, n, row, page, block, slot)) {
+            const uint8_t *blk = kv4_block(c, HD, page, kvh, block);
+            const uint32_t ck = *reinterpret_cast<const uint16_t *>(blk + kv4_k_half(HD, slot, g, b));
+            const uint32_t cv = *reinterpret_cast<const uint16_t *>(blk + kv4_off_v(HD) + kv4_v_half(HD, slot, g, b));
+            dequantise4(ck, *reinterpret_cast<const __half *>(blk + kv4_off_dk(HD) + 2 * (slot * NB + b)), xk);
+            dequantise4(cv, *reinterpret_cast<const __half *>(blk + kv4_off_dv(HD) + 2 * (slot * NB + b)), xv);
+        }
+        store4(k + (size_t)row * k_row + (size_t)kvh * HD + 4 * four, wide, xk);
+        store4(v + (size_t)row * v_row + (size_t)kvh * HD + 4 * four, wide, xv);
+    }
+}
+
+int type_bytes(int type) { return type == HOLO_DT_F32 ? 4 : 2; }
+
+struct Rows {
+    const holo_kv4 *c;
+    void *k, *v;
+    long long k_row, v_row;
+    int rows;
+    const int *cu, *start, *seqs;
+    int n;
+};
+
+template <bool APPEND, typename T, int HD>
+void launch_rows(const Rows &r, const Kv4View &view, bool wide, int sms, cudaStream_t st) {
+    const long long total = (long long)r.rows * view.n_kv * (HD / 4);
+    const long long want = (total + ROW_THREADS - 1) / ROW_THREADS, most = (long long)sms * 32;
+    const unsigned grid = (unsigned)(want < most ? want : most);
+    if (APPEND)
+        append_kernel<T, HD><<<grid, ROW_THREADS, 0, st>>>(view, (const T *)r.k, (const T *)r.v, r.k_row, r.v_row, r.rows,
+                                                          r.cu, r.start, r.seqs, r.n, wide);
+    else
+        read_kernel<T, HD><<<grid, ROW_THREADS, 0, st>>>(view, (T *)r.k, (T *)r.v, r.k_row, r.v_row, r.rows, r.cu,
+                                                        r.start, r.seqs, r.n, wide);
+}
+
+template <bool APPEND, typename T>
+void launch_rows_hd(const Rows &r, const Kv4View &view, bool wide, int sms, cudaStream_t st) {
+    switch (r.c->head_dim) {
+    case 64: launch_rows<APPEND, T, 64>(r, view, wide, sms, st); break;
+    case 128: launch_rows<APPEND, T, 128>(r, view, wide, sms, st); break;
+    default: launch_rows<APPEND, T, 256>(r, view, wide, sms, st); break;
+    }
+}
+
+template <bool APPEND>
+int run_rows(Rows r, int layer, int type, const char *what) {
+    Kv4View view;
+    cudaStream_t st;
+    if (!kv4_begin(r.c, layer, what, view, st, nullptr)) return cuda_last_status();
+    if (type != HOLO_DT_F32 && type != HOLO_DT_F16 && type != HOLO_DT_BF16) {
+        holo_set_status(HOLO_E_UNSUPPORTED, what);
+        return HOLO_E_UNSUPPORTED;
+    }
+    const long long dense = (long long)r.c->n_kv_heads * r.c->head_dim;
+    if (r.k_row == 0) r.k_row = dense;
+    if (r.v_row == 0) r.v_row = dense;
+    if (r.rows < 0 || r.n < 0 || r.n > r.c->max_seqs || r.k_row < dense || r.v_row < dense ||
+        (r.rows > 0 && r.n > 0 && (!r.k || !r.v || !r.cu || !r.start))) {
+        holo_set_status(HOLO_E_ARG, what);
+        return HOLO_E_ARG;
+    }
+    if (r.rows == 0 || r.n == 0) return HOLO_OK;
+    const int size = type_bytes(type), four = 4 * size;
+    if (((uintptr_t)r.k | (uintptr_t)r.v) % size) {
+        holo_set_status(HOLO_E_ARG, what);
+        return HOLO_E_ARG;
+    }
+    // four values a load where every four of a row is aligned, else one by one
+    const bool wide = ((uintptr_t)r.k | (uintptr_t)r.v) % four == 0 && (r.k_row | r.v_row) % 4 == 0;
+    const int sms = holo_dev()->sms;
+    switch (type) {
+    case HOLO_DT_F32: launch_rows_hd<APPEND, float>(r, view, wide, sms, st); break;
+    case HOLO_DT_F16: launch_rows_hd<APPEND, __half>(r, view, wide, sms, st); break;
+    default: launch_rows_hd<APPEND, __nv_bfloat16>(r, view, wide, sms, st); break;
+    }
+    return kv4_end(what);
+}
+
+}  // namespace
+
+bool kv4_shape_ok(const holo_kv4 *c) {
+    return c && c->n_layers > 0 && c->n_kv_heads > 0 && (c->head_dim == 64 || c->head_dim == 128 || c->head_dim == 256) &&
+           c->page_tokens > 0 && c->page_tokens <= 256 && c->page_tokens % KV4_BLOCK == 0 && c->n_pages > 0 &&
+           c->max_seqs > 0 && c->max_pages > 0 && c->n_kv_heads <= 1024 && c->max_seqs <= (1 << 16) &&
+           c->n_pages <= (1 << 20) && (long long)c->max_pages * c->page_tokens <= 0x7fffffffLL;
+}
+
+bool kv4_begin(const holo_kv4 *c, int layer, const char *what, Kv4View &view, cudaStream_t &st, Kv4Work *work) {
+    HoloDevice *D = holo_dev();
+    if (!D) return false;
+    if (!kv4_shape_ok(c) || layer < 0 || layer >= c->n_layers || !c->pool || (uintptr_t)c->pool % 16 || !c->tables ||
+        !c->lens) {
+        holo_set_status(HOLO_E_ARG, what);
+        return false;
+    }
+    st = c->stream ? (cudaStream_t)c->stream : holo_stream();
+    view.page_blocks = c->page_tokens / KV4_BLOCK;
+    const size_t page = (size_t)c->n_kv_heads * view.page_blocks * kv4_block_bytes(c->head_dim);
+    view.pool = (uint8_t *)c->pool + (size_t)layer * c->n_pages * page;
+    view.tables = c->tables;
+    view.lens = c->lens;
+    view.refs = c->refs;
+    view.n_kv = c->n_kv_heads;
+    view.page_tokens = c->page_tokens;
+    view.n_pages = c->n_pages;
+    view.max_seqs = c->max_seqs;
+    view.max_pages = c->max_pages;
+    view.status = D->status;
+    if (work) {
+        uint8_t *w = (uint8_t *)(c->work ? c->work : own_work(cuda_kv4_work_bytes(c)));
+        if (!w) return false;
+        if ((uintptr_t)w % 16) {
+            holo_set_status(HOLO_E_ARG, what);
+            return false;
+        }
+        work->counters = (int *)w;
+        work->plan = (int *)(w + counter_bytes(c));
+        work->partial = (float *)(w + counter_bytes(c) + plan_bytes(c));
+    }
+    return true;
+}
+
+int kv4_end(const char *what) { return holo_check_launch(what) ? HOLO_OK : cuda_last_status(); }
+
+extern "C" {
+
+size_t cuda_kv4_pool_bytes(const holo_kv4 *c) {
+    if (!kv4_shape_ok(c)) return 0;
+    return (size_t)c->n_layers * c->n_pages * c->n_kv_heads * (c->page_tokens / KV4_BLOCK) * kv4_block_bytes(c->head_dim);
+}
+
+size_t cuda_kv4_work_bytes(const holo_kv4 *c) {
+    if (!kv4_shape_ok(c)) return 0;
+    return counter_bytes(c) + plan_bytes(c) + partial_bytes(c);
+}
+
+int cuda_kv4_append(const holo_kv4 *c, int layer, const void *k, const void *v, int type, long long k_row,
+                    long long v_row, int rows, const int *cu_rows, const int *start, const int *seqs, int n) {
+    return run_rows<true>({c, (void *)k, (void *)v, k_row, v_row, rows, cu_rows, start, seqs, n}, layer, type,
+                          "cuda_kv4_append");
+}
+
+int cuda_kv4_read(const holo_kv4 *c, int layer, void *k, void *v, int type, long long k_row, long long v_row, int rows,
+                  const int *cu_rows, const int *start, const int *seqs, int n) {
+    return run_rows<false>({c, k, v, k_row, v_row, rows, cu_rows, start, seqs, n}, layer, type, "cuda_kv4_read");
+}
+
+}  // extern "C"

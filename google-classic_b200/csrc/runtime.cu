@@ -177,7 +177,8 @@ int cuda_last_status(void) {
         if (e != cudaSuccess) holo_set_status((int)e, "stream synchronise");
         if (cudaMemcpy(&dev_status, D->status, sizeof(int), cudaMemcpyDeviceToHost) == cudaSuccess &&
             dev_status != 0)
-            holo_set_status(dev_status, "kernel bounded wait timed out");
+            holo_set_status(dev_status, dev_status == HOLO_E_TIMEOUT ? "kernel bounded wait timed out"
+                                                                     : "refused by a kernel: no free page, or an index out of range");
     }
     if (n > 0) {
         int na_status = holo_noalloc_collect_status(current_device(), false);
@@ -203,6 +204,7 @@ void cuda_clear_status(void) {
         cudaMemset(g_dev[id].status, 0, sizeof(int));
         cudaMemset(g_dev[id].mv_counters, 0, sizeof(int) * MV_MAX_ROWBLOCKS);
         cudaMemset(g_dev[id].mvb_counters, 0, sizeof(int) * MVB_MAX_GROUPS);
+        if (g_dev[id].kv4_work) cudaMemset(g_dev[id].kv4_work, 0, g_dev[id].kv4_work_bytes);
         cudaDeviceSynchronize();
     }
     int n = 0;
@@ -281,6 +283,7 @@ void cuda_cleanup(void) {
     cudaFree(D.reduce_buf);
     cudaFreeHost(D.pinned);
     if (D.tmp) cudaFree(D.tmp);
+    if (D.kv4_work) cudaFree(D.kv4_work);
     D = HoloDevice();
     std::lock_guard<std::mutex> lk(g_reg_mu);
     g_registry.clear();

@@ -25,6 +25,7 @@ TYPE_NAMES = {F32: "f32", F16: "f16", Q4_0: "q4_0", Q8_0: "q8_0", Q4_K: "q4_k", 
 BLOCK_ELEMS = {Q8_0: 32, Q4_0: 32, Q4_K: 256, Q6_K: 256, F16: 1, F32: 1}
 BLOCK_BYTES = {Q8_0: 34, Q4_0: 18, Q4_K: 144, Q6_K: 210, F16: 2, F32: 4}
 
+DT_F32, DT_F16, DT_BF16 = 0, 1, 30       # HOLO_DT_* of include/holo_b200.h
 ACT_F32, ACT_Q8 = 0, 1
 Q4K_REF, Q4K_GGML = 0, 1
 ROPE_HALF, ROPE_ADJACENT = 0, 1          # holo_model_desc.rope_mode
@@ -39,6 +40,7 @@ def row_bytes(gtype: int, cols: int) -> int:
 
 
 _vp, _fp, _i, _f, _sz = C.c_void_p, C.POINTER(C.c_float), C.c_int, C.c_float, C.c_size_t
+_ll = C.c_longlong
 
 # name -> (restype, argtypes); the C declarations are in include/*.h
 SIGNATURES = {
@@ -108,6 +110,14 @@ SIGNATURES = {
     "holo_model_last_timing": (_i, [_vp, _vp, _vp]),
     "holo_model_pos": (_i, [_vp]), "holo_model_reset": (None, [_vp]), "holo_model_free": (None, [_vp]),
     "cuda_matmul_quant_batched": (_i, [_vp, _vp, _vp, _i, _i, _i]),
+    "cuda_attention_packed": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "cuda_kv4_pool_bytes": (_sz, [_vp]), "cuda_kv4_work_bytes": (_sz, [_vp]),
+    "cuda_kv4_extend": (_i, [_vp, _vp, _vp, _vp, _i]),
+    "cuda_kv4_append": (_i, [_vp, _i, _vp, _vp, _i, _ll, _ll, _i, _vp, _vp, _vp, _i]),
+    "cuda_kv4_read": (_i, [_vp, _i, _vp, _vp, _i, _ll, _ll, _i, _vp, _vp, _vp, _i]),
+    "cuda_kv4_attention": (_i, [_vp, _i, _vp, _vp, _i, _ll, _ll, _i, _f, _vp, _i]),
+    "cuda_kv4_fork": (_i, [_vp, _vp, _vp, _i]), "cuda_kv4_release": (_i, [_vp, _vp, _i]),
+    "cuda_kv4_compact": (_i, [_vp]), "cuda_kv4_copy_pages": (_i, [_vp, _vp, _vp, _i]),
     "holo_model_forward_batch": (_i, [_vp, _vp, _vp]),
     "holo_model_generate_batch": (_i, [_vp, _vp, _i, _i, _vp, _vp, _vp]),
     "holo_model_comm_handle": (_i, [_vp, _vp]), "holo_model_shard": (_i, [_vp, _vp]), "holo_model_open_peers": (_i, [_vp, _vp]),

@@ -1,0 +1,99 @@
+"""Attention over packed prompts (include/holo_b200.h, cuda_attention_packed)
+on torch tensors.
+
+The reference forwards a prompt one position at a time (src/ai/llm.c:1049);
+here whole prompts of different lengths are rows of one call.  The arithmetic
+is the library's (csrc/packed_attn.cu); work is enqueued on torch's current
+stream.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import load, DT_F32, DT_F16, DT_BF16, HOLO_OK
+
+DTYPES = {torch.float32: DT_F32, torch.float16: DT_F16, torch.bfloat16: DT_BF16}
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+LEGACY_STREAM = 1   # cudaStreamLegacy: torch's default stream has the handle 0, which the library takes for its own
+
+
+def stream_of(t) -> int:
+    """The handle of torch's current stream on the device of t, which has to
+    be the current device (the library's state belongs to it)."""
+    index = t.device.index
+    if t.device.type != "cuda" or index != torch.cuda.current_device():
+        raise ValueError(f"tensor on {t.device}: the current CUDA device is needed")
+    return _raw_stream(index) or LEGACY_STREAM
+
+
+def check(rc: int, what: str):
+    """Raise on an error status, and clear it."""
+    if rc != HOLO_OK:
+        lib = load()
+        msg = lib.cuda_last_status_string().decode(errors="replace")
+        lib.cuda_clear_status()
+        raise RuntimeError(f"{what}: status {rc} ({msg})")
+
+
+class PackedDesc(C.Structure):
+    """holo_packed_desc."""
+    _fields_ = [("type", C.c_int), ("n_heads", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int),
+                ("n_seqs", C.c_int), ("total", C.c_int), ("scale", C.c_float),
+                ("q_row", C.c_longlong), ("q_head", C.c_longlong), ("k_row", C.c_longlong), ("k_head", C.c_longlong),
+                ("v_row", C.c_longlong), ("v_head", C.c_longlong), ("out_row", C.c_longlong),
+                ("out_head", C.c_longlong), ("stream", C.c_void_p)]
+
+
+def row_stride(t, what: str) -> int:
+    """Elements between the rows of t [rows][heads][head_dim] whose heads are
+    adjacent; 0, dense, where one row or none leaves it open."""
+    rows, heads, hd = t.shape
+    s = t.stride()
+    if (heads > 1 and s[1] != hd) or s[2] != 1 or (rows > 1 and s[0] < heads * hd):
+        raise ValueError(f"{what}: strides {s} of {tuple(t.shape)}: the heads of a row have to be adjacent, and rows apart")
+    return s[0] if rows > 1 else 0
+
+
+def _strides(t, what: str):
+    """Elements between the rows and between the heads of t [rows][heads][head_dim]."""
+    rows, heads, hd = t.shape
+    s = t.stride()
+    if s[2] != 1 or (rows > 1 and s[0] < hd) or (heads > 1 and s[1] < hd):
+        raise ValueError(f"{what}: strides {s} of {tuple(t.shape)}: the values of a head have to be adjacent, and heads apart")
+    return s[0] if rows > 1 else 0, s[1] if heads > 1 else 0
+
+
+def attention_packed(q, k, v, cu_seqlens, out=None, lse=None, scale: float = 0.0):
+    """Causal attention of packed prompts: q [total][n_heads][head_dim], k and
+    v [total][n_kv_heads][head_dim] (float16 or bfloat16, any strides between
+    rows and heads), cu_seqlens int32 [n_seqs + 1] on the device.  Returns out
+    (made when None); lse, when given, is float32 [n_heads][total] and gets
+    each row's log-sum-exp.  scale 0: 1 / sqrt(head_dim)."""
+    total, n_heads, hd = q.shape
+    if k.shape != v.shape or k.shape[0] != total or k.shape[2] != hd:
+        raise ValueError(f"attention_packed: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if out.shape != q.shape:
+        raise ValueError(f"attention_packed: out {tuple(out.shape)} for q {tuple(q.shape)}")
+    dtype = q.dtype
+    if dtype not in DTYPES or k.dtype != dtype or v.dtype != dtype or out.dtype != dtype:
+        raise TypeError(f"attention_packed: q {q.dtype}, k {k.dtype}, v {v.dtype}, out {out.dtype}: one type is needed")
+    if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or not cu_seqlens.is_contiguous():
+        raise TypeError("attention_packed: cu_seqlens is a contiguous int32 vector")
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (n_heads, total) or not lse.is_contiguous()):
+        raise TypeError("attention_packed: lse is a contiguous float32 [n_heads][total]")
+    device = q.device
+    for t in (k, v, out, cu_seqlens) if lse is None else (k, v, out, cu_seqlens, lse):
+        if t.device != device:
+            raise ValueError(f"attention_packed: tensors on {device} and {t.device}")
+    d = PackedDesc(DTYPES[dtype], n_heads, k.shape[1], hd, cu_seqlens.shape[0] - 1, total, scale,
+                   *_strides(q, "attention_packed: q"), *_strides(k, "attention_packed: k"),
+                   *_strides(v, "attention_packed: v"), *_strides(out, "attention_packed: out"), stream_of(q))
+    rc = load().cuda_attention_packed(C.byref(d), out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                      cu_seqlens.data_ptr(), None if lse is None else lse.data_ptr())
+    if rc:
+        check(rc, "cuda_attention_packed")
+    return out

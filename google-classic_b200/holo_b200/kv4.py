@@ -1,0 +1,183 @@
+"""A paged KV cache held in 4 bits (include/holo_b200.h, holo_kv4), on torch
+tensors.
+
+The reference keeps one contiguous fp32 cache a model (src/ai/llm.c:1165-1177)
+and serves one sequence.  Here many sequences share a pool of pages: their
+tables name the pages, forks share them, and everything is decided on the
+device.  The arithmetic is the library's (csrc/kv4_*.cu); work is enqueued on
+torch's current stream.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import load
+from .attention import DTYPES, check, row_stride, stream_of
+
+BLOCK = 16   # positions a block of a page
+
+
+class Kv4Desc(C.Structure):
+    """holo_kv4."""
+    _fields_ = [("n_layers", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int), ("page_tokens", C.c_int),
+                ("n_pages", C.c_int), ("max_seqs", C.c_int), ("max_pages", C.c_int), ("pool", C.c_void_p),
+                ("tables", C.c_void_p), ("lens", C.c_void_p), ("refs", C.c_void_p), ("work", C.c_void_p),
+                ("stream", C.c_void_p)]
+
+
+def _ints(t, what: str, shape=None):
+    if t.dtype != torch.int32 or not t.is_contiguous() or (shape is not None and tuple(t.shape) != tuple(shape)):
+        raise TypeError(f"{what} is a contiguous int32 tensor{'' if shape is None else ' ' + str(tuple(shape))}")
+    return t
+
+
+class Kv4Cache:
+    """The cache and its sequences.
+
+    Either made empty, of n_pages pages for max_seqs sequences of up to
+    max_pages pages each, or over tensors that the caller has: pool (uint8,
+    n_layers x n_pages x n_kv_heads x page_tokens / 16 x 18 * head_dim), tables
+    (int32 [max_seqs][max_pages]), lens (int32 [max_seqs]) and, for the calls
+    that allocate or move pages, refs (int32 [n_pages]).
+
+    Lists of sequences are int32 vectors on the device; seqs None is the
+    first ones in order.  Calls return when they are enqueued.  What a kernel
+    found wrong (no free page, an index out of range) is raised by check()."""
+
+    def __init__(self, n_layers: int, n_kv_heads: int, head_dim: int, page_tokens: int = 64, n_pages: int = 0,
+                 max_seqs: int = 0, max_pages: int = 0, pool=None, tables=None, lens=None, refs=None, device="cuda"):
+        self.lib = load()
+        blocks = page_tokens // BLOCK
+        if pool is None:
+            pool = torch.zeros(n_layers, n_pages, n_kv_heads, blocks, 18 * head_dim, dtype=torch.uint8, device=device)
+            tables = torch.full((max_seqs, max_pages), -1, dtype=torch.int32, device=device)
+            lens = torch.zeros(max_seqs, dtype=torch.int32, device=device)
+            refs = torch.zeros(n_pages, dtype=torch.int32, device=device)
+        if pool.dtype != torch.uint8 or not pool.is_contiguous() or pool.dim() != 5 or (
+                tuple(pool.shape[2:]) != (n_kv_heads, blocks, 18 * head_dim)) or pool.shape[0] != n_layers:
+            raise TypeError(f"Kv4Cache: pool {tuple(pool.shape)} {pool.dtype}")
+        _ints(tables, "Kv4Cache: tables")
+        _ints(lens, "Kv4Cache: lens", tables.shape[:1])
+        if refs is not None:
+            _ints(refs, "Kv4Cache: refs", (pool.shape[1],))
+        for t in (tables, lens, refs):
+            if t is not None and t.device != pool.device:
+                raise ValueError(f"Kv4Cache: tensors on {pool.device} and {t.device}")
+        self.pool, self.tables, self.lens, self.refs = pool, tables, lens, refs
+        self.desc = d = Kv4Desc(n_layers, n_kv_heads, head_dim, page_tokens, pool.shape[1], tables.shape[0],
+                                tables.shape[1], pool.data_ptr(), tables.data_ptr(), lens.data_ptr(),
+                                None if refs is None else refs.data_ptr())
+        self._at = C.addressof(d)
+        size = self.lib.cuda_kv4_work_bytes(self._at)
+        if size == 0:
+            raise ValueError("Kv4Cache: this shape is not supported (head_dim 64/128/256, page_tokens a multiple of 16)")
+        stream_of(pool)
+        self.work = torch.zeros(size, dtype=torch.uint8, device=pool.device)
+        d.work = self.work.data_ptr()
+
+    def _call(self, what: str, fn, *args):
+        self.desc.stream = stream_of(self.pool)
+        rc = fn(self._at, *args)
+        if rc:
+            check(rc, what)
+
+    def _seqs(self, seqs, n=None):
+        """(pointer, count) of a list of sequences."""
+        if seqs is None:
+            return None, self.desc.max_seqs if n is None else n
+        if seqs.dtype != torch.int32 or seqs.dim() != 1 or not seqs.is_contiguous() or seqs.device != self.pool.device:
+            raise TypeError("Kv4Cache: a list of sequences is a contiguous int32 vector on the cache's device")
+        return seqs.data_ptr(), seqs.shape[0]
+
+    def check(self):
+        """Waits for the work enqueued so far and raises what a kernel found wrong."""
+        torch.cuda.current_stream(self.pool.device).synchronize()
+        check(self.lib.cuda_last_status(), "Kv4Cache")
+
+    def extend(self, counts, seqs=None, start=None):
+        """Room for counts[i] more positions of each sequence; returns start,
+        their lengths before (-1 where there was no room)."""
+        _ints(counts, "Kv4Cache.extend: counts")
+        p, n = self._seqs(seqs, counts.shape[0])
+        if start is None:
+            start = torch.empty_like(counts)
+        if counts.shape != (n,) or _ints(start, "Kv4Cache.extend: start").shape != (n,):
+            raise ValueError("Kv4Cache.extend: one count and start a sequence")
+        self._call("cuda_kv4_extend", self.lib.cuda_kv4_extend, p, counts.data_ptr(), start.data_ptr(), n)
+        return start
+
+    def _rows(self, what, k, v, cu_rows, start, seqs):
+        d = self.desc
+        n = cu_rows.shape[0] - 1
+        p, m = self._seqs(seqs, n)
+        if (k.shape != v.shape or k.dim() != 3 or k.shape[1] != d.n_kv_heads or k.shape[2] != d.head_dim or m != n
+                or start.shape != (n,)):
+            raise ValueError(f"{what}: k {tuple(k.shape)}, v {tuple(v.shape)}, {n} sequences in cu_rows")
+        if k.dtype not in DTYPES or v.dtype != k.dtype:
+            raise TypeError(f"{what}: k {k.dtype}, v {v.dtype}")
+        if cu_rows.dtype != torch.int32 or start.dtype != torch.int32 or not cu_rows.is_contiguous() or not start.is_contiguous():
+            raise TypeError(f"{what}: cu_rows and start are contiguous int32 vectors")
+        device = self.pool.device
+        if k.device != device or v.device != device or cu_rows.device != device or start.device != device:
+            raise ValueError(f"{what}: a tensor is not on {device}")
+        return (k.data_ptr(), v.data_ptr(), DTYPES[k.dtype], row_stride(k, what), row_stride(v, what), k.shape[0],
+                cu_rows.data_ptr(), start.data_ptr(), p, n)
+
+    def append(self, layer: int, k, v, cu_rows, start, seqs=None):
+        """Writes rows cu_rows[i] .. cu_rows[i + 1] of k and v [rows][n_kv_heads]
+        [head_dim] (float32, float16 or bfloat16) to the positions from
+        start[i] on of each sequence."""
+        self._call("cuda_kv4_append", self.lib.cuda_kv4_append, layer,
+                   *self._rows("Kv4Cache.append", k, v, cu_rows, start, seqs))
+
+    def read(self, layer: int, cu_rows, start, k, v, seqs=None):
+        """The same rows read back into k and v, which are returned."""
+        self._call("cuda_kv4_read", self.lib.cuda_kv4_read, layer,
+                   *self._rows("Kv4Cache.read", k, v, cu_rows, start, seqs))
+        return k, v
+
+    def attention(self, layer: int, q, out=None, seqs=None, scale: float = 0.0):
+        """Attention of one query a sequence, q [n][n_heads][head_dim], over
+        all the positions that it holds; out like q."""
+        d = self.desc
+        n, n_heads, hd = q.shape
+        p, m = self._seqs(seqs, n)
+        if out is None:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        if m != n or hd != d.head_dim or out.shape != q.shape:
+            raise ValueError(f"Kv4Cache.attention: q {tuple(q.shape)}, out {tuple(out.shape)}, {m} sequences")
+        if q.dtype not in DTYPES or out.dtype != q.dtype:
+            raise TypeError(f"Kv4Cache.attention: q {q.dtype}, out {out.dtype}")
+        if q.device != self.pool.device or out.device != q.device:
+            raise ValueError(f"Kv4Cache.attention: a tensor is not on {self.pool.device}")
+        self._call("cuda_kv4_attention", self.lib.cuda_kv4_attention, layer, out.data_ptr(), q.data_ptr(),
+                   DTYPES[q.dtype], row_stride(q, "Kv4Cache.attention: q"), row_stride(out, "Kv4Cache.attention: out"),
+                   n_heads, scale, p, n)
+        return out
+
+    def fork(self, parents, children):
+        """children[i], an empty sequence, becomes a copy of parents[i]: full
+        pages are shared, a last page with room left is copied."""
+        p, n = self._seqs(parents)
+        k, m = self._seqs(children)
+        if n != m:
+            raise ValueError("Kv4Cache.fork: one child a parent")
+        self._call("cuda_kv4_fork", self.lib.cuda_kv4_fork, p, k, n)
+
+    def release(self, seqs):
+        """Empties sequences; pages that no other one holds become free."""
+        self._call("cuda_kv4_release", self.lib.cuda_kv4_release, *self._seqs(seqs))
+
+    def compact(self):
+        """Moves the pages in use to the front of the pool."""
+        self._call("cuda_kv4_compact", self.lib.cuda_kv4_compact)
+
+    def copy_pages(self, src, dst):
+        """Copies pages src[i] to dst[i] in every layer."""
+        p, n = self._seqs(src)
+        k, m = self._seqs(dst)
+        if n != m:
+            raise ValueError("Kv4Cache.copy_pages: one target a source")
+        self._call("cuda_kv4_copy_pages", self.lib.cuda_kv4_copy_pages, p, k, n)

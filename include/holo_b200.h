@@ -309,6 +309,123 @@ void holo_model_free(void *model);
  * accumulation.  Device pointers; HOLO_STATUS_OK or an error status. */
 int cuda_matmul_quant_batched(float *Y, const void *W, const float *X, int M, int N, int K);
 
+/* ---- serving many sequences: element types ---------------------------------
+ * Types of the rows that the operators below read and write (GGUF type ids). */
+#define HOLO_DT_F32  0
+#define HOLO_DT_F16  1
+#define HOLO_DT_BF16 30
+
+/* ---- attention over packed prompts --------------------------------------------
+ * No counterpart in the reference, which forwards one prompt one position at
+ * a time (src/ai/llm.c:1049, 1180-1210).  n_seqs prompts of different lengths
+ * lie one after another in the rows of q, k, v and out: sequence s has the
+ * rows cu_seqlens[s] .. cu_seqlens[s+1] (device int32, n_seqs + 1 values,
+ * from 0 to total; a sequence may be empty).  Row i, head h:
+ *   out = sum_j softmax_j(scale * q[i][h] . k[j][h / group]) * v[j][h / group]
+ * over the rows j <= i of its own sequence, group = n_heads / n_kv_heads.
+ * Scores, softmax statistics and sums are fp32; the softmax weights are
+ * rounded to the rows' type before they multiply v, and out once to it.
+ * q and out: [total][n_heads][head_dim], k and v: [total][n_kv_heads]
+ * [head_dim], with *_row elements from row to row and *_head from head to head
+ * (0: dense); head_dim 64, 128 or 256, type HOLO_DT_F16 or HOLO_DT_BF16.
+ * Values in masked places, infinities and NaN included, change nothing. */
+typedef struct {
+    int type;                       /* HOLO_DT_F16 or HOLO_DT_BF16: q, k, v and out */
+    int n_heads, n_kv_heads, head_dim;
+    int n_seqs, total;              /* sequences; rows of q, k, v and out */
+    float scale;                    /* of the scores; 0: 1 / sqrt(head_dim) */
+    long long q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;
+    void *stream;                   /* cudaStream_t; NULL: the library's (cuda_set_stream) */
+} holo_packed_desc;
+/* Device pointers; lse (fp32 [n_heads][total], each row's log of its sum of
+ * exp(scores)) may be NULL.  HOLO_STATUS_OK or the error status it records. */
+int cuda_attention_packed(const holo_packed_desc *d, void *out, const void *q, const void *k, const void *v,
+                          const int *cu_seqlens, float *lse);
+
+/* ---- a paged KV cache held in 4 bits ----------------------------------------------
+ * No counterpart in the reference, whose cache is one contiguous fp32 array a
+ * model (src/ai/llm.c:1165-1177).  Keys and values are held in pages of
+ * page_tokens positions that the sequences' tables name, so that sequences
+ * grow, share a common start, and leave, without moving one another.
+ *
+ * Values: groups of 32 consecutive values of a head share an fp16 scale
+ * d = m / -8, m the group's value of largest magnitude (the first of them);
+ * code = rint(x / d) + 8 clipped to 0..15, and x reads back as
+ * d * (code - 8): the arithmetic of GGUF's Q4_0.  A group with a value that is
+ * not finite reads back as NaN.
+ *
+ * Layout: pool [n_layers][n_pages][n_kv_heads][page_tokens / 16] blocks of 16
+ * positions, 18 * head_dim bytes each (nb = head_dim / 32 groups):
+ *   key codes    [position][quarter t of a group][group b] words of 8 codes:
+ *                nibble i is value 32 b + 8 t + i
+ *   value codes  [g / 2][position / 2][g % 2][position % 2][group b] halfwords
+ *                of 4 codes, g = 0..7: nibble i is value 32 b + 4 g + i
+ *   key scales   [position][group b] fp16
+ *   value scales [position][group b] fp16
+ * (a lane of a tensor-core fragment reads its share of a block with 16-byte
+ * loads, and a run of blocks of a page is one copy).
+ *
+ * tables [max_seqs][max_pages]: the pages of each sequence in order, -1 past
+ * them; lens [max_seqs]: positions held; refs [n_pages]: how many sequences
+ * hold a page, 0 for a free one.  All device memory of the caller's.  An empty
+ * cache has tables all -1, lens and refs all 0.  The calls are ordered by their
+ * stream and copy nothing to the host; what a kernel finds wrong (no free
+ * page, a page or sequence number out of range) is recorded for
+ * cuda_last_status, and the sequence it concerns is left out. */
+typedef struct {
+    int n_layers, n_kv_heads, head_dim;     /* head_dim 64, 128 or 256 */
+    int page_tokens, n_pages;               /* page_tokens a multiple of 16, up to 256; n_pages up to 2^20 */
+    int max_seqs, max_pages;                /* rows (up to 2^16) and columns of tables */
+    void *pool;                             /* cuda_kv4_pool_bytes, 16-byte aligned */
+    int *tables, *lens, *refs;
+    void *work;                             /* cuda_kv4_work_bytes, zero-filled before the first call and kept by
+                                             * the calls; NULL: the library's own.  Calls that may overlap (other
+                                             * streams) need work of their own */
+    void *stream;                           /* cudaStream_t; NULL: the library's (cuda_set_stream) */
+} holo_kv4;
+/* 0 for a shape that is not supported (nothing is recorded). */
+size_t cuda_kv4_pool_bytes(const holo_kv4 *c);
+size_t cuda_kv4_work_bytes(const holo_kv4 *c);
+
+/* Below: seqs NULL is the sequences 0 .. n-1, and lists name no sequence
+ * twice.  All return HOLO_STATUS_OK or the error status they record. */
+
+/* Makes room for counts[i] more positions of sequence seqs[i] and counts them
+ * into lens; start[i] is its length before.  New pages are the lowest free
+ * ones, in the order of the list.  Where the free pages or the table's columns do not
+ * suffice for a sequence (and, for want of pages, for those after it that need
+ * some), it is left as it was, start[i] is -1, and HOLO_E_NOMEM is recorded. */
+int cuda_kv4_extend(const holo_kv4 *c, const int *seqs, const int *counts, int *start, int n);
+/* Writes rows cu_rows[i] .. cu_rows[i+1] of k and v ([rows][n_kv_heads][head_dim]
+ * of `type`, *_row elements from row to row, 0: dense) to the positions
+ * start[i], start[i] + 1 ... of sequence seqs[i]; start[i] < 0: none. */
+int cuda_kv4_append(const holo_kv4 *c, int layer, const void *k, const void *v, int type, long long k_row,
+                    long long v_row, int rows, const int *cu_rows, const int *start, const int *seqs, int n);
+/* The same positions read back to k and v, rounded to `type`; rows whose page
+ * is missing become zero. */
+int cuda_kv4_read(const holo_kv4 *c, int layer, void *k, void *v, int type, long long k_row, long long v_row,
+                  int rows, const int *cu_rows, const int *start, const int *seqs, int n);
+/* One query a sequence over all the positions that it holds:
+ *   out[i][h] = sum_j softmax_j(scale * q[i][h] . k[j][h / group]) * v[j][h / group],
+ * j < lens[seqs[i]]; zeros for an empty sequence.  q and out [n][n_heads]
+ * [head_dim] of `type` (fp32, fp16 or bf16), *_row elements from row to row
+ * (0: dense), n_heads / n_kv_heads <= 16; scale 0: 1 / sqrt(head_dim).  fp32
+ * accumulation; with fp32 rows the products keep fp32's precision too. */
+int cuda_kv4_attention(const holo_kv4 *c, int layer, void *out, const void *q, int type, long long q_row,
+                       long long out_row, int n_heads, float scale, const int *seqs, int n);
+/* children[i] (an empty sequence) becomes a copy of parents[i]: the full pages are
+ * shared, a last page with room left is copied, in every layer, to the lowest
+ * free page.  Parents may repeat; no parent is a child of the same call. */
+int cuda_kv4_fork(const holo_kv4 *c, const int *parents, const int *children, int n);
+/* Empties sequences; pages that no other one holds become free. */
+int cuda_kv4_release(const holo_kv4 *c, const int *seqs, int n);
+/* Moves the pages in use to the front of the pool: those at or above their
+ * number, in ascending order, to the free ones below it, and renames them in
+ * tables.  A pool may be cut there afterwards. */
+int cuda_kv4_compact(const holo_kv4 *c);
+/* Copies pages src[i] to dst[i] in every layer (no page is both, no dst twice). */
+int cuda_kv4_copy_pages(const holo_kv4 *c, const int *src, const int *dst, int n);
+
 /* Seeded synthetic weights on the device: rows x cols values N(0, std) from a
  * counter-based generator, written to dst as raw GGUF blocks of ggml_type
  * (0 F32, 1 F16 plain values; 8 Q8_0, 2 Q4_0, 12 Q4_K round-to-nearest), the

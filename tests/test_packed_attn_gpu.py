@@ -1,0 +1,160 @@
+"""Attention over packed prompts (include/holo_b200.h, cuda_attention_packed)
+against the formula in 64 bits (serving_reference.py)."""
+import numpy as np
+import pytest
+import torch
+
+import holo_b200 as hb
+import serving_reference as ref
+
+pytestmark = pytest.mark.gpu
+DTYPES = {"f16": torch.float16, "bf16": torch.bfloat16}
+
+
+@pytest.fixture(scope="module")
+def packed(dev):
+    from holo_b200.attention import attention_packed
+    return attention_packed
+
+
+def cu_of(lens):
+    return torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32, device="cuda")
+
+
+def rows(lens, heads, n_kv, hd, dtype, seed, spread=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return [(torch.randn(sum(lens), h, hd, generator=g) * m).to(DTYPES[dtype]).cuda()
+            for h, m in ((heads, spread), (n_kv, spread), (n_kv, 1.0))]
+
+
+def check(packed, lens, heads, n_kv, hd, dtype, seed, scale=0.0, spread=1.0, some=None):
+    q, k, v = rows(lens, heads, n_kv, hd, dtype, seed, spread)
+    out, lse = torch.full_like(q, 9.0), torch.full((heads, sum(lens)), 9.0, device="cuda")
+    packed(q, k, v, cu_of(lens), out, lse, scale)
+    assert torch.equal(packed(q, k, v, cu_of(lens), scale=scale), out)
+    torch.cuda.synchronize()
+    y, qs, ks, vs = (x.double().cpu().numpy() for x in (out, q, k, v))
+    sc, ls = scale or hd ** -0.5, lse.double().cpu().numpy()
+    for h in some or range(heads):
+        a = 0
+        for n in lens:
+            kh, vh, qh = ks[a:a + n, h * n_kv // heads], vs[a:a + n, h * n_kv // heads], qs[a:a + n, h]
+            if n:
+                want, sums = ref.attend(qh, kh, vh, sc, causal=True)
+                assert np.abs(y[a:a + n, h] - want).max() <= ref.bound(qh, kh, vh, sc, dtype), (h, n)
+                # scores off by s, the sum of n exps by (n + 8) 2^-23
+                s = hd * 2.0 ** -22 * np.abs(qh).max() * np.abs(kh).max() * sc
+                assert np.abs(ls[h, a:a + n] - sums).max() <= 2 * s + (n + 8) * 2.0 ** -23 + 2.0 ** -22 * np.abs(sums).max()
+            a += n
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,n_kv,hd", [(4, 2, 64), (3, 1, 128), (2, 2, 256), (8, 1, 128)])
+def test_matches_formula(packed, dtype, heads, n_kv, hd):
+    """Lengths about the tiles' edges, empty sequences first, between and last."""
+    check(packed, [0, 1, 127, 128, 0, 129, 3, 255, 256, 257, 0], heads, n_kv, hd, dtype, heads + hd)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_long_sequence(packed, hd):
+    check(packed, [1500, 77], 2, 1, hd, "bf16", 4)
+
+
+def test_many_short_sequences(packed):
+    lens = list(np.random.default_rng(0).integers(0, 20, 300))
+    check(packed, lens, 4, 1, 64, "f16", 5, some=[0, 3])
+
+
+@pytest.mark.parametrize("spread,scale", [(1.0, 0.5), (6.0, 0.0), (1e-3, 0.0)])
+def test_scales(packed, spread, scale):
+    """Sharp softmax weights, flat ones, and a scale of one's own."""
+    check(packed, [300, 40], 2, 1, 128, "f16", 6, scale=scale, spread=spread)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_values_in_masked_places_change_nothing(packed, hd, bad):
+    """A sequence whose keys and values are not finite leaves its neighbours alone, and a token that is not finite leaves the
+    earlier ones of its own sequence alone; those after it show it."""
+    lens = [70, 90, 130]
+    q, k, v = rows(lens, 4, 2, hd, "f16", 7)
+    cu = cu_of(lens)
+    want = packed(q, k, v, cu).clone()
+    k[75:160], v[75:160] = bad, bad        # from token 5 of the second sequence on
+    got = packed(q, k, v, cu)
+    assert torch.equal(got[:75], want[:75]) and torch.equal(got[160:], want[160:])
+    assert got[75:160].isnan().all()
+
+
+def test_strides(packed):
+    """q, k and v as columns of one matrix of rows, heads before rows, and an odd offset that no wide load takes."""
+    lens, heads, n_kv, hd = [130, 30], 4, 2, 64
+    total = sum(lens)
+    q, k, v = rows(lens, heads, n_kv, hd, "f16", 8)
+    want = packed(q, k, v, cu_of(lens))
+    both = torch.cat([q.flatten(1), k.flatten(1), v.flatten(1)], 1)
+    cut = [x.unflatten(1, (-1, hd)) for x in both.split([heads * hd, n_kv * hd, n_kv * hd], 1)]
+    assert torch.equal(packed(*cut, cu_of(lens)), want)
+    turned = [x.transpose(0, 1).contiguous().transpose(0, 1) for x in (q, k, v)]
+    out = torch.empty(heads, total, hd, dtype=q.dtype, device="cuda").transpose(0, 1)
+    assert torch.equal(packed(*turned, cu_of(lens), out=out), want)
+    odd = torch.zeros(total, 1 + both.shape[1], dtype=both.dtype, device="cuda")
+    odd[:, 1:] = both
+    cut = [x.unflatten(1, (-1, hd)) for x in odd[:, 1:].split([heads * hd, n_kv * hd, n_kv * hd], 1)]
+    got = packed(*cut, cu_of(lens))
+    tol = ref.bound(*(x.double().cpu().numpy().reshape(-1, hd) for x in (q, k, v)), hd ** -0.5, "f16")
+    assert (got.double() - want.double()).abs().max() <= 2 * tol
+
+
+def test_rows_outside_the_sequences_keep_their_memory(packed):
+    """cu_seqlens that does not reach the last rows: no more than those rows' results may change."""
+    q, k, v = rows([200], 2, 1, 64, "f16", 9)
+    want = packed(q, k, v, cu_of([200]))
+    out = torch.zeros_like(q)
+    packed(q, k, v, cu_of([150]), out=out)
+    assert torch.equal(out[:150], want[:150])
+
+
+def test_streams_and_graphs(packed):
+    q, k, v = rows([300, 20], 2, 1, 128, "bf16", 10)
+    cu = cu_of([300, 20])
+    want = packed(q, k, v, cu).clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = packed(q, k, v, cu)
+    side.synchronize()
+    assert torch.equal(got, want)
+    out = torch.zeros_like(q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        packed(q, k, v, cu, out=out)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
+def test_refusals(packed):
+    q, k, v = rows([10], 4, 2, 64, "f16", 1)
+    cu = cu_of([10])
+    with pytest.raises(TypeError):
+        packed(q.float(), k.float(), v, cu)
+    with pytest.raises(TypeError):
+        packed(q, k, v.bfloat16(), cu)
+    with pytest.raises(TypeError):
+        packed(q, k, v, cu.long())
+    with pytest.raises(ValueError):
+        packed(q, k[:9], v[:9], cu)
+    with pytest.raises(ValueError):
+        packed(q, k, v.transpose(1, 2).contiguous().transpose(1, 2), cu)
+    with pytest.raises(ValueError):
+        packed(q, k[:1].expand_as(k), v, cu)
+    with pytest.raises(RuntimeError, match=str(hb.HOLO_E_UNSUPPORTED)):
+        packed(q.float(), k.float(), v.float(), cu)
+    with pytest.raises(RuntimeError, match=str(hb.HOLO_E_UNSUPPORTED)):
+        packed(q[..., :32].contiguous(), k[..., :32].contiguous(), v[..., :32].contiguous(), cu)
+    with pytest.raises(RuntimeError, match=str(hb.HOLO_E_ARG)):
+        packed(q[:, :3], k, v, cu)
+    with pytest.raises(RuntimeError, match=str(hb.HOLO_E_ARG)):
+        packed(q, k, v, cu, scale=-1.0)
+    assert packed(q[:0], k[:0], v[:0], cu_of([0])).shape == (0, 4, 64)
