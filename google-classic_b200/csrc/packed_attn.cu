@@ -1,11 +1,46 @@
 // packed_attn.cu -- causal attention of whole prompts of different lengths
 // that lie one after another in the rows (holo_b200.h, cuda_attention_packed).
+//
+// Two kernels.  The tensor-core kernel takes rows that TMA can address
+// (head size 64 or 128, bases and strides of whole 16 bytes); other rows, and
+// head size 256, whose output does not fit in TMEM beside the scores, take one
+// warp a row and head.
+//
+// Tensor-core kernel: a CTA takes 256 query rows of one head and sequence as
+// two tiles of 128, and walks the sequence's keys 128 at a time up to the
+// diagonal.
+//   S_t = Q_t K^T    tcgen05.mma, Q_t and K from shared memory, S_t in TMEM
+//   P_t = 2^(c S_t - m)   a thread a row: it reads its row of S_t, keeps the
+//                    row's maximum m and sum l, and writes P_t (16 bits) over S_t
+//   O_t += P_t V     tcgen05.mma, P_t from TMEM, V from shared memory as it
+//                    lies (keys by dims: the transposed operand), O_t in TMEM
+// Warps 0-3 and 4-7 are the softmax of tile 0 and 1 (TMEM lane = query row),
+// warp 8 issues the MMAs, warp 9 the TMA loads of K and V into a ring of tiles
+// of 128 keys.  The two tiles alternate, so that the tensor core works on one
+// while the other's exponentials are taken: for head size 128 a pair of tiles
+// is 4 x 128^3 MACs, 2048 cycles of the tensor core, and 2 x 128^2
+// exponentials, 2048 cycles of the special-function units.
+// O_t is rescaled only when a row's maximum has grown by more than 2^8 since
+// the last time, which after the first key tiles is rare; P <= 256 loses no
+// precision, its rounding being relative.
+//
+// A masked place never counts: its P is an exact 0, and the values that are not
+// finite in a diagonal tile of V, the only ones with masked places, are set to 0
+// by warps 10 and 11 before the tensor core reads the tile.  The rows that do
+// see such a value, and any whose result is not finite, are taken again alone
+// over their own keys.
 #include "holo_common.cuh"
+#include "mv_unit.cuh"
+#include "tc_util.cuh"
 
+#include <cuda.h>
 #include <cuda_bf16.h>
-#include <cfloat>
+
+#include <mutex>
 
 namespace {
+
+using namespace holo_tc;
 
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -20,29 +55,34 @@ struct PackedArgs {
     int n_seqs, total, n_heads, group;
     float scale;
     long long q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;
+    int *status;
 };
 
-// the sequence of a row: the last s with cu[s] <= row
-__device__ __forceinline__ int packed_seq(const int *__restrict__ cu, int n, int row) {
-    int lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (__ldg(cu + mid) <= row) lo = mid;
-        else hi = mid;
-    }
-    return lo;
+// first row and length of sequence s, inside the rows whatever cu says
+__device__ __forceinline__ void packed_seq(const PackedArgs &a, int s, int &first, int &len) {
+    first = max(0, __ldg(a.cu + s));
+    len = max(0, min(a.total, __ldg(a.cu + s + 1)) - first);
 }
 
-// One warp a row and head, lane l holding dims l, l + 32, ...: online softmax
-// over the row's own keys.
+// ---------------------------------------------------------------------------
+// one warp a row and head: lane l holds dims l, l + 32, ...; online softmax
+// over the row's own keys
+// ---------------------------------------------------------------------------
 template <typename T, int HD>
 __global__ void __launch_bounds__(128)
 packed_simple_kernel(const __grid_constant__ PackedArgs a) {
     constexpr int NB = HD / 32;
     const int row = blockIdx.x * 4 + (threadIdx.x >> 5), h = blockIdx.y, lane = threadIdx.x & 31;
     if (row >= a.total) return;
-    const int s = packed_seq(a.cu, a.n_seqs, row);
-    const int first = max(0, a.cu[s]);
+    int lo = 0, hi = a.n_seqs;   // the last s with cu[s] <= row
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (__ldg(a.cu + mid) <= row) lo = mid;
+        else hi = mid;
+    }
+    int first, len;
+    packed_seq(a, lo, first, len);
+    if (row < first || row >= first + len) return;
     const T *q = (const T *)a.q + row * a.q_row + h * a.q_head;
     float qv[NB], acc[NB], m = -INFINITY, l = 0.0f;
 #pragma unroll
@@ -51,12 +91,14 @@ packed_simple_kernel(const __grid_constant__ PackedArgs a) {
         acc[b] = 0.0f;
     }
     for (int j = first; j <= row; ++j) {
-        const T *k = (const T *)a.k + j * a.k_row + h / a.group * a.k_head, *v = (const T *)a.v + j * a.v_row + h / a.group * a.v_head;
+        const T *k = (const T *)a.k + j * a.k_row + h / a.group * a.k_head;
+        const T *v = (const T *)a.v + j * a.v_row + h / a.group * a.v_head;
         float dot = 0.0f;
 #pragma unroll
         for (int b = 0; b < NB; ++b) dot = fmaf(qv[b], to_float(k[32 * b + lane]), dot);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        if (dot == -INFINITY) continue;   // weight 0
         const float mn = fmaxf(m, dot), fix = expf(m - mn), e = expf(dot - mn);
         l = l * fix + e;
         m = mn;
@@ -79,12 +121,471 @@ void launch_simple(const PackedArgs &a, int hd, cudaStream_t st) {
     }
 }
 
+// ---------------------------------------------------------------------------
+// tensor-core kernel
+// ---------------------------------------------------------------------------
+constexpr int PK_ROWS = 128;           // query rows a tile (MMA M), keys a tile (MMA N of S, K of P V)
+constexpr int PK_THREADS = 384;        // three warpgroups
+// registers a thread, of 384 * 168 at launch: 2 * 208 + 80 <= 3 * 168
+constexpr int PK_SOFTMAX_REGS = 208, PK_OTHER_REGS = 80;
+constexpr uint32_t PK_TMEM_COLS = 512; // S_0, S_1, O_0, O_1: 128 columns each
+constexpr float PK_GROWTH = 8.0f;      // log2 of what a row's maximum may grow by before its O is rescaled
+constexpr int PK_STAGES = 5;           // ring of K and V tiles
+
+template <int HD> struct PkGeom {
+    static constexpr int TILE = PK_ROWS * HD * 2;   // bytes of a Q, K or V tile
+    static constexpr size_t SMEM = 1024 + (size_t)(2 + PK_STAGES) * TILE;
+};
+
+struct PkBars {
+    uint64_t q_full[2], s_full[2], p_full[2], o_done[2], kv_full[PK_STAGES], kv_empty[PK_STAGES], v_checked[2], drain;
+    uint32_t tmem;
+    int first, len, pair;              // the CTA's work: its sequence's first row and length, and 256-row tile
+    int bad_from;                      // first key of the diagonal tiles with a value that is not finite
+};
+
+__device__ __forceinline__ void pk_tma_load(void *dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        :: "r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar)) : "memory");
+}
+
+// descriptor of an MN-major, 128-byte-swizzled operand of 128 K rows: a K row
+// is 128 bytes (64 MN values), 8 of them 1024 bytes (SBO), the next 64 MN
+// values 128 rows on (LBO)
+__device__ __forceinline__ uint64_t pk_desc_mn(const void *smem) {
+    return (uint64_t)((smem_addr(smem) >> 4) & 0x3FFFu) | ((uint64_t)(PK_ROWS * 128 >> 4) << 16) |
+           ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+template <typename T> struct PkType;
+template <> struct PkType<__half> {
+    static constexpr uint32_t AB = 0;   // fp16 operands
+    static constexpr uint32_t EXPONENT = 0x7c007c00u;
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        uint32_t r;
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        return r;
+    }
+};
+template <> struct PkType<__nv_bfloat16> {
+    static constexpr uint32_t AB = (1u << 7) | (1u << 10);   // bf16 operands
+    static constexpr uint32_t EXPONENT = 0x7f807f80u;
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        uint32_t r;
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        return r;
+    }
+};
+
+__device__ __forceinline__ float pk_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// two fp32 values in one 64-bit register, for the paired fp32 instructions
+__device__ __forceinline__ uint64_t pk_pair(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void pk_split(uint64_t p, float &lo, float &hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p));
+}
+__device__ __forceinline__ uint64_t pk_fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t pk_add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// Row `row` of head h over its own keys first .. row, by one thread: for rows
+// whose tiles hold values that are not finite.
+template <typename T, int HD>
+__device__ __noinline__ void pk_row_alone(const PackedArgs &a, int row, int first, int h) {
+    const T *q = (const T *)a.q + row * a.q_row + h * a.q_head;
+    float acc[HD], m = -INFINITY, l = 0.0f;
+    for (int d = 0; d < HD; ++d) acc[d] = 0.0f;
+    for (int j = first; j <= row; ++j) {
+        const T *k = (const T *)a.k + j * a.k_row + h / a.group * a.k_head;
+        const T *v = (const T *)a.v + j * a.v_row + h / a.group * a.v_head;
+        float dot = 0.0f;
+        for (int d = 0; d < HD; ++d) dot = fmaf(to_float(q[d]), to_float(k[d]), dot);
+        dot *= a.scale;
+        if (dot == -INFINITY) continue;   // weight 0
+        const float mn = fmaxf(m, dot), fix = expf(m - mn), e = expf(dot - mn);
+        l = l * fix + e;
+        m = mn;
+        for (int d = 0; d < HD; ++d) acc[d] = fmaf(e, to_float(v[d]), acc[d] * fix);
+    }
+    T *o = (T *)a.out + row * a.out_row + h * a.out_head;
+    for (int d = 0; d < HD; ++d) from_float(acc[d] / l, o[d]);
+    if (a.lse) a.lse[(size_t)h * a.total + row] = m + logf(l);
+}
+
+// The work of CTA group r (heads apart), longest first: the 256-row tiles of
+// all sequences in the order of their index, the highest first, and of the
+// sequences.  One warp; false if there are no more than r.
+__device__ __forceinline__ bool pk_find_work(const PackedArgs &a, int r, int &first, int &len, int &pair) {
+    const int lane = threadIdx.x & 31;
+    int longest = 0;
+    for (int s = lane; s < a.n_seqs; s += 32) {
+        packed_seq(a, s, first, len);
+        longest = max(longest, (len + 255) >> 8);
+    }
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    // tiles of index t or above, over all sequences
+    auto from = [&](int t) {
+        int n = 0;
+        for (int s = lane; s < a.n_seqs; s += 32) {
+            int f, l;
+            packed_seq(a, s, f, l);
+            n += max(0, ((l + 255) >> 8) - t);
+        }
+        return __reduce_add_sync(0xffffffffu, n);
+    };
+    if (from(0) <= r) return false;
+    int lo = 0, hi = longest;   // from(lo) > r >= from(hi)
+    int above = 0;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1, n = from(mid);
+        if (n > r) lo = mid;
+        else hi = mid, above = n;
+    }
+    pair = lo;
+    int skip = r - above;       // of the sequences with a tile `lo`
+    for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
+        int f = 0, l = 0;
+        if (s0 + lane < a.n_seqs) packed_seq(a, s0 + lane, f, l);
+        const unsigned has = __ballot_sync(0xffffffffu, ((l + 255) >> 8) > lo);
+        const int n = __popc(has);
+        if (skip < n) {
+            const int src = __fns(has, 0, skip + 1);
+            first = __shfl_sync(0xffffffffu, f, src);
+            len = __shfl_sync(0xffffffffu, l, src);
+            return true;
+        }
+        skip -= n;
+    }
+    return false;
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(PK_THREADS, 1)
+packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ CUtensorMap qmap,
+                 const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+    using G = PkGeom<HD>;
+    extern __shared__ uint8_t pk_smem_raw[];
+    __shared__ PkBars B;
+    uint8_t *sq = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(pk_smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t *skv = sq + 2 * G::TILE;
+    const int h = blockIdx.x % a.n_heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (warp == 0) {
+        int first = 0, len = 0, pair = -1;
+        if (!pk_find_work(a, blockIdx.x / a.n_heads, first, len, pair)) pair = -1;
+        if (lane == 0) B.first = first, B.len = len, B.pair = pair;
+        if (pair >= 0) tc_alloc(&B.tmem, PK_TMEM_COLS);
+    } else if (warp == 1 && lane == 0) {
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&B.q_full[t], 1);
+            mbar_init(&B.s_full[t], 1);
+            mbar_init(&B.p_full[t], 128);
+            mbar_init(&B.o_done[t], 1);
+            mbar_init(&B.v_checked[t], 64);
+        }
+        B.bad_from = 0x7fffffff;
+        for (int i = 0; i < PK_STAGES; ++i) {
+            mbar_init(&B.kv_full[i], 1);
+            mbar_init(&B.kv_empty[i], 1);
+        }
+        mbar_init(&B.drain, 1);
+        fence_barrier_init();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (B.pair < 0) return;
+    const int first = B.first, len = B.len, row0 = 256 * B.pair;       // rows of the sequence from row0 on
+    const int n0 = 2 * B.pair + 1, n1 = len > row0 + PK_ROWS ? n0 + 1 : 0;   // key tiles of the two query tiles
+    const int n = max(n0, n1);
+    const uint32_t tmem = B.tmem;
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PK_OTHER_REGS));
+        if (warp == 9 && lane == 0) {
+            // ---- loads: Q_0, K_0, Q_1, V_0, K_1, V_1, ... ----
+            const int kvh = h / a.group;
+            auto load = [&](uint8_t *dst, const CUtensorMap *map, int head, int row, uint64_t *bar) {
+                mbar_arrive_expect_tx(bar, G::TILE);
+#pragma unroll
+                for (int x = 0; x < HD; x += 64) pk_tma_load(dst + x / 64 * (PK_ROWS * 128), map, x, head, row, bar);
+            };
+            load(sq, &qmap, h, first + row0, &B.q_full[0]);
+            int i = 0;
+            bool ok = true;
+            for (; i < 2 * n; ++i) {
+                const int slot = i % PK_STAGES;
+                ok = mbar_wait_bounded(&B.kv_empty[slot], (i / PK_STAGES & 1) ^ 1, a.status, HOLO_E_TIMEOUT);
+                if (!ok) break;
+                load(skv + slot * G::TILE, i & 1 ? &vmap : &kmap, kvh, first + (i >> 1) * PK_ROWS, &B.kv_full[slot]);
+                if (i == 0 && n1) load(sq + G::TILE, &qmap, h, first + row0 + PK_ROWS, &B.q_full[1]);
+            }
+            if (!ok)   // the loads in flight land before the CTA leaves
+                for (int k = max(0, i - PK_STAGES); k < i; ++k)
+                    mbar_wait_bounded(&B.kv_full[k % PK_STAGES], k / PK_STAGES & 1, a.status, HOLO_E_TIMEOUT);
+        } else if (warp == 8 && lane == 0) {
+            // ---- MMAs ----
+            constexpr uint32_t id_s = tc_idesc_f16(PK_ROWS, PK_ROWS) | PkType<T>::AB;
+            constexpr uint32_t id_o = tc_idesc_f16(PK_ROWS, HD) | PkType<T>::AB | 1u << 16;   // B transposed
+            bool ok = true;
+            auto wait = [&](uint64_t *bar, int parity) {
+                ok = ok && mbar_wait_bounded(bar, parity, a.status, HOLO_E_TIMEOUT);
+                tc_fence_after();
+                return ok;
+            };
+            auto wait_kv = [&](int i) { return wait(&B.kv_full[i % PK_STAGES], i / PK_STAGES & 1); };
+            auto scores = [&](int t, int j) {   // S_t = Q_t K_j^T
+                const uint64_t q = sw128_desc(sq + t * G::TILE), k = sw128_desc(skv + 2 * j % PK_STAGES * G::TILE);
+#pragma unroll
+                for (int s = 0; s < HD / 16; ++s) {
+                    const uint64_t off = (uint64_t)(((s >> 2) * (PK_ROWS * 128) + (s & 3) * 32) >> 4);
+                    tc_mma(tmem + t * 128, q + off, k + off, id_s, s > 0);
+                }
+                tc_commit(&B.s_full[t]);
+            };
+            if (wait(&B.q_full[0], 0) && wait_kv(0)) scores(0, 0);
+            if (n1 && wait(&B.q_full[1], 0)) scores(1, 0);
+            if (ok) tc_commit(&B.kv_empty[0]);
+            for (int j = 0; j < n && ok; ++j) {
+                wait_kv(2 * j + 1);
+#pragma unroll 1
+                for (int t = 0; t < 2; ++t) {
+                    const int nt = t ? n1 : n0;
+                    if (j >= nt) continue;
+                    if (j >= n0 - 1) wait(&B.v_checked[j - (n0 - 1)], 0);
+                    if (!wait(&B.p_full[t], j & 1)) break;
+                    const uint64_t v = pk_desc_mn(skv + (2 * j + 1) % PK_STAGES * G::TILE);
+#pragma unroll
+                    for (int s = 0; s < PK_ROWS / 16; ++s)   // 16 keys: 8 columns of P, 16 rows of V
+                        tc_mma_ts(tmem + 256 + t * 128, tmem + t * 128 + 8 * s, v + (uint64_t)(s * 2048 >> 4), id_o,
+                                  j > 0 || s > 0);
+                    tc_commit(&B.o_done[t]);
+                    if (t == 1 || !n1) tc_commit(&B.kv_empty[(2 * j + 1) % PK_STAGES]);
+                    if (j + 1 < nt) {
+                        // P_t and the next S_t share columns: P_t has been read first
+                        if (!wait_kv(2 * j + 2) || !wait(&B.o_done[t], j & 1)) break;
+                        scores(t, j + 1);
+                    }
+                    if ((t == 1 || !n1) && j + 1 < n) tc_commit(&B.kv_empty[(2 * j + 2) % PK_STAGES]);
+                }
+            }
+            if (!ok) {   // the MMAs in flight end before the CTA leaves
+                tc_commit(&B.drain);
+                mbar_wait_bounded(&B.drain, 0, a.status, HOLO_E_TIMEOUT);
+            }
+        }
+        if (warp >= 10) {
+            // ---- diagonal tiles of V: no value that is not finite in a masked place ----
+            for (int j = n0 - 1; j < n; ++j) {
+                const int i = 2 * j + 1;
+                const bool ok = mbar_wait_bounded(&B.kv_full[i % PK_STAGES], i / PK_STAGES & 1, a.status, HOLO_E_TIMEOUT);
+                uint4 *tile = reinterpret_cast<uint4 *>(skv + i % PK_STAGES * G::TILE);
+                for (int e = threadIdx.x - 320; e < G::TILE / 16 && ok; e += 64) {
+                    uint4 w = tile[e];
+                    constexpr uint32_t X = PkType<T>::EXPONENT;
+                    const uint32_t b[4] = {__vcmpeq2(w.x & X, X), __vcmpeq2(w.y & X, X), __vcmpeq2(w.z & X, X),
+                                           __vcmpeq2(w.w & X, X)};
+                    if (b[0] | b[1] | b[2] | b[3]) {
+                        tile[e] = make_uint4(w.x & ~b[0], w.y & ~b[1], w.z & ~b[2], w.w & ~b[3]);
+                        const int key = j * PK_ROWS + (e & (PK_ROWS * 8 - 1)) / 8;   // 8 pieces of 16 bytes a key
+                        if (key < len) atomicMin(&B.bad_from, key);
+                    }
+                }
+                holo_mv::fence_proxy_async_smem();
+                mbar_arrive(&B.v_checked[j - (n0 - 1)]);
+            }
+        }
+        __syncwarp();
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PK_SOFTMAX_REGS));
+        const int t = warp >> 2, r = threadIdx.x & 127, nt = t ? n1 : n0;   // tile, row of the tile
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        const uint32_t ts = tmem + t * 128 + lanes, to = tmem + 256 + t * 128 + lanes;
+        const float c = a.scale * 1.4426950408889634f;
+        float m = -INFINITY;   // log2 of what P is scaled by
+        float l = 0.0f;
+        bool ok = true;
+        for (int j = 0; j < nt; ++j) {
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&B.s_full[t], j & 1, a.status, HOLO_E_TIMEOUT));
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t s[2][64];
+            tc_ld64(ts, s[0]);
+            tc_ld64(ts + 64, s[1]);
+            if (j == nt - 1) {   // the diagonal: row r sees keys 0 .. r of the tile
+#pragma unroll
+                for (int i = 0; i < 128; ++i)
+                    if (i > r) s[i >> 6][i & 63] = 0xff800000u;
+            }
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int i = 0; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(s[i >> 6][i & 63]));
+            const float mn = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c);
+            const bool grow = mn > m + PK_GROWTH;
+            if (j == 0) {
+                m = mn;
+            } else if (__any_sync(0xffffffffu, grow)) {
+                const float fix = grow ? pk_ex2(m - mn) : 1.0f;
+                if (grow) m = mn;
+                l *= fix;
+                ok = __all_sync(0xffffffffu, mbar_wait_bounded(&B.o_done[t], (j - 1) & 1, a.status, HOLO_E_TIMEOUT));
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll 1
+                for (int cb = 0; cb < HD; cb += 32) {
+                    uint32_t o[32];
+                    tc_ld32(to + cb, o);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fix);
+                    tc_st32(to + cb, o);
+                }
+            }
+            const float sub = m == -INFINITY ? 0.0f : m;   // nothing but -inf so far: weights 0
+            const uint64_t c2 = pk_pair(c, c), sub2 = pk_pair(-sub, -sub);
+            uint64_t sum[2] = {0, 0};
+            uint32_t p[64];
+#pragma unroll
+            for (int i = 0; i < 64; ++i) {
+                float x, y;
+                pk_split(pk_fma2(pk_pair(__uint_as_float(s[i >> 5][2 * i & 63]), __uint_as_float(s[i >> 5][(2 * i + 1) & 63])), c2,
+                                 sub2), x, y);
+                x = pk_ex2(x);
+                y = pk_ex2(y);
+                sum[i & 1] = pk_add2(sum[i & 1], pk_pair(x, y));
+                p[i] = PkType<T>::pack(x, y);
+            }
+            tc_st32(ts, p);
+            tc_st32(ts + 32, p + 32);
+            float x, y;
+            pk_split(pk_add2(sum[0], sum[1]), x, y);
+            l += x + y;
+            tc_fence_before();
+            mbar_arrive(&B.p_full[t]);
+        }
+        // ---- O_t / l to the rows ----
+        if (nt > 0 && ok) {
+            ok = mbar_wait_bounded(&B.o_done[t], (nt - 1) & 1, a.status, HOLO_E_TIMEOUT);
+            for (int i = 0; i < nt - (n0 - 1) && ok; ++i)
+                ok = mbar_wait_bounded(&B.v_checked[i], 0, a.status, HOLO_E_TIMEOUT);
+            ok = __all_sync(0xffffffffu, ok);
+        }
+        if (nt > 0 && ok) {
+            tc_fence_after();
+            const int i = row0 + t * PK_ROWS + r, row = first + i;
+            const bool mine = i < len;
+            const float inv = 1.0f / l;
+            T *o = (T *)a.out + (mine ? row * a.out_row : 0) + h * a.out_head;
+            bool finite = i < B.bad_from;
+#pragma unroll
+            for (int cb = 0; cb < HD; cb += 32) {
+                uint32_t v[32];
+                tc_ld32(to + cb, v);
+#pragma unroll
+                for (int k = 0; k < 32; k += 8) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float x = __uint_as_float(v[k + 2 * e]) * inv, y = __uint_as_float(v[k + 2 * e + 1]) * inv;
+                        finite = finite && isfinite(x) && isfinite(y);
+                        w[e] = PkType<T>::pack(x, y);
+                    }
+                    if (mine) *reinterpret_cast<uint4 *>(o + cb + k) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            if (mine) {
+                if (!finite) pk_row_alone<T, HD>(a, row, first, h);
+                else if (a.lse) a.lse[(size_t)h * a.total + row] = (m + log2f(l)) * 0.6931471805599453f;
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        tc_dealloc(tmem, PK_TMEM_COLS);
+    }
+}
+
+using EncodeTiled = decltype(&cuTensorMapEncodeTiled);
+EncodeTiled encode_tiled() {
+    static std::once_flag once;
+    static EncodeTiled fn = nullptr;
+    std::call_once(once, [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r) == cudaSuccess &&
+            r == cudaDriverEntryPointSuccess)
+            fn = (EncodeTiled)p;
+        cudaGetLastError();
+    });
+    return fn;
+}
+
+// [rows][heads][hd] as boxes of 128 rows of one head, 64 values wide; rows past
+// the end read as zeros.  A stride that one row or head leaves open is any valid one.
+bool make_map(CUtensorMap *map, int type, const void *p, int hd, int heads, int rows, long long row, long long head) {
+    const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)heads, (cuuint64_t)rows};
+    const cuuint64_t strides[2] = {(cuuint64_t)head * 2, (cuuint64_t)row * 2};
+    const cuuint32_t box[3] = {64, 1, PK_ROWS}, one[3] = {1, 1, 1};
+    const CUtensorMapDataType dt = type == HOLO_DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    return encode_tiled()(map, dt, 3, const_cast<void *>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int HD>
+bool launch_tc(const PackedArgs &a, int type, cudaStream_t st) {
+    CUtensorMap qm, km, vm;
+    const int kv = a.n_heads / a.group;
+    if (!make_map(&qm, type, a.q, HD, a.n_heads, a.total, a.q_row, a.q_head) ||
+        !make_map(&km, type, a.k, HD, kv, a.total, a.k_row, a.k_head) ||
+        !make_map(&vm, type, a.v, HD, kv, a.total, a.v_row, a.v_head))
+        return false;
+    static bool configured[16] = {false};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 16 || !configured[dev]) {
+        if (cudaFuncSetAttribute(packed_tc_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (int)PkGeom<HD>::SMEM) != cudaSuccess)
+            return false;
+        if (dev < 16) configured[dev] = true;
+    }
+    // at most this many 256-row tiles over all sequences; a CTA without one leaves
+    const long long pairs = ((long long)a.total + 255LL * a.n_seqs) / 256;
+    const long long grid = pairs * a.n_heads;
+    if (grid > 0x7fffffffLL) return false;
+    packed_tc_kernel<T, HD><<<(unsigned)grid, PK_THREADS, PkGeom<HD>::SMEM, st>>>(a, qm, km, vm);
+    return true;
+}
+
+// whether TMA can address rows of this base and these strides (elements)
+bool tma_rows(const void *p, long long row, long long head) {
+    return (uintptr_t)p % 16 == 0 && row % 8 == 0 && head % 8 == 0 && row < (1LL << 38) && head < (1LL << 38);
+}
+
 }  // namespace
 
 extern "C" int cuda_attention_packed(const holo_packed_desc *d, void *out, const void *q, const void *k, const void *v,
                                      const int *cu_seqlens, float *lse) {
     const char *what = "cuda_attention_packed";
-    if (!holo_dev()) return cuda_last_status();
+    HoloDevice *D = holo_dev();
+    if (!D) return cuda_last_status();
     auto refuse = [&](int code) {
         holo_set_status(code, what);
         return code;
@@ -108,11 +609,20 @@ extern "C" int cuda_attention_packed(const holo_packed_desc *d, void *out, const
     a.k_row = d->k_row ? d->k_row : d->n_kv_heads * hd, a.k_head = d->k_head ? d->k_head : hd;
     a.v_row = d->v_row ? d->v_row : d->n_kv_heads * hd, a.v_head = d->v_head ? d->v_head : hd;
     a.out_row = d->out_row ? d->out_row : d->n_heads * hd, a.out_head = d->out_head ? d->out_head : hd;
+    a.status = D->status;
     if (a.q_row < hd || a.k_row < hd || a.v_row < hd || a.out_row < hd || a.q_head < hd || a.k_head < hd || a.v_head < hd ||
         a.out_head < hd)
         return refuse(HOLO_E_ARG);
     cudaStream_t st = d->stream ? (cudaStream_t)d->stream : holo_stream();
-    if (d->type == HOLO_DT_F16) launch_simple<__half>(a, d->head_dim, st);
-    else launch_simple<__nv_bfloat16>(a, d->head_dim, st);
+    bool done = false;
+    if (hd <= 128 && tma_rows(q, a.q_row, a.q_head) && tma_rows(k, a.k_row, a.k_head) && tma_rows(v, a.v_row, a.v_head) &&
+        tma_rows(out, a.out_row, a.out_head) && encode_tiled()) {
+        if (d->type == HOLO_DT_F16) done = hd == 64 ? launch_tc<__half, 64>(a, d->type, st) : launch_tc<__half, 128>(a, d->type, st);
+        else done = hd == 64 ? launch_tc<__nv_bfloat16, 64>(a, d->type, st) : launch_tc<__nv_bfloat16, 128>(a, d->type, st);
+    }
+    if (!done) {
+        if (d->type == HOLO_DT_F16) launch_simple<__half>(a, d->head_dim, st);
+        else launch_simple<__nv_bfloat16>(a, d->head_dim, st);
+    }
     return holo_check_launch(what) ? HOLO_OK : cuda_last_status();
 }
