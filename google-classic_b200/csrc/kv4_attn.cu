@@ -9,10 +9,11 @@
 //            laid out to match, the 16 taken out of it; the accumulator of
 //            each group of 32 starts at -8 * 2^-24 * sum(q), which makes the codes
 //            signed, and its result is multiplied by the group's scale.
-//   values   Codes of two positions become fp16 (n - 8) with one or and one
-//            subtraction a pair (exact); A: 16 dims, B: the softmax weights of
-//            8 heads times the position's scale of the group, transposed by
-//            movmatrix.
+//   values   A pair of codes is taken from two positions' words, and is an fp16
+//            operand the same way; A: 16 dims, B: the softmax weights of 8 heads
+//            times the position's scale of the group, transposed by movmatrix.
+//            One more MMA with A all -8 * 2^-24 makes the codes signed 16
+//            positions at a time, before the sum could grow by them.
 // Only the weights are rounded (to fp16; for fp32 rows a second fp16 term
 // carries the rest, as for q).  So that they use fp16's range whatever the
 // values' size, they are scaled by a power of two that follows the largest
@@ -35,14 +36,16 @@ constexpr int AT_WARPS = 4, AT_THREADS = 32 * AT_WARPS;
 constexpr int AT_UNIT = 2;                     // blocks of 16 positions a unit
 constexpr int AT_UNIT_POS = AT_UNIT * KV4_BLOCK;
 constexpr int AT_WHOLE = 16;                   // items of up to so many units are not cut
-constexpr float AT_SHIFT = 256.0f;             // weights times scales lie below this
+constexpr float AT_GROWTH = 6.0f;              // log2 of what a maximum may grow by before the sums are rescaled
+constexpr int AT_SHIFT = 8;                    // weights times scales lie below 2 to this and AT_GROWTH: 2^14
 
 template <int HD> struct AtGeom {
     static constexpr int NB = HD / KV4_GROUP;
     static constexpr int BLOCK_BYTES = kv4_block_bytes(HD);
     static constexpr int STAGES = HD == 64 ? 4 : 3;
     static constexpr int RING = AT_WARPS * STAGES * AT_UNIT * BLOCK_BYTES;
-    static constexpr int JOIN = AT_WARPS * KV4_HEADS * HD * 4;
+    static constexpr int ROW = HD + 4;          // floats of a head in the join: its lanes' 16-byte stores spread over all banks
+    static constexpr int JOIN = AT_WARPS * KV4_HEADS * ROW * 4;
     static constexpr int SMEM = RING + JOIN;
     static constexpr int CTAS = HD == 256 ? 1 : 3;   // an SM
     static constexpr int SLOT = KV4_HEADS * (HD + 2);   // floats of a partial result: m and l of the heads, then the outputs
@@ -55,7 +58,8 @@ struct AtArgs {
     const int *seqs;
     int n, n_heads, group, chunks;             // chunks of KV4_HEADS query heads a KV head
     float scale;
-    uint64_t page_magic;                       // ceil(2^32 / page_blocks)
+    uint32_t page_magic;                       // ceil(2^32 / page_blocks); 0 for 1
+    bool wide;                                 // rows of out are 16-byte aligned
     int *counters;
     float *partial;
 };
@@ -65,15 +69,20 @@ __device__ __forceinline__ float at_ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ void at_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+// d = a b + c: pure, so that the compiler may interleave independent ones
+__device__ __forceinline__ void at_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1, float c0, float c1, float c2, float c3) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+__device__ __forceinline__ void at_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    at_mma(d, a0, a1, a2, a3, b0, b1, d[0], d[1], d[2], d[3]);
 }
 __device__ __forceinline__ uint32_t at_transpose(uint32_t x) {
     uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
 __device__ __forceinline__ uint32_t at_pack(float lo, float hi) {
@@ -82,15 +91,6 @@ __device__ __forceinline__ uint32_t at_pack(float lo, float hi) {
     return r;
 }
 __device__ __forceinline__ float2 at_unpack(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2 *>(&x)); }
-// two codes, 0..15 each in a half at bit 0 or 4 (mask), as fp16 code - 8 or 16 (code - 8)
-template <uint32_t MASK, uint32_t BIAS>
-__device__ __forceinline__ uint32_t at_signed(uint32_t x) {
-    uint32_t y;
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(y) : "r"(x), "n"(MASK), "n"(0x64006400u));   // (x & MASK) | 1024.0
-    const uint32_t bias = BIAS;
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&y), *reinterpret_cast<const __half2 *>(&bias));
-    return *reinterpret_cast<const uint32_t *>(&r);
-}
 template <int N> struct AtWords { uint32_t w[N]; };
 template <int N> __device__ __forceinline__ AtWords<N> at_lds(const uint8_t *p) {
     AtWords<N> r;
@@ -109,7 +109,7 @@ struct Walk {
     int i, s, len, units;      // sequence: its place in the list, number, positions, units an item
     int item;                  // KV head * chunks + chunk
     int first, take;           // units of the item in the part
-    long long rest;            // units of the part from `first` on
+    int rest;                  // units of the part from `first` on
 };
 
 __device__ __forceinline__ int at_units(const Kv4View &c, const AtArgs &a, int i, int &s, int &len) {
@@ -122,7 +122,7 @@ __device__ __forceinline__ int at_units(const Kv4View &c, const AtArgs &a, int i
     len = max(0, min(__ldg(c.lens + s), c.max_pages * c.page_tokens));
     return (len + AT_UNIT_POS - 1) / AT_UNIT_POS;
 }
-__device__ __forceinline__ void at_clip(Walk &w) { w.take = (int)min((long long)(w.units - w.first), w.rest); }
+__device__ __forceinline__ void at_clip(Walk &w) { w.take = min(w.units - w.first, w.rest); }
 // the next item of the part; rest 0 at its end
 __device__ __forceinline__ void at_next(const Kv4View &c, const AtArgs &a, Walk &w) {
     w.rest -= w.take;
@@ -142,22 +142,49 @@ __device__ __forceinline__ void at_next(const Kv4View &c, const AtArgs &a, Walk 
 }
 
 // inclusive sum over the CTA
-__device__ __forceinline__ long long at_scan(long long v, long long *sh, long long &total) {
+__device__ __forceinline__ int at_scan(int v, int *sh, int &total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long u = __shfl_up_sync(0xffffffffu, v, o);
+        const int u = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += u;
     }
     __syncthreads();
     if (lane == 31) sh[warp] = v;
     __syncthreads();
     total = 0;
+#pragma unroll
     for (int w = 0; w < AT_WARPS; ++w) {
         if (w < warp) v += sh[w];
         total += sh[w];
     }
     return v;
+}
+
+// The list cut over `ctas` parts: the first `more` of them have one unit more than the others.
+struct Cuts {
+    int size, more;
+    __device__ __forceinline__ int begin(int part) const { return part * size + min(part, more); }
+    __device__ __forceinline__ int part_of(int unit) const {
+        const int big = more * (size + 1);
+        return unit < big ? unit / (size + 1) : more + (unit - big) / size;
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ void at_store4(T *p, bool wide, float x, float y, float z, float w) {
+    if (wide) {
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<float4 *>(p) = make_float4(x, y, z, w);
+        } else {
+            uint2 u;
+            T *h = reinterpret_cast<T *>(&u);
+            h[0] = kv4_from_float<T>(x), h[1] = kv4_from_float<T>(y), h[2] = kv4_from_float<T>(z), h[3] = kv4_from_float<T>(w);
+            *reinterpret_cast<uint2 *>(p) = u;
+        }
+    } else {
+        p[0] = kv4_from_float<T>(x), p[1] = kv4_from_float<T>(y), p[2] = kv4_from_float<T>(z), p[3] = kv4_from_float<T>(w);
+    }
 }
 
 template <typename T, int HD>
@@ -169,10 +196,11 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
     constexpr int TERMS = FINE ? 2 : 1;
     extern __shared__ __align__(128) uint8_t at_smem[];
     __shared__ uint64_t full[AT_WARPS][STAGES];
-    __shared__ long long scan[AT_WARPS];
+    __shared__ int scan[AT_WARPS];
     __shared__ Walk begin;
-    __shared__ long long part_start, part_end;
-    __shared__ float join_m[AT_WARPS][KV4_HEADS], join_l[AT_WARPS][KV4_HEADS];
+    __shared__ int part_start, part_end;
+    __shared__ float join_m[AT_WARPS][KV4_HEADS], join_l[AT_WARPS][KV4_HEADS], join_w[AT_WARPS][KV4_HEADS];
+    __shared__ float join_den[KV4_HEADS];
     __shared__ int last;
     float *join = reinterpret_cast<float *>(at_smem + G::RING);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -181,108 +209,127 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
     if (lane < STAGES) mbar_init(&full[warp][lane], 1);
     fence_barrier_init();
 
+    auto zeros = [&]() {                      // sequences without positions (a number out of range: left alone)
+        for (int i = blockIdx.x; i < a.n; i += gridDim.x) {
+            int s, len;
+            if (at_units(c, a, i, s, len) == 0 && s >= 0)
+                for (int d = 4 * threadIdx.x; d < a.n_heads * HD; d += 4 * AT_THREADS)
+                    at_store4<T>((T *)a.out + i * a.out_row + d, a.wide, 0.0f, 0.0f, 0.0f, 0.0f);
+        }
+    };
+
     // ---- the CTA's part of the list ----
     const int items = c.n_kv * a.chunks;
-    long long all = 0;
+    int all = 0, s0 = -1, len0 = 0, u0 = 0, end0 = 0;   // of thread's sequence in the last step of the sum
     for (int i0 = 0; i0 < a.n; i0 += AT_THREADS) {
         const int i = i0 + threadIdx.x;
-        int s, len, u = 0;
+        u0 = 0, s0 = -1, len0 = 0;
         if (i < a.n) {
-            u = at_units(c, a, i, s, len);
-            if (s < 0 && blockIdx.x == 0) kv4_report(c.status, HOLO_E_ARG);
+            u0 = at_units(c, a, i, s0, len0);
+            if (s0 < 0 && blockIdx.x == 0) kv4_report(c.status, HOLO_E_ARG);
         }
-        long long total;
-        at_scan((long long)u * items, scan, total);
+        int total;
+        end0 = all + at_scan(u0 * items, scan, total);
         all += total;
     }
     // no more CTAs than leave each warp a unit
-    const int ctas = (int)min((long long)gridDim.x, max(1LL, (all + AT_WARPS - 1) / AT_WARPS));
-    // sequences without positions: zeros (a sequence number out of range: left alone)
-    for (int i = blockIdx.x; i < a.n; i += gridDim.x) {
-        int s, len;
-        if (at_units(c, a, i, s, len) == 0 && s >= 0)
-            for (int d = threadIdx.x; d < a.n_heads * HD; d += AT_THREADS)
-                ((T *)a.out)[i * a.out_row + d] = kv4_from_float<T>(0.0f);
+    const int ctas = min((int)gridDim.x, max(1, (all + AT_WARPS - 1) / AT_WARPS));
+    if ((int)blockIdx.x >= ctas) {
+        zeros();
+        return;
     }
-    if ((int)blockIdx.x >= ctas) return;
-    // Its part [u0, u1): the even cuts of the list, moved down to the item's start
+    // Its part: the even cuts of the list, moved down to the item's start
     // where the item is short.  Cuts inside longer items stay, so that the parts that an item spans follow from them.
-    const long long cut0 = all * blockIdx.x / ctas, cut1 = all * (blockIdx.x + 1) / ctas;
-    if (threadIdx.x == 0) part_end = all;
+    const Cuts cuts = {all / ctas, all % ctas};
+    const int cut0 = cuts.begin(blockIdx.x), cut1 = cuts.begin(blockIdx.x + 1);
+    if (threadIdx.x == 0) part_start = 0, part_end = blockIdx.x + 1 == ctas ? all : 0;
+    __syncthreads();
     {
-        long long before = 0;
+        int before = 0;
         for (int i0 = 0; i0 < a.n && before <= cut1; i0 += AT_THREADS) {
-            const int i = i0 + threadIdx.x;
-            int s = -1, len = 0, u = 0;
-            if (i < a.n) u = at_units(c, a, i, s, len);
-            long long total;
-            const long long end = before + at_scan((long long)u * items, scan, total), start = end - (long long)u * items;
-            if (start <= cut0 && cut0 < end) {
-                Walk w;
-                w.i = i, w.s = s, w.len = len, w.units = u;
-                w.item = (int)((cut0 - start) / u);
-                w.first = u > AT_WHOLE ? (int)((cut0 - start) % u) : 0;
-                begin = w;
-                part_start = start + (long long)w.item * u + w.first;
+            if (a.n > AT_THREADS) {           // else as the sum left it
+                const int i = i0 + threadIdx.x;
+                u0 = 0, s0 = -1, len0 = 0;
+                if (i < a.n) u0 = at_units(c, a, i, s0, len0);
+                int total;
+                end0 = before + at_scan(u0 * items, scan, total);
+                before += total;
             }
-            if (start <= cut1 && cut1 < end) part_end = u > AT_WHOLE ? cut1 : start + (cut1 - start) / u * u;
-            before += total;
+            const int start = end0 - u0 * items;
+            if (start <= cut0 && cut0 < end0) {
+                Walk w;
+                w.i = i0 + threadIdx.x, w.s = s0, w.len = len0, w.units = u0;
+                w.item = (cut0 - start) / u0;
+                w.first = u0 > AT_WHOLE ? cut0 - start - w.item * u0 : 0;
+                begin = w;
+                part_start = start + w.item * u0 + w.first;
+            }
+            if (start <= cut1 && cut1 < end0) part_end = u0 > AT_WHOLE ? cut1 : start + (cut1 - start) / u0 * u0;
         }
         __syncthreads();
     }
-    const long long u0 = part_start, u1 = part_end;
-    if (u0 >= u1) return;
+    const int from = part_start, to = part_end;
+    if (from >= to) {
+        zeros();
+        return;
+    }
     Walk head = begin;
-    head.rest = u1 - u0;
+    head.rest = to - from;
     at_clip(head);
 
     // ---- the warp's loads: unit `unit` of item `load` ----
     Walk load = head;
     int unit = load.first + warp;
-    auto settle = [&]() {                     // to the next unit that there is
+    const uint8_t *load_base = nullptr;       // of the KV head
+    const int *load_table = nullptr;
+    const uint32_t page_bytes = (uint32_t)c.n_kv * c.page_blocks * G::BLOCK_BYTES;
+    auto settle = [&]() {                     // to the next unit that there is, and its item
         while (load.rest > 0 && unit >= load.first + load.take) {
             at_next(c, a, load);
             unit = load.first + warp;
         }
+        load_base = c.pool + (uint32_t)(load.item / a.chunks * c.page_blocks * G::BLOCK_BYTES);
+        load_table = c.tables + (size_t)max(0, load.s) * c.max_pages;
     };
     settle();
-    int entry = -1;                           // lanes 0 and 1: the page of their block of it
-    int block = 0;                            // and the block in the sequence
+    int entry = -1, in_page = 0;              // lanes 0 and 1: the page of their block of it, and the block there
     auto look_up = [&]() {
-        block = unit * AT_UNIT + lane;
-        if (load.rest > 0 && lane < AT_UNIT && block * KV4_BLOCK < load.len)
-            entry = __ldg(c.tables + (size_t)load.s * c.max_pages + (int)((block * a.page_magic) >> 32));
+        const int block = unit * AT_UNIT + lane;
+        if (load.rest > 0 && lane < AT_UNIT && block * KV4_BLOCK < load.len) {
+            const int col = a.page_magic ? (int)__umulhi((uint32_t)block, a.page_magic) : block;
+            in_page = block - col * c.page_blocks;
+            entry = __ldg(load_table + col);
+        }
     };
     look_up();
-    int issued = 0;
+    int issued = 0, fill = 0;                 // copies issued, the slot of the next one
     auto issue = [&]() {                      // its copies, and the table entries of the next one
         if (load.rest <= 0) return;
-        const int slot = issued % STAGES;
         const int blocks = min(AT_UNIT, (load.len - unit * AT_UNIT_POS + KV4_BLOCK - 1) / KV4_BLOCK);
-        if (lane == 0) mbar_arrive_expect_tx(&full[warp][slot], blocks * G::BLOCK_BYTES);
+        if (lane == 0) mbar_arrive_expect_tx(&full[warp][fill], blocks * G::BLOCK_BYTES);
         __syncwarp();
         if (lane < blocks) {
-            if (entry < 0 || entry >= c.n_pages) {
+            if ((uint32_t)entry >= (uint32_t)c.n_pages) {
                 kv4_report(c.status, HOLO_E_ARG);
                 entry = 0;
             }
-            const int in_page = block - (int)((block * a.page_magic) >> 32) * c.page_blocks;
-            const uint8_t *src = kv4_block(c, HD, entry, load.item / a.chunks, in_page);
             asm volatile(
                 "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                :: "r"(smem_addr(ring + (slot * AT_UNIT + lane) * G::BLOCK_BYTES)), "l"(src), "r"(G::BLOCK_BYTES),
-                   "r"(smem_addr(&full[warp][slot])) : "memory");
+                :: "r"(smem_addr(ring + (fill * AT_UNIT + lane) * G::BLOCK_BYTES)),
+                   "l"(load_base + (size_t)(uint32_t)entry * page_bytes + in_page * G::BLOCK_BYTES), "r"(G::BLOCK_BYTES),
+                   "r"(smem_addr(&full[warp][fill])) : "memory");
         }
         ++issued;
+        fill = fill + 1 == STAGES ? 0 : fill + 1;
         unit += AT_WARPS;
-        settle();
+        if (unit >= load.first + load.take) settle();
         look_up();
     };
     __syncwarp();
     for (int k = 0; k < STAGES; ++k) issue();
 
     // ---- items ----
-    int used = 0;
+    int used = 0, slot = 0, phase = 0;        // units taken, the slot of the next one and its barrier's phase
     bool ok = true;
     for (Walk w = head; w.rest > 0; at_next(c, a, w)) {
         const int kvh = w.item / a.chunks, head0 = kvh * a.group + (w.item % a.chunks) * KV4_HEADS;
@@ -348,75 +395,99 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
         int power = -32;                      // of two: the largest |value scale| lies below it
 
         for (int u = w.first + warp; u < w.first + w.take; u += AT_WARPS) {
-            const int slot = used % STAGES;
-            ok = ok && mbar_wait_bounded(&full[warp][slot], used / STAGES & 1, c.status, HOLO_E_TIMEOUT);
+            ok = ok && mbar_wait_bounded(&full[warp][slot], phase, c.status, HOLO_E_TIMEOUT);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            ++used;
             const uint8_t *buf = ring + slot * AT_UNIT * G::BLOCK_BYTES;
+            ++used;
+            if (++slot == STAGES) slot = 0, phase ^= 1;
             const int left = w.len - u * AT_UNIT_POS;   // positions of the sequence from the unit's first on
+            const bool tail = left < AT_UNIT_POS;
             // scores of positions g, g + 8 (+ 16 a block), heads 2 t and 2 t + 1
             float s[AT_UNIT][4];
             AtWords<NB / 2> dv[AT_UNIT][2];
-            uint32_t dmax = 0;
+            __half2 dmax = __float2half2_rn(0.0f);
 #pragma unroll
             for (int k = 0; k < AT_UNIT; ++k) {
                 const uint8_t *blk = buf + k * G::BLOCK_BYTES;
-                const bool live[2] = {16 * k + g < left, 16 * k + g + 8 < left};
                 const AtWords<NB> w0 = at_lds<NB>(blk + g * (HD / 2) + t * 4 * NB);
                 const AtWords<NB> w1 = at_lds<NB>(blk + (g + 8) * (HD / 2) + t * 4 * NB);
                 const AtWords<NB / 2> d0 = at_lds<NB / 2>(blk + kv4_off_dk(HD) + g * 2 * NB);
                 const AtWords<NB / 2> d1 = at_lds<NB / 2>(blk + kv4_off_dk(HD) + (g + 8) * 2 * NB);
                 dv[k][0] = at_lds<NB / 2>(blk + kv4_off_dv(HD) + g * 2 * NB);
                 dv[k][1] = at_lds<NB / 2>(blk + kv4_off_dv(HD) + (g + 8) * 2 * NB);
-                float r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                float acc[NB][4];
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    float acc[4] = {start[b][0], start[b][1], start[b][0], start[b][1]};
-                    const uint32_t x = w0.w[b], y = w1.w[b], x8 = x >> 8, y8 = y >> 8;
+                for (int b = 0; b < NB; ++b)
+                    at_mma(acc[b], w0.w[b] & 0x000f000fu, w1.w[b] & 0x000f000fu, w0.w[b] >> 8 & 0x000f000fu,
+                           w1.w[b] >> 8 & 0x000f000fu, qf[0][b][0][0], qf[0][b][0][1], start[b][0], start[b][1], start[b][0],
+                           start[b][1]);
 #pragma unroll
-                    for (int f = 0; f < TERMS; ++f) {
-                        at_mma(acc, x & 0x000f000fu, y & 0x000f000fu, x8 & 0x000f000fu, y8 & 0x000f000fu, qf[f][b][0][0],
-                               qf[f][b][0][1]);
-                        at_mma(acc, x & 0x00f000f0u, y & 0x00f000f0u, x8 & 0x00f000f0u, y8 & 0x00f000f0u, qf[f][b][1][0],
-                               qf[f][b][1][1]);
-                    }
-                    const float2 e0 = at_unpack(d0.w[b >> 1]), e1 = at_unpack(d1.w[b >> 1]);
-                    const float s0 = b & 1 ? e0.y : e0.x, s1 = b & 1 ? e1.y : e1.x;
-                    r[0] = fmaf(s0, acc[0], r[0]);
-                    r[1] = fmaf(s0, acc[1], r[1]);
-                    r[2] = fmaf(s1, acc[2], r[2]);
-                    r[3] = fmaf(s1, acc[3], r[3]);
+                for (int b = 0; b < NB; ++b)
+                    at_mma(acc[b], w0.w[b] & 0x00f000f0u, w1.w[b] & 0x00f000f0u, w0.w[b] >> 8 & 0x00f000f0u,
+                           w1.w[b] >> 8 & 0x00f000f0u, qf[0][b][1][0], qf[0][b][1][1]);
+                if (FINE) {
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+                        at_mma(acc[b], w0.w[b] & 0x000f000fu, w1.w[b] & 0x000f000fu, w0.w[b] >> 8 & 0x000f000fu,
+                               w1.w[b] >> 8 & 0x000f000fu, qf[TERMS - 1][b][0][0], qf[TERMS - 1][b][0][1]);
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+                        at_mma(acc[b], w0.w[b] & 0x00f000f0u, w1.w[b] & 0x00f000f0u, w0.w[b] >> 8 & 0x00f000f0u,
+                               w1.w[b] >> 8 & 0x00f000f0u, qf[TERMS - 1][b][1][0], qf[TERMS - 1][b][1][1]);
                 }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[k][e] = live[e >> 1] ? r[e] * factor[e & 1] : -INFINITY;
+                for (int e = 0; e < 4; ++e) s[k][e] = 0.0f;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    const float2 e0 = at_unpack(d0.w[b >> 1]), e1 = at_unpack(d1.w[b >> 1]);
+                    const float s0 = b & 1 ? e0.y : e0.x, s1 = b & 1 ? e1.y : e1.x;
+                    s[k][0] = fmaf(s0, acc[b][0], s[k][0]);
+                    s[k][1] = fmaf(s0, acc[b][1], s[k][1]);
+                    s[k][2] = fmaf(s1, acc[b][2], s[k][2]);
+                    s[k][3] = fmaf(s1, acc[b][3], s[k][3]);
+                }
+                if (tail) {                   // past the end: weight 0, whatever lies there
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+                        if (16 * k + g + 8 * x >= left) {
+                            s[k][2 * x] = s[k][2 * x + 1] = -INFINITY;
+#pragma unroll
+                            for (int i = 0; i < NB / 2; ++i) dv[k][x].w[i] = 0;
+                        }
+                }
 #pragma unroll
                 for (int x = 0; x < 2; ++x)
 #pragma unroll
-                    for (int i = 0; i < NB / 2; ++i) {
-                        if (!live[x]) dv[k][x].w[i] = 0;   // whatever lies there
-                        dmax = __vmaxu2(dmax, dv[k][x].w[i] & 0x7fff7fffu);
-                    }
+                    for (int i = 0; i < NB / 2; ++i)
+                        dmax = __hmax2(dmax, __habs2(*reinterpret_cast<const __half2 *>(&dv[k][x].w[i])));
             }
-            // maxima of the unit, over positions (and of the scales, over all)
+            // Maxima of the lane's positions, and of the scales.  Only where one has grown by more than
+            // AT_GROWTH (a scale: by a power of two) is the warp's maximum taken and the sums rescaled.
             float mn[2];
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                mn[x] = fmaxf(fmaxf(s[0][x], s[0][x + 2]), fmaxf(s[1][x], s[1][x + 2]));
+                mn[x] = fmaxf(s[0][x], s[0][x + 2]);
 #pragma unroll
-                for (int i = 4; i < 32; i <<= 1) mn[x] = fmaxf(mn[x], __shfl_xor_sync(0xffffffffu, mn[x], i));
-                mn[x] = fmaxf(mn[x], m[x]);
+                for (int k = 1; k < AT_UNIT; ++k) mn[x] = fmaxf(mn[x], fmaxf(s[k][x], s[k][x + 2]));
+                mn[x] *= factor[x];
             }
-            const uint32_t big = __reduce_max_sync(0xffffffffu, max(dmax & 0xffffu, dmax >> 16));
-            const int pn = max(power, (int)(big >> 10) - 14);   // fp16 exponent field e: below 2^(e - 14)
-            if (__any_sync(0xffffffffu, mn[0] > m[0] || mn[1] > m[1]) || pn > power) {
+            const uint32_t big = (uint32_t)__half_as_ushort(__hmax(__low2half(dmax), __high2half(dmax)));
+            if (__any_sync(0xffffffffu, mn[0] > m[0] + AT_GROWTH || mn[1] > m[1] + AT_GROWTH || (int)(big >> 10) - 14 > power)) {
+#pragma unroll
+                for (int i = 4; i < 32; i <<= 1) {
+                    mn[0] = fmaxf(mn[0], __shfl_xor_sync(0xffffffffu, mn[0], i));
+                    mn[1] = fmaxf(mn[1], __shfl_xor_sync(0xffffffffu, mn[1], i));
+                }
+                // fp16 exponent field e: below 2^(e - 14)
+                const int pn = max(power, (int)(__reduce_max_sync(0xffffffffu, big) >> 10) - 14);
                 const float lower = __uint_as_float((uint32_t)(127 + power - pn) << 23);   // 2^(power - pn)
                 float fix[2];
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    fix[x] = mn[x] > m[x] ? at_ex2(m[x] - mn[x]) : 1.0f;
+                    mn[x] = fmaxf(ceilf(mn[x]), m[x]);   // whole: rescaling is exact
+                    fix[x] = (mn[x] > m[x] ? at_ex2(m[x] - mn[x]) : 1.0f) * lower;
                     l[x] *= fix[x];
-                    fix[x] *= lower;
                     m[x] = mn[x];
                 }
                 power = pn;
@@ -427,10 +498,10 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
 #pragma unroll
                         for (int e = 0; e < 4; ++e) o[b][x][e] *= fix[e & 1];
             }
-            const float unit_scale = __uint_as_float((uint32_t)(127 - power) << 23) * AT_SHIFT;
+            // weights 2^(s - m) times 2^(AT_SHIFT - power)
             float sub[2];
 #pragma unroll
-            for (int x = 0; x < 2; ++x) sub[x] = m[x] == -INFINITY ? 0.0f : m[x];
+            for (int x = 0; x < 2; ++x) sub[x] = (m[x] == -INFINITY ? 0.0f : m[x]) + (float)(power - AT_SHIFT);
 #pragma unroll
             for (int k = 0; k < AT_UNIT; ++k) {
                 const uint8_t *blk = buf + k * G::BLOCK_BYTES;
@@ -438,7 +509,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
                 float p[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    p[e] = at_ex2(s[k][e] - sub[e & 1]);
+                    p[e] = at_ex2(fmaf(s[k][e], factor[e & 1], -sub[e & 1]));
                     l[e & 1] += p[e];
                 }
                 // codes of positions 2 t, 2 t + 1 and 2 t + 8, 2 t + 9, values 4 g .. 4 g + 3 of every group
@@ -447,7 +518,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
                     const float2 e0 = at_unpack(dv[k][0].w[b >> 1]), e1 = at_unpack(dv[k][1].w[b >> 1]);
-                    const float s0 = (b & 1 ? e0.y : e0.x) * unit_scale, s1 = (b & 1 ? e1.y : e1.x) * unit_scale;
+                    const float s0 = b & 1 ? e0.y : e0.x, s1 = b & 1 ? e1.y : e1.x;
                     float y[4] = {p[0] * s0, p[1] * s0, p[2] * s1, p[3] * s1};
                     uint32_t pf[TERMS][2];
 #pragma unroll
@@ -460,18 +531,21 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
                             y[0] -= a0.x, y[1] -= a0.y, y[2] -= a1.x, y[3] -= a1.y;
                         }
                     }
-                    constexpr uint32_t LOW = 0x5410, HIGH = 0x7632;
-                    const uint32_t pick = b & 1 ? HIGH : LOW;
+                    const uint32_t pick = b & 1 ? 0x7632u : 0x5410u;
                     const uint32_t x0 = __byte_perm(v0.w[b >> 1], v0.w[NB / 2 + (b >> 1)], pick);
                     const uint32_t x1 = __byte_perm(v1.w[b >> 1], v1.w[NB / 2 + (b >> 1)], pick);
+                    // rows g and g + 8: codes 2 x and, 16 times as large, 2 x + 1; then -8 of each
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const uint32_t z0 = x0 >> (8 * x), z1 = x1 >> (8 * x);
-                        const uint32_t a0 = at_signed<0x000f000fu, 0x64086408u>(z0), a1 = at_signed<0x00f000f0u, 0x64806480u>(z0);
-                        const uint32_t a2 = at_signed<0x000f000fu, 0x64086408u>(z1), a3 = at_signed<0x00f000f0u, 0x64806480u>(z1);
+                    for (int x = 0; x < 2; ++x)
 #pragma unroll
-                        for (int f = 0; f < TERMS; ++f) at_mma(o[b][x], a0, a1, a2, a3, pf[f][0], pf[f][1]);
-                    }
+                        for (int f = 0; f < TERMS; ++f)
+                            at_mma(o[b][x], x0 >> (8 * x) & 0x000f000fu, x0 >> (8 * x) & 0x00f000f0u,
+                                   x1 >> (8 * x) & 0x000f000fu, x1 >> (8 * x) & 0x00f000f0u, pf[f][0], pf[f][1]);
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+#pragma unroll
+                        for (int f = 0; f < TERMS; ++f)
+                            at_mma(o[b][x], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, pf[f][0], pf[f][1]);
                 }
             }
             __syncwarp();                     // the slot has been read
@@ -483,74 +557,93 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
         for (int x = 0; x < 2; ++x)
 #pragma unroll
             for (int i = 4; i < 32; i <<= 1) l[x] += __shfl_xor_sync(0xffffffffu, l[x], i);
+        // l and o hold 2^(AT_SHIFT - power) too; o's codes 2^-24, odd ones 16 times as large
+        const float scaled = (float)(AT_SHIFT - power);
         if (g == 0) {
-            join_m[warp][2 * t] = m[0], join_m[warp][2 * t + 1] = m[1];
+            join_m[warp][2 * t] = m[0] - scaled, join_m[warp][2 * t + 1] = m[1] - scaled;
             join_l[warp][2 * t] = l[0], join_l[warp][2 * t + 1] = l[1];
         }
-        const float back = __uint_as_float((uint32_t)(127 + power) << 23) / AT_SHIFT;
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)   // values 32 b + 4 g + 2 x (and + 1, 16 times as large), heads 2 t + (e & 1)
-                    join[(warp * KV4_HEADS + 2 * t + (e & 1)) * HD + 32 * b + 4 * g + 2 * x + (e >> 1)] =
-                        o[b][x][e] * (e & 2 ? back * 0.0625f : back);
+            for (int e = 0; e < 2; ++e)       // values 32 b + 4 g .. + 3 of head 2 t + e
+                *reinterpret_cast<float4 *>(join + (warp * KV4_HEADS + 2 * t + e) * G::ROW + 32 * b + 4 * g) =
+                    make_float4(o[b][0][e] * 16777216.0f, o[b][0][e + 2] * 1048576.0f, o[b][1][e] * 16777216.0f,
+                                o[b][1][e + 2] * 1048576.0f);
         __syncthreads();
         const bool whole = w.first == 0 && w.take == w.units;
-        const int slot0 = w.first > 0 ? 0 : 1;
-        float *mine = a.partial + ((size_t)blockIdx.x * 2 + slot0) * G::SLOT;
-        for (int d = threadIdx.x; d < heads * HD; d += AT_THREADS) {
-            const int h = d / HD;
-            float top = -INFINITY, sum = 0.0f, den = 0.0f;
+        float *mine = a.partial + ((size_t)blockIdx.x * 2 + (w.first > 0 ? 0 : 1)) * G::SLOT;
+        if (threadIdx.x < KV4_HEADS) {
+            const int h = threadIdx.x;
+            float top = -INFINITY, den = 0.0f;
 #pragma unroll
             for (int i = 0; i < AT_WARPS; ++i)
                 if (join_l[i][h] != 0.0f) top = fmaxf(top, join_m[i][h]);
 #pragma unroll
-            for (int i = 0; i < AT_WARPS; ++i)
-                if (join_l[i][h] != 0.0f) {
-                    const float f = at_ex2(join_m[i][h] - top);
-                    sum = fmaf(join[(i * KV4_HEADS + h) * HD + d % HD], f, sum);
-                    den = fmaf(join_l[i][h], f, den);
-                }
+            for (int i = 0; i < AT_WARPS; ++i) {
+                const float f = join_l[i][h] != 0.0f ? at_ex2(join_m[i][h] - top) : 0.0f;
+                join_w[i][h] = f;
+                den = fmaf(join_l[i][h], f, den);
+            }
+            join_den[h] = den;
+            if (!whole) mine[2 * h] = top, mine[2 * h + 1] = den;
+        }
+        __syncthreads();
+        T *out = (T *)a.out + w.i * a.out_row + (long long)head0 * HD;
+        for (int d = 4 * threadIdx.x; d < heads * HD; d += 4 * AT_THREADS) {
+            const int h = d / HD;
+            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int i = 0; i < AT_WARPS; ++i) {
+                const float4 v = *reinterpret_cast<const float4 *>(join + (i * KV4_HEADS + h) * G::ROW + d % HD);
+                const float f = join_w[i][h];
+                sum.x = fmaf(v.x, f, sum.x), sum.y = fmaf(v.y, f, sum.y), sum.z = fmaf(v.z, f, sum.z), sum.w = fmaf(v.w, f, sum.w);
+            }
             if (whole) {
-                ((T *)a.out)[w.i * a.out_row + (long long)(head0 + h) * HD + d % HD] = kv4_from_float<T>(sum / den);
+                const float den = join_den[h];
+                at_store4<T>(out + d, a.wide, sum.x / den, sum.y / den, sum.z / den, sum.w / den);
             } else {
-                mine[2 * KV4_HEADS + d] = sum;
-                if (d % HD == 0) mine[2 * h] = top, mine[2 * h + 1] = den;
+                *reinterpret_cast<float4 *>(mine + 2 * KV4_HEADS + d) = sum;
             }
         }
         if (!whole) {
-            // the item's units lie in the parts of CTAs c0 .. c1: part k holds unit u where k = ((u + 1) * ctas - 1) / all
-            const long long begins = (w.first > 0 ? u0 - w.first : u1 - w.rest);
-            const int c0 = (int)(((begins + 1) * ctas - 1) / all), c1 = (int)(((begins + w.units) * ctas - 1) / all);
+            // the item's units lie in parts p0 .. p1; the last part to come joins their results, in order
+            const int begins = w.first > 0 ? from - w.first : to - w.rest;
+            const int p0 = cuts.part_of(begins), p1 = cuts.part_of(begins + w.units - 1);
             int *counter = a.counters + (size_t)w.i * items + w.item;
             __threadfence();
             __syncthreads();
-            if (threadIdx.x == 0) last = atomicAdd(counter, 1) == c1 - c0;
+            if (threadIdx.x == 0) last = atomicAdd(counter, 1) == p1 - p0;
             __syncthreads();
             if (last) {
                 __threadfence();
                 if (threadIdx.x == 0) *counter = 0;
-                for (int d = threadIdx.x; d < heads * HD; d += AT_THREADS) {
-                    const int h = d / HD;
-                    float top = -INFINITY, sum = 0.0f, den = 0.0f;
-                    for (int k = c0; k <= c1; ++k) {
-                        const float *p = a.partial + ((size_t)k * 2 + (k == c0 ? 1 : 0)) * G::SLOT;
-                        const float pm = __ldcg(p + 2 * h), pl = __ldcg(p + 2 * h + 1), po = __ldcg(p + 2 * KV4_HEADS + d);
-                        if (pl != 0.0f) {
-                            const float mx = fmaxf(top, pm), f = at_ex2(pm - mx), fo = sum == 0.0f && den == 0.0f ? 0.0f : at_ex2(top - mx);
-                            sum = fmaf(po, f, sum * fo);
-                            den = fmaf(pl, f, den * fo);
-                            top = mx;
-                        }
+                const float *part = a.partial + ((size_t)p0 * 2 + 1) * G::SLOT;   // then every second one, one less
+                auto at = [&](int k) { return part + (size_t)(k ? 2 * k - 1 : 0) * G::SLOT; };
+                for (int d = 4 * threadIdx.x; d < heads * HD; d += 4 * AT_THREADS) {
+                    const int h = d / HD, n = p1 - p0 + 1;
+                    float top = -INFINITY, den = 0.0f;
+#pragma unroll 8
+                    for (int k = 0; k < n; ++k) {
+                        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(at(k)) + h);
+                        if (ml.y != 0.0f) top = fmaxf(top, ml.x);
                     }
-                    ((T *)a.out)[w.i * a.out_row + (long long)(head0 + h) * HD + d % HD] = kv4_from_float<T>(sum / den);
+                    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+                    for (int k = 0; k < n; ++k) {
+                        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(at(k)) + h);
+                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(at(k) + 2 * KV4_HEADS + d));
+                        const float f = ml.y != 0.0f ? at_ex2(ml.x - top) : 0.0f;
+                        den = fmaf(ml.y, f, den);
+                        sum.x = fmaf(v.x, f, sum.x), sum.y = fmaf(v.y, f, sum.y), sum.z = fmaf(v.z, f, sum.z), sum.w = fmaf(v.w, f, sum.w);
+                    }
+                    at_store4<T>(out + d, a.wide, sum.x / den, sum.y / den, sum.z / den, sum.w / den);
                 }
             }
         }
         __syncthreads();                      // the join's memory is free again
     }
+    zeros();
     if (!ok)                                  // copies in flight land before the CTA leaves
         for (int k = used; k < issued; ++k)
             mbar_wait_bounded(&full[warp][k % STAGES], k / STAGES & 1, c.status, HOLO_E_TIMEOUT);
@@ -609,7 +702,11 @@ extern "C" int cuda_kv4_attention(const holo_kv4 *c, int layer, void *out, const
     a.out = out, a.q = q, a.q_row = q_row, a.out_row = out_row, a.seqs = seqs;
     a.n = n, a.n_heads = n_heads, a.group = group, a.chunks = (group + KV4_HEADS - 1) / KV4_HEADS;
     a.scale = scale == 0.0f ? 1.0f / sqrtf((float)c->head_dim) : scale;
-    a.page_magic = (((uint64_t)1 << 32) + view.page_blocks - 1) / view.page_blocks;
+    // units of the list, at most: counted in an int
+    const long long units = ((long long)c->max_pages * c->page_tokens + AT_UNIT_POS - 1) / AT_UNIT_POS;
+    if (units * n * c->n_kv_heads * a.chunks > 0x40000000LL) return refuse(HOLO_E_UNSUPPORTED);
+    a.page_magic = view.page_blocks == 1 ? 0 : (uint32_t)((((uint64_t)1 << 32) + view.page_blocks - 1) / view.page_blocks);
+    a.wide = (uintptr_t)out % 16 == 0 && out_row * size % 16 == 0;
     a.counters = work.counters, a.partial = work.partial;
     const int sms = holo_dev()->sms;
     bool done;
