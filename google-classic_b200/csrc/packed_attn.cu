@@ -138,7 +138,7 @@ template <int HD> struct PkGeom {
 };
 
 struct PkBars {
-    uint64_t q_full[2], s_full[2], p_full[2], o_done[2], kv_full[PK_STAGES], kv_empty[PK_STAGES], v_checked[2], drain;
+    uint64_t q_full[2], s_full[2], p_full[2], o_done[2], kv_full[PK_STAGES], kv_empty[PK_STAGES], v_here[2], v_checked[2], drain;
     uint32_t tmem;
     int first, len, pair;              // the CTA's work: its sequence's first row and length, and 256-row tile
     int bad_from;                      // first key of the diagonal tiles with a value that is not finite
@@ -297,6 +297,7 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
             mbar_init(&B.s_full[t], 1);
             mbar_init(&B.p_full[t], 128);
             mbar_init(&B.o_done[t], 1);
+            mbar_init(&B.v_here[t], 1);
             mbar_init(&B.v_checked[t], 64);
         }
         B.bad_from = 0x7fffffff;
@@ -364,6 +365,7 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
             if (ok) tc_commit(&B.kv_empty[0]);
             for (int j = 0; j < n && ok; ++j) {
                 wait_kv(2 * j + 1);
+                if (j >= n0 - 1) mbar_arrive(&B.v_here[j - (n0 - 1)]);   // for its check
 #pragma unroll 1
                 for (int t = 0; t < 2; ++t) {
                     const int nt = t ? n1 : n0;
@@ -393,8 +395,9 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
         if (warp >= 10) {
             // ---- diagonal tiles of V: no value that is not finite in a masked place ----
             for (int j = n0 - 1; j < n; ++j) {
+                // (the ring's barrier alone would not do: its phase may be several before this tile's)
                 const int i = 2 * j + 1;
-                const bool ok = mbar_wait_bounded(&B.kv_full[i % PK_STAGES], i / PK_STAGES & 1, a.status, HOLO_E_TIMEOUT);
+                const bool ok = mbar_wait_bounded(&B.v_here[j - (n0 - 1)], 0, a.status, HOLO_E_TIMEOUT);
                 uint4 *tile = reinterpret_cast<uint4 *>(skv + i % PK_STAGES * G::TILE);
                 for (int e = threadIdx.x - 320; e < G::TILE / 16 && ok; e += 64) {
                     uint4 w = tile[e];

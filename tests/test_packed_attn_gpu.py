@@ -86,6 +86,22 @@ def test_values_in_masked_places_change_nothing(packed, hd, bad):
     assert got[75:160].isnan().all()
 
 
+@pytest.mark.parametrize("n", [390, 520, 650, 1300])
+def test_values_in_masked_places_of_a_long_sequence(packed, n):
+    """The same at the end of a sequence of several key tiles, whichever place in the load ring its last tile has; and repeated
+    calls over memory that other values have been in agree."""
+    q, k, v = rows([n, 200], 2, 1, 128, "bf16", n)
+    cu = cu_of([n, 200])
+    want = packed(q, k, v, cu).clone()
+    k2, v2 = k.clone(), v.clone()
+    v2[n:], k2[n:] = float("nan"), float("nan")
+    v2[n - 20:n], k2[n - 20:n] = float("inf"), float("nan")
+    for _ in range(3):
+        got = packed(q, k2, v2, cu)
+        assert torch.equal(got[:n - 20], want[:n - 20]) and got[n - 20:].isnan().all()
+        assert torch.equal(packed(q, k, v, cu), want)
+
+
 def test_strides(packed):
     """q, k and v as columns of one matrix of rows, heads before rows, and an odd offset that no wide load takes."""
     lens, heads, n_kv, hd = [130, 30], 4, 2, 64
