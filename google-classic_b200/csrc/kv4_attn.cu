@@ -278,34 +278,44 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
     at_clip(head);
 
     // ---- the warp's loads: unit `unit` of item `load` ----
-    Walk load = head;
-    int unit = load.first + warp;
-    const uint8_t *load_base = nullptr;       // of the KV head
-    const int *load_table = nullptr;
+    // The walks lie in shared memory (one a warp each): only an item's change reads them.
+    __shared__ Walk walk_load[AT_WARPS], walk_use[AT_WARPS];
+    Walk &load = walk_load[warp], &w = walk_use[warp];
+    if (lane == 0) load = head, w = head;
+    __syncwarp();
+    int unit = head.first + warp, unit_end, load_len;   // unit_end 0: no more
+    const uint8_t *load_base;                 // of the KV head
+    const int *load_table;
     const uint32_t page_bytes = (uint32_t)c.n_kv * c.page_blocks * G::BLOCK_BYTES;
     auto settle = [&]() {                     // to the next unit that there is, and its item
-        while (load.rest > 0 && unit >= load.first + load.take) {
-            at_next(c, a, load);
-            unit = load.first + warp;
+        Walk x = load;
+        while (x.rest > 0 && unit >= x.first + x.take) {
+            at_next(c, a, x);
+            unit = x.first + warp;
         }
-        load_base = c.pool + (uint32_t)(load.item / a.chunks * c.page_blocks * G::BLOCK_BYTES);
-        load_table = c.tables + (size_t)max(0, load.s) * c.max_pages;
+        __syncwarp();
+        if (lane == 0) load = x;
+        __syncwarp();
+        unit_end = x.rest > 0 ? x.first + x.take : 0;
+        load_len = x.len;
+        load_base = c.pool + (uint32_t)(x.item / a.chunks * c.page_blocks * G::BLOCK_BYTES);
+        load_table = c.tables + (size_t)max(0, x.s) * c.max_pages;
     };
     settle();
     int entry = -1, in_page = 0;              // lanes 0 and 1: the page of their block of it, and the block there
     auto look_up = [&]() {
         const int block = unit * AT_UNIT + lane;
-        if (load.rest > 0 && lane < AT_UNIT && block * KV4_BLOCK < load.len) {
+        if (unit < unit_end && lane < AT_UNIT && block * KV4_BLOCK < load_len) {
             const int col = a.page_magic ? (int)__umulhi((uint32_t)block, a.page_magic) : block;
             in_page = block - col * c.page_blocks;
             entry = __ldg(load_table + col);
         }
     };
     look_up();
-    int issued = 0, fill = 0;                 // copies issued, the slot of the next one
+    int ahead = 0, fill = 0;                  // units issued and not yet taken, the slot of the next one
     auto issue = [&]() {                      // its copies, and the table entries of the next one
-        if (load.rest <= 0) return;
-        const int blocks = min(AT_UNIT, (load.len - unit * AT_UNIT_POS + KV4_BLOCK - 1) / KV4_BLOCK);
+        if (unit >= unit_end) return;
+        const int blocks = min(AT_UNIT, (load_len - unit * AT_UNIT_POS + KV4_BLOCK - 1) / KV4_BLOCK);
         if (lane == 0) mbar_arrive_expect_tx(&full[warp][fill], blocks * G::BLOCK_BYTES);
         __syncwarp();
         if (lane < blocks) {
@@ -319,19 +329,20 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
                    "l"(load_base + (size_t)(uint32_t)entry * page_bytes + in_page * G::BLOCK_BYTES), "r"(G::BLOCK_BYTES),
                    "r"(smem_addr(&full[warp][fill])) : "memory");
         }
-        ++issued;
+        ++ahead;
         fill = fill + 1 == STAGES ? 0 : fill + 1;
         unit += AT_WARPS;
-        if (unit >= load.first + load.take) settle();
+        if (unit >= unit_end) settle();
         look_up();
     };
     __syncwarp();
     for (int k = 0; k < STAGES; ++k) issue();
 
     // ---- items ----
-    int used = 0, slot = 0, phase = 0;        // units taken, the slot of the next one and its barrier's phase
+    int slot = 0, phase = 0;                  // the slot of the next unit to take and its barrier's phase
     bool ok = true;
-    for (Walk w = head; w.rest > 0; at_next(c, a, w)) {
+    while (w.rest > 0) {
+        const int len = w.len, u_end = w.first + w.take;
         const int kvh = w.item / a.chunks, head0 = kvh * a.group + (w.item % a.chunks) * KV4_HEADS;
         const int heads = min(KV4_HEADS, (kvh + 1) * a.group - head0);
         // q of head g: quarter t of every group, times a power of two; B fragments of the two steps of a group
@@ -394,14 +405,14 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
         int power = -32;                      // of two: the largest |value scale| lies below it
 
-        for (int u = w.first + warp; u < w.first + w.take; u += AT_WARPS) {
+        for (int u = w.first + warp; u < u_end; u += AT_WARPS) {
             ok = ok && mbar_wait_bounded(&full[warp][slot], phase, c.status, HOLO_E_TIMEOUT);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             const uint8_t *buf = ring + slot * AT_UNIT * G::BLOCK_BYTES;
-            ++used;
+            --ahead;
             if (++slot == STAGES) slot = 0, phase ^= 1;
-            const int left = w.len - u * AT_UNIT_POS;   // positions of the sequence from the unit's first on
+            const int left = len - u * AT_UNIT_POS;   // positions of the sequence from the unit's first on
             const bool tail = left < AT_UNIT_POS;
             // scores of positions g, g + 8 (+ 16 a block), heads 2 t and 2 t + 1
             float s[AT_UNIT][4];
@@ -642,11 +653,18 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
             }
         }
         __syncthreads();                      // the join's memory is free again
+        Walk x = w;
+        at_next(c, a, x);
+        __syncwarp();
+        if (lane == 0) w = x;
+        __syncwarp();
     }
     zeros();
     if (!ok)                                  // copies in flight land before the CTA leaves
-        for (int k = used; k < issued; ++k)
-            mbar_wait_bounded(&full[warp][k % STAGES], k / STAGES & 1, c.status, HOLO_E_TIMEOUT);
+        for (; ahead > 0; --ahead) {
+            mbar_wait_bounded(&full[warp][slot], phase, c.status, HOLO_E_TIMEOUT);
+            if (++slot == STAGES) slot = 0, phase ^= 1;
+        }
 }
 
 template <typename T, int HD>

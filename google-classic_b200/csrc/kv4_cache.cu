@@ -1,10 +1,13 @@
 // kv4_cache.cu -- the paged 4-bit KV cache: sizes and argument checks, rows of
 // keys and values quantised into their pages, and read back.
 //
-// Eight lanes hold a group of 32 values (four each) of one row, head and side:
+// Four lanes hold a group of 32 values (eight each) of one row, head and side:
 // the group's value of largest magnitude is found over them with shuffles, and
-// each lane writes the halfword of its four codes.  Both kernels move each
-// byte once and are bound by memory traffic.
+// a lane writes the word of its eight key codes, or two halfwords of value codes.
+// A CTA takes up to 16 rows, whose places (sequence, page, block) are looked up
+// once; rows that share a block meet in one CTA, so its partly written sectors are
+// completed in L2.  Both kernels move each byte once and are bound by memory
+// traffic where there are many rows, by latency where there are few.
 #include "kv4.cuh"
 
 #include <mutex>
@@ -56,169 +59,154 @@ __device__ __forceinline__ int seq_of_row(const int *__restrict__ cu, int n, int
     return lo;
 }
 
-// where row `row` of the packed rows lies: its block and place; false where it
-// has none (rows outside cu, a sequence left out, a missing page)
-__device__ __forceinline__ bool row_place(const Kv4View &c, const int *cu, const int *start, const int *seqs, int n,
-                                          int row, int &page, int &block, int &slot) {
+constexpr int ROW_MAX = 16;            // rows a CTA
+
+// where a row lies: byte offset of its block of KV head 0 in the layer (-1:
+// nowhere), place in the block
+struct Place {
+    long long at;
+    int slot;
+};
+
+__device__ __forceinline__ Place row_place(const Kv4View &c, int hd, const int *cu, const int *start, const int *seqs,
+                                           int n, int row) {
     const int i = seq_of_row(cu, n, row);
-    const int first = __ldg(cu + i), at0 = __ldg(start + i), s = seqs ? __ldg(seqs + i) : i;
-    if (row < first || row >= __ldg(cu + i + 1) || at0 < 0) return false;
-    if (s < 0 || s >= c.max_seqs) {
-        kv4_report(c.status, HOLO_E_ARG);
-        return false;
-    }
+    const int first = __ldg(cu + i), end = __ldg(cu + i + 1), at0 = __ldg(start + i), s = seqs ? __ldg(seqs + i) : i;
+    Place p = {-1, 0};
+    if (row < first || row >= end || at0 < 0) return p;
     const long long pos = (long long)at0 + (row - first);
-    const long long col = pos / c.page_tokens;
-    if (col >= c.max_pages) {
+    if (s < 0 || s >= c.max_seqs || pos >= (long long)c.max_pages * c.page_tokens) {
         kv4_report(c.status, HOLO_E_ARG);
-        return false;
+        return p;
     }
-    page = __ldg(c.tables + (size_t)s * c.max_pages + col);
+    const int col = (int)pos / c.page_tokens, in_page = (int)pos - col * c.page_tokens;
+    const int page = __ldg(c.tables + (size_t)s * c.max_pages + col);
     if (page < 0 || page >= c.n_pages) {
         kv4_report(c.status, HOLO_E_ARG);
-        return false;
+        return p;
     }
-    const int in_page = (int)(pos - col * c.page_tokens);
-    block = in_page / KV4_BLOCK;
-    slot = in_page % KV4_BLOCK;
-    return true;
+    p.at = ((long long)page * c.n_kv * c.page_blocks + in_page / KV4_BLOCK) * kv4_block_bytes(hd);
+    p.slot = in_page % KV4_BLOCK;
+    return p;
 }
 
-template <typename T> struct Four { T v[4]; };
-
+// eight values of a row; wide: 16-byte aligned
 template <typename T>
-__device__ __forceinline__ void load4(const T *p, bool wide, float (&x)[4]) {
+__device__ __forceinline__ void load8(const T *p, bool wide, float (&x)[8]) {
     if (wide) {
-        if constexpr (sizeof(T) == 4) {
-            const float4 w = __ldg(reinterpret_cast<const float4 *>(p));
-            x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w;
-        } else {
-            const uint2 w = __ldg(reinterpret_cast<const uint2 *>(p));
-            const T *h = reinterpret_cast<const T *>(&w);
+        uint4 w[sizeof(T) / 2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = kv4_to_float<T>(h[i]);
-        }
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+        const T *h = reinterpret_cast<const T *>(w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = kv4_to_float<T>(h[i]);
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = kv4_to_float<T>(p[i]);
+        for (int i = 0; i < 8; ++i) x[i] = kv4_to_float<T>(p[i]);
     }
 }
 
 template <typename T>
-__device__ __forceinline__ void store4(T *p, bool wide, const float (&x)[4]) {
+__device__ __forceinline__ void store8(T *p, bool wide, const float (&x)[8]) {
     if (wide) {
-        if constexpr (sizeof(T) == 4) {
-            *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
-        } else {
-            uint2 w;
-            T *h = reinterpret_cast<T *>(&w);
+        uint4 w[sizeof(T) / 2];
+        T *h = reinterpret_cast<T *>(w);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) h[i] = kv4_from_float<T>(x[i]);
-            *reinterpret_cast<uint2 *>(p) = w;
-        }
+        for (int i = 0; i < 8; ++i) h[i] = kv4_from_float<T>(x[i]);
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4 *>(p)[i] = w[i];
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = kv4_from_float<T>(x[i]);
+        for (int i = 0; i < 8; ++i) p[i] = kv4_from_float<T>(x[i]);
     }
 }
 
-// four codes of a lane and the scale of its group, over the eight lanes that
+// eight codes of a lane and the scale of its group, over the four lanes that
 // hold it: d = fp16(m / -8), code = rint(x / d) + 8 in 0..15 (fp32 arithmetic,
 // each operation rounded once), NaN as the scale where a value is not finite
-__device__ __forceinline__ uint32_t quantise4(const float (&x)[4], __half &d) {
+__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], __half &d) {
     float m = x[0];
     bool finite = isfinite(x[0]);
 #pragma unroll
-    for (int i = 1; i < 4; ++i) {
+    for (int i = 1; i < 8; ++i) {
         if (fabsf(x[i]) > fabsf(m)) m = x[i];
         finite = finite && isfinite(x[i]);
     }
     // of two equal magnitudes the lower lane's stays
-    const int lane = threadIdx.x & 7;
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
-        const float other = __shfl_xor_sync(0xffffffffu, m, o, 8);
-        const bool lower = (lane & o) != 0;   // the other lane is the lower one
+    for (int o = 1; o < 4; o <<= 1) {
+        const float other = __shfl_xor_sync(0xffffffffu, m, o, 4);
+        const bool lower = (threadIdx.x & o) != 0;   // the other lane is the lower one
         if (fabsf(other) > fabsf(m) || (lower && fabsf(other) == fabsf(m))) m = other;
     }
     const unsigned all = __ballot_sync(0xffffffffu, finite);
-    const unsigned mine = 0xffu << (threadIdx.x & 24);
+    const unsigned mine = 0xfu << (threadIdx.x & 28);
     d = (all & mine) == mine ? __float2half_rn(m * -0.125f) : __ushort_as_half(0x7e00);
     const float w = __half2float(d);
     uint32_t codes = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
         const int q = w == 0.0f ? 0 : __float2int_rn(__fdiv_rn(x[i], w));
         codes |= (uint32_t)max(0, min(15, q + 8)) << (4 * i);
     }
     return codes;
 }
 
-// Thread = (row, head, group b, four values g).  blockIdx.x strides the rows'
-// fours; whole groups of eight threads stay together (the shuffles), past the
-// end too.
-template <typename T, int HD>
-__global__ void __launch_bounds__(ROW_THREADS)
-append_kernel(const __grid_constant__ Kv4View c, const T *__restrict__ k, const T *__restrict__ v, long long k_row,
-              long long v_row, int rows, const int *__restrict__ cu, const int *__restrict__ start,
-              const int *__restrict__ seqs, int n, bool wide) {
-    constexpr int NB = HD / KV4_GROUP, FOURS = HD / 4;
-    const long long per_row = (long long)c.n_kv * FOURS, total = (long long)rows * per_row;
-    const long long step = (long long)gridDim.x * ROW_THREADS;
-    for (long long e0 = (long long)blockIdx.x * ROW_THREADS; e0 < total; e0 += step) {
-        const long long e = e0 + threadIdx.x;
-        const bool in = e < total;
-        const int row = in ? (int)(e / per_row) : 0, in_row = in ? (int)(e - (long long)row * per_row) : 0;
-        const int kvh = in_row / FOURS, four = in_row % FOURS, b = four >> 3, g = four & 7;
-        int page = 0, block = 0, slot = 0;
-        const bool ok = in && row_place(c, cu, start, seqs, n, row, page, block, slot);
-        float xk[4] = {0.0f, 0.0f, 0.0f, 0.0f}, xv[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (ok) {
-            load4(k + (size_t)row * k_row + (size_t)kvh * HD + 4 * four, wide, xk);
-            load4(v + (size_t)row * v_row + (size_t)kvh * HD + 4 * four, wide, xv);
-        }
-        __half dk, dv;
-        const uint32_t ck = quantise4(xk, dk), cv = quantise4(xv, dv);
-        if (ok) {
-            uint8_t *blk = kv4_block(c, HD, page, kvh, block);
-            *reinterpret_cast<uint16_t *>(blk + kv4_k_half(HD, slot, g, b)) = (uint16_t)ck;
-            *reinterpret_cast<uint16_t *>(blk + kv4_off_v(HD) + kv4_v_half(HD, slot, g, b)) = (uint16_t)cv;
-            if (g == 0) {
-                *reinterpret_cast<__half *>(blk + kv4_off_dk(HD) + 2 * (slot * NB + b)) = dk;
-                *reinterpret_cast<__half *>(blk + kv4_off_dv(HD) + 2 * (slot * NB + b)) = dv;
-            }
-        }
-    }
-}
-
-__device__ __forceinline__ void dequantise4(uint32_t codes, __half d, float (&x)[4]) {
+__device__ __forceinline__ void dequantise8(uint32_t codes, __half d, float (&x)[8]) {
     const float w = __half2float(d);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = w * (float)((int)((codes >> (4 * i)) & 15u) - 8);
+    for (int i = 0; i < 8; ++i) x[i] = w * (float)((int)((codes >> (4 * i)) & 15u) - 8);
 }
 
-template <typename T, int HD>
+// Thread = (row, head, group b, eight values t), of the CTA's rows.  `lanes`
+// = n_kv * HD / 8 threads a row (a multiple of eight), `magic` = ceil(2^32 / lanes).
+template <bool APPEND, typename T, int HD>
 __global__ void __launch_bounds__(ROW_THREADS)
-read_kernel(const __grid_constant__ Kv4View c, T *__restrict__ k, T *__restrict__ v, long long k_row, long long v_row,
+rows_kernel(const __grid_constant__ Kv4View c, T *__restrict__ k, T *__restrict__ v, long long k_row, long long v_row,
             int rows, const int *__restrict__ cu, const int *__restrict__ start, const int *__restrict__ seqs, int n,
-            bool wide) {
-    constexpr int NB = HD / KV4_GROUP, FOURS = HD / 4;
-    const long long per_row = (long long)c.n_kv * FOURS, total = (long long)rows * per_row;
-    const long long step = (long long)gridDim.x * ROW_THREADS;
-    for (long long e = (long long)blockIdx.x * ROW_THREADS + threadIdx.x; e < total; e += step) {
-        const int row = (int)(e / per_row), in_row = (int)(e - (long long)row * per_row);
-        const int kvh = in_row / FOURS, four = in_row % FOURS, b = four >> 3, g = four & 7;
-        int page, block, slot;
-        float xk[4] = {0.0f, 0.0f, 0.0f, 0.0f}, xv[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (row_place(c, cu, start, seqs, n, row, page, block, slot)) {
-            const uint8_t *blk = kv4_block(c, HD, page, kvh, block);
-            const uint32_t ck = *reinterpret_cast<const uint16_t *>(blk + kv4_k_half(HD, slot, g, b));
-            const uint32_t cv = *reinterpret_cast<const uint16_t *>(blk + kv4_off_v(HD) + kv4_v_half(HD, slot, g, b));
-            dequantise4(ck, *reinterpret_cast<const __half *>(blk + kv4_off_dk(HD) + 2 * (slot * NB + b)), xk);
-            dequantise4(cv, *reinterpret_cast<const __half *>(blk + kv4_off_dv(HD) + 2 * (slot * NB + b)), xv);
+            bool wide, int rows_cta, int lanes, uint32_t magic) {
+    constexpr int NB = HD / KV4_GROUP, EIGHTS = HD / 8;
+    __shared__ Place places[ROW_MAX];
+    const int row0 = blockIdx.x * rows_cta, mine = min(rows_cta, rows - row0);
+    if ((int)threadIdx.x < mine) places[threadIdx.x] = row_place(c, HD, cu, start, seqs, n, row0 + threadIdx.x);
+    __syncthreads();
+    const int total = mine * lanes;
+    for (int e0 = blockIdx.y * ROW_THREADS; e0 < total; e0 += gridDim.y * ROW_THREADS) {
+        const int e = e0 + threadIdx.x;
+        const int r = min((int)__umulhi((uint32_t)e, magic), mine - 1), in_row = e - r * lanes;
+        const int kvh = in_row / EIGHTS, eight = in_row % EIGHTS, b = eight >> 2, t = eight & 3;
+        const Place p = places[r];
+        const bool in = e < total, ok = in && p.at >= 0;
+        const size_t at_k = (size_t)(row0 + r) * k_row + (size_t)kvh * HD + 8 * eight;
+        const size_t at_v = (size_t)(row0 + r) * v_row + (size_t)kvh * HD + 8 * eight;
+        uint8_t *blk = c.pool + p.at + (size_t)kvh * c.page_blocks * kv4_block_bytes(HD);
+        uint32_t *word = reinterpret_cast<uint32_t *>(blk + kv4_k_half(HD, p.slot, 2 * t, b));
+        uint16_t *half0 = reinterpret_cast<uint16_t *>(blk + kv4_off_v(HD) + kv4_v_half(HD, p.slot, 2 * t, b));
+        uint16_t *half1 = reinterpret_cast<uint16_t *>(blk + kv4_off_v(HD) + kv4_v_half(HD, p.slot, 2 * t + 1, b));
+        __half *scale_k = reinterpret_cast<__half *>(blk + kv4_off_dk(HD) + 2 * (p.slot * NB + b));
+        __half *scale_v = reinterpret_cast<__half *>(blk + kv4_off_dv(HD) + 2 * (p.slot * NB + b));
+        float xk[8] = {}, xv[8] = {};
+        if (APPEND) {
+            if (ok) {
+                load8(k + at_k, wide, xk);
+                load8(v + at_v, wide, xv);
+            }
+            __half dk, dv;
+            const uint32_t ck = quantise8(xk, dk), cv = quantise8(xv, dv);
+            if (ok) {
+                *word = ck;
+                *half0 = (uint16_t)cv;
+                *half1 = (uint16_t)(cv >> 16);
+                if (t == 0) *scale_k = dk, *scale_v = dv;
+            }
+        } else if (in) {
+            if (ok) {
+                dequantise8(*word, *scale_k, xk);
+                dequantise8(*half0 | (uint32_t)*half1 << 16, *scale_v, xv);
+            }
+            store8(k + at_k, wide, xk);
+            store8(v + at_v, wide, xv);
         }
-        store4(k + (size_t)row * k_row + (size_t)kvh * HD + 4 * four, wide, xk);
-        store4(v + (size_t)row * v_row + (size_t)kvh * HD + 4 * four, wide, xv);
     }
 }
 
@@ -235,15 +223,16 @@ struct Rows {
 
 template <bool APPEND, typename T, int HD>
 void launch_rows(const Rows &r, const Kv4View &view, bool wide, int sms, cudaStream_t st) {
-    const long long total = (long long)r.rows * view.n_kv * (HD / 4);
-    const long long want = (total + ROW_THREADS - 1) / ROW_THREADS, most = (long long)sms * 32;
-    const unsigned grid = (unsigned)(want < most ? want : most);
-    if (APPEND)
-        append_kernel<T, HD><<<grid, ROW_THREADS, 0, st>>>(view, (const T *)r.k, (const T *)r.v, r.k_row, r.v_row, r.rows,
-                                                          r.cu, r.start, r.seqs, r.n, wide);
-    else
-        read_kernel<T, HD><<<grid, ROW_THREADS, 0, st>>>(view, (T *)r.k, (T *)r.v, r.k_row, r.v_row, r.rows, r.cu,
-                                                        r.start, r.seqs, r.n, wide);
+    // 16 rows a CTA where that still makes four CTAs an SM, else fewer, and the heads of
+    // one row over several CTAs where one row is all there is for each SM
+    const int lanes = view.n_kv * (HD / 8);
+    const int rows_cta = max(1, min(ROW_MAX, r.rows / (4 * sms)));
+    const unsigned x = (unsigned)((r.rows + rows_cta - 1) / rows_cta);
+    const int steps = (rows_cta * lanes + ROW_THREADS - 1) / ROW_THREADS;
+    const unsigned y = (unsigned)max(1, min(steps, (int)(4 * sms / x)));
+    const uint32_t magic = (uint32_t)((((uint64_t)1 << 32) + lanes - 1) / lanes);
+    rows_kernel<APPEND, T, HD><<<dim3(x, y), ROW_THREADS, 0, st>>>(view, (T *)r.k, (T *)r.v, r.k_row, r.v_row, r.rows, r.cu,
+                                                                  r.start, r.seqs, r.n, wide, rows_cta, lanes, magic);
 }
 
 template <bool APPEND, typename T>
@@ -273,13 +262,13 @@ int run_rows(Rows r, int layer, int type, const char *what) {
         return HOLO_E_ARG;
     }
     if (r.rows == 0 || r.n == 0) return HOLO_OK;
-    const int size = type_bytes(type), four = 4 * size;
+    const int size = type_bytes(type);
     if (((uintptr_t)r.k | (uintptr_t)r.v) % size) {
         holo_set_status(HOLO_E_ARG, what);
         return HOLO_E_ARG;
     }
-    // four values a load where every four of a row is aligned, else one by one
-    const bool wide = ((uintptr_t)r.k | (uintptr_t)r.v) % four == 0 && (r.k_row | r.v_row) % 4 == 0;
+    // 16-byte accesses where every eight values of a row are aligned, else one by one
+    const bool wide = ((uintptr_t)r.k | (uintptr_t)r.v) % 16 == 0 && (r.k_row * size | r.v_row * size) % 16 == 0;
     const int sms = holo_dev()->sms;
     switch (type) {
     case HOLO_DT_F32: launch_rows_hd<APPEND, float>(r, view, wide, sms, st); break;

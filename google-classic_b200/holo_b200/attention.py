@@ -15,17 +15,26 @@ import torch
 from . import load, DT_F32, DT_F16, DT_BF16, HOLO_OK
 
 DTYPES = {torch.float32: DT_F32, torch.float16: DT_F16, torch.bfloat16: DT_BF16}
-_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
 LEGACY_STREAM = 1   # cudaStreamLegacy: torch's default stream has the handle 0, which the library takes for its own
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # absent from builds of torch without CUDA
+_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
-def stream_of(t) -> int:
-    """The handle of torch's current stream on the device of t, which has to
-    be the current device (the library's state belongs to it)."""
-    index = t.device.index
-    if t.device.type != "cuda" or index != torch.cuda.current_device():
-        raise ValueError(f"tensor on {t.device}: the current CUDA device is needed")
+def stream_of(index: int) -> int:
+    """The handle of torch's current stream on CUDA device `index`, which has
+    to be the current device (the library's state belongs to it)."""
+    if index < 0 or index != _device():
+        raise ValueError(f"tensors on device {index}: the current CUDA device is needed")
     return _raw_stream(index) or LEGACY_STREAM
+
+
+_LIB = None
+
+
+def _lib():
+    global _LIB
+    _LIB = load()
+    return _LIB
 
 
 def check(rc: int, what: str):
@@ -46,11 +55,13 @@ class PackedDesc(C.Structure):
                 ("out_head", C.c_longlong), ("stream", C.c_void_p)]
 
 
-def row_stride(t, what: str) -> int:
-    """Elements between the rows of t [rows][heads][head_dim] whose heads are
+def row_stride(t, heads: int, hd: int, what: str) -> int:
+    """Elements between the rows of t [rows][heads][hd] whose heads are
     adjacent; 0, dense, where one row or none leaves it open."""
-    rows, heads, hd = t.shape
+    if t.is_contiguous():
+        return 0
     s = t.stride()
+    rows = t.shape[0]
     if (heads > 1 and s[1] != hd) or s[2] != 1 or (rows > 1 and s[0] < heads * hd):
         raise ValueError(f"{what}: strides {s} of {tuple(t.shape)}: the heads of a row have to be adjacent, and rows apart")
     return s[0] if rows > 1 else 0
@@ -58,6 +69,8 @@ def row_stride(t, what: str) -> int:
 
 def _strides(t, what: str):
     """Elements between the rows and between the heads of t [rows][heads][head_dim]."""
+    if t.is_contiguous():
+        return 0, 0
     rows, heads, hd = t.shape
     s = t.stride()
     if s[2] != 1 or (rows > 1 and s[0] < hd) or (heads > 1 and s[1] < hd):
@@ -71,12 +84,13 @@ def attention_packed(q, k, v, cu_seqlens, out=None, lse=None, scale: float = 0.0
     rows and heads), cu_seqlens int32 [n_seqs + 1] on the device.  Returns out
     (made when None); lse, when given, is float32 [n_heads][total] and gets
     each row's log-sum-exp.  scale 0: 1 / sqrt(head_dim)."""
-    total, n_heads, hd = q.shape
-    if k.shape != v.shape or k.shape[0] != total or k.shape[2] != hd:
+    shape, kv_shape = q.shape, k.shape
+    total, n_heads, hd = shape
+    if kv_shape != v.shape or len(kv_shape) != 3 or kv_shape[0] != total or kv_shape[2] != hd:
         raise ValueError(f"attention_packed: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    if out.shape != q.shape:
+    elif out.shape != shape:
         raise ValueError(f"attention_packed: out {tuple(out.shape)} for q {tuple(q.shape)}")
     dtype = q.dtype
     if dtype not in DTYPES or k.dtype != dtype or v.dtype != dtype or out.dtype != dtype:
@@ -85,14 +99,14 @@ def attention_packed(q, k, v, cu_seqlens, out=None, lse=None, scale: float = 0.0
         raise TypeError("attention_packed: cu_seqlens is a contiguous int32 vector")
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != (n_heads, total) or not lse.is_contiguous()):
         raise TypeError("attention_packed: lse is a contiguous float32 [n_heads][total]")
-    device = q.device
-    for t in (k, v, out, cu_seqlens) if lse is None else (k, v, out, cu_seqlens, lse):
-        if t.device != device:
-            raise ValueError(f"attention_packed: tensors on {device} and {t.device}")
-    d = PackedDesc(DTYPES[dtype], n_heads, k.shape[1], hd, cu_seqlens.shape[0] - 1, total, scale,
+    index = q.get_device()
+    if k.get_device() != index or v.get_device() != index or out.get_device() != index or cu_seqlens.get_device() != index or (
+            lse is not None and lse.get_device() != index):
+        raise ValueError("attention_packed: the tensors are on different devices")
+    d = PackedDesc(DTYPES[dtype], n_heads, kv_shape[1], hd, cu_seqlens.shape[0] - 1, total, scale,
                    *_strides(q, "attention_packed: q"), *_strides(k, "attention_packed: k"),
-                   *_strides(v, "attention_packed: v"), *_strides(out, "attention_packed: out"), stream_of(q))
-    rc = load().cuda_attention_packed(C.byref(d), out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                   *_strides(v, "attention_packed: v"), *_strides(out, "attention_packed: out"), stream_of(index))
+    rc = (_LIB or _lib()).cuda_attention_packed(C.addressof(d), out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
                                       cu_seqlens.data_ptr(), None if lse is None else lse.data_ptr())
     if rc:
         check(rc, "cuda_attention_packed")

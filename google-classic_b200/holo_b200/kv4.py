@@ -70,15 +70,17 @@ class Kv4Cache:
                                 tables.shape[1], pool.data_ptr(), tables.data_ptr(), lens.data_ptr(),
                                 None if refs is None else refs.data_ptr())
         self._at = C.addressof(d)
+        self._heads = (n_kv_heads, head_dim)
         size = self.lib.cuda_kv4_work_bytes(self._at)
         if size == 0:
             raise ValueError("Kv4Cache: this shape is not supported (head_dim 64/128/256, page_tokens a multiple of 16)")
-        stream_of(pool)
+        self._index = pool.get_device()
+        stream_of(self._index)
         self.work = torch.zeros(size, dtype=torch.uint8, device=pool.device)
         d.work = self.work.data_ptr()
 
     def _call(self, what: str, fn, *args):
-        self.desc.stream = stream_of(self.pool)
+        self.desc.stream = stream_of(self._index)
         rc = fn(self._at, *args)
         if rc:
             check(rc, what)
@@ -87,7 +89,7 @@ class Kv4Cache:
         """(pointer, count) of a list of sequences."""
         if seqs is None:
             return None, self.desc.max_seqs if n is None else n
-        if seqs.dtype != torch.int32 or seqs.dim() != 1 or not seqs.is_contiguous() or seqs.device != self.pool.device:
+        if seqs.dtype != torch.int32 or seqs.dim() != 1 or not seqs.is_contiguous() or seqs.get_device() != self._index:
             raise TypeError("Kv4Cache: a list of sequences is a contiguous int32 vector on the cache's device")
         return seqs.data_ptr(), seqs.shape[0]
 
@@ -109,21 +111,20 @@ class Kv4Cache:
         return start
 
     def _rows(self, what, k, v, cu_rows, start, seqs):
-        d = self.desc
-        n = cu_rows.shape[0] - 1
-        p, m = self._seqs(seqs, n)
-        if (k.shape != v.shape or k.dim() != 3 or k.shape[1] != d.n_kv_heads or k.shape[2] != d.head_dim or m != n
-                or start.shape != (n,)):
+        shape, n = k.shape, cu_rows.shape[0] - 1
+        p, m = (None, n) if seqs is None else self._seqs(seqs)
+        if shape != v.shape or len(shape) != 3 or shape[1:] != self._heads or m != n or start.shape != (n,):
             raise ValueError(f"{what}: k {tuple(k.shape)}, v {tuple(v.shape)}, {n} sequences in cu_rows")
-        if k.dtype not in DTYPES or v.dtype != k.dtype:
+        dtype = k.dtype
+        if dtype not in DTYPES or v.dtype != dtype:
             raise TypeError(f"{what}: k {k.dtype}, v {v.dtype}")
         if cu_rows.dtype != torch.int32 or start.dtype != torch.int32 or not cu_rows.is_contiguous() or not start.is_contiguous():
             raise TypeError(f"{what}: cu_rows and start are contiguous int32 vectors")
-        device = self.pool.device
-        if k.device != device or v.device != device or cu_rows.device != device or start.device != device:
-            raise ValueError(f"{what}: a tensor is not on {device}")
-        return (k.data_ptr(), v.data_ptr(), DTYPES[k.dtype], row_stride(k, what), row_stride(v, what), k.shape[0],
-                cu_rows.data_ptr(), start.data_ptr(), p, n)
+        i = self._index
+        if k.get_device() != i or v.get_device() != i or cu_rows.get_device() != i or start.get_device() != i:
+            raise ValueError(f"{what}: a tensor is not on the cache's device")
+        return (k.data_ptr(), v.data_ptr(), DTYPES[dtype], row_stride(k, *self._heads, what), row_stride(v, *self._heads, what),
+                shape[0], cu_rows.data_ptr(), start.data_ptr(), p, n)
 
     def append(self, layer: int, k, v, cu_rows, start, seqs=None):
         """Writes rows cu_rows[i] .. cu_rows[i + 1] of k and v [rows][n_kv_heads]
@@ -141,20 +142,21 @@ class Kv4Cache:
     def attention(self, layer: int, q, out=None, seqs=None, scale: float = 0.0):
         """Attention of one query a sequence, q [n][n_heads][head_dim], over
         all the positions that it holds; out like q."""
-        d = self.desc
-        n, n_heads, hd = q.shape
-        p, m = self._seqs(seqs, n)
+        shape = q.shape
+        n, n_heads, hd = shape
+        p, m = (None, n) if seqs is None else self._seqs(seqs)
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        if m != n or hd != d.head_dim or out.shape != q.shape:
+        if m != n or hd != self._heads[1] or out.shape != shape:
             raise ValueError(f"Kv4Cache.attention: q {tuple(q.shape)}, out {tuple(out.shape)}, {m} sequences")
-        if q.dtype not in DTYPES or out.dtype != q.dtype:
+        dtype = q.dtype
+        if dtype not in DTYPES or out.dtype != dtype:
             raise TypeError(f"Kv4Cache.attention: q {q.dtype}, out {out.dtype}")
-        if q.device != self.pool.device or out.device != q.device:
-            raise ValueError(f"Kv4Cache.attention: a tensor is not on {self.pool.device}")
+        if q.get_device() != self._index or out.get_device() != self._index:
+            raise ValueError("Kv4Cache.attention: a tensor is not on the cache's device")
         self._call("cuda_kv4_attention", self.lib.cuda_kv4_attention, layer, out.data_ptr(), q.data_ptr(),
-                   DTYPES[q.dtype], row_stride(q, "Kv4Cache.attention: q"), row_stride(out, "Kv4Cache.attention: out"),
-                   n_heads, scale, p, n)
+                   DTYPES[dtype], row_stride(q, n_heads, hd, "Kv4Cache.attention: q"),
+                   row_stride(out, n_heads, hd, "Kv4Cache.attention: out"), n_heads, scale, p, n)
         return out
 
     def fork(self, parents, children):
