@@ -299,6 +299,15 @@ __device__ __forceinline__ uint64_t l2_policy_evict_first() {
     return p;
 }
 
+// Programmatic dependent launch.  A kernel launched with holo_launch_early may
+// start while the kernel before it on the stream still runs: it calls
+// early_wait() before its first access to global memory (which returns once that
+// kernel has ended and its writes are visible), and early_next() to let the
+// kernel after it start the same way.  What the kernel before may have written is
+// not read through the non-coherent path (__ldg, const __restrict__).
+__device__ __forceinline__ void early_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void early_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // named barrier among a subset of warps
 __device__ __forceinline__ void named_bar_sync(int id, int nthreads) {
     asm volatile("bar.sync %0, %1;" :: "r"(id), "r"(nthreads) : "memory");
@@ -319,6 +328,17 @@ __device__ __forceinline__ float ubyte_to_float(uint32_t w, int k) {
 
 __device__ __forceinline__ float half_bits_to_float(uint32_t h16) {
     return __half2float(__ushort_as_half((unsigned short)h16));
+}
+
+template <typename... P, typename... A>
+inline cudaError_t holo_launch_early(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A &&...args) {
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid, cfg.blockDim = block, cfg.dynamicSmemBytes = smem, cfg.stream = st;
+    cfg.attrs = &attr, cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
 
 #endif  // __CUDACC__

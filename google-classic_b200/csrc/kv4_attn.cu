@@ -113,13 +113,13 @@ struct Walk {
 };
 
 __device__ __forceinline__ int at_units(const Kv4View &c, const AtArgs &a, int i, int &s, int &len) {
-    s = a.seqs ? __ldg(a.seqs + i) : i;
+    s = a.seqs ? __ldcg(a.seqs + i) : i;
     len = 0;
     if (s < 0 || s >= c.max_seqs) {
         s = -1;
         return 0;
     }
-    len = max(0, min(__ldg(c.lens + s), c.max_pages * c.page_tokens));
+    len = max(0, min(__ldcg(c.lens + s), c.max_pages * c.page_tokens));
     return (len + AT_UNIT_POS - 1) / AT_UNIT_POS;
 }
 __device__ __forceinline__ void at_clip(Walk &w) { w.take = min(w.units - w.first, w.rest); }
@@ -208,6 +208,8 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
 
     if (lane < STAGES) mbar_init(&full[warp][lane], 1);
     fence_barrier_init();
+    early_wait();
+    early_next();
 
     auto zeros = [&]() {                      // sequences without positions (a number out of range: left alone)
         for (int i = blockIdx.x; i < a.n; i += gridDim.x) {
@@ -308,7 +310,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
         if (unit < unit_end && lane < AT_UNIT && block * KV4_BLOCK < load_len) {
             const int col = a.page_magic ? (int)__umulhi((uint32_t)block, a.page_magic) : block;
             in_page = block - col * c.page_blocks;
-            entry = __ldg(load_table + col);
+            entry = __ldcg(load_table + col);
         }
     };
     look_up();
@@ -679,8 +681,7 @@ bool launch(const Kv4View &view, AtArgs a, int sms, cudaStream_t st) {
         if (dev < 16) configured[dev] = true;
     }
     const int grid = min(sms * G::CTAS, KV4_MAX_CTAS);
-    kv4_attn_kernel<T, HD><<<grid, AT_THREADS, G::SMEM, st>>>(view, a);
-    return true;
+    return holo_launch_early(kv4_attn_kernel<T, HD>, grid, AT_THREADS, G::SMEM, st, view, a) == cudaSuccess;
 }
 
 template <typename T>

@@ -49,11 +49,11 @@ void *own_work(size_t bytes) {
 }
 
 // the sequence i with cu[i] <= row < cu[i + 1]: the last i with cu[i] <= row
-__device__ __forceinline__ int seq_of_row(const int *__restrict__ cu, int n, int row) {
+__device__ __forceinline__ int seq_of_row(const int *cu, int n, int row) {
     int lo = 0, hi = n;   // cu[lo] <= row < cu[hi]
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (__ldg(cu + mid) <= row) lo = mid;
+        if (__ldcg(cu + mid) <= row) lo = mid;
         else hi = mid;
     }
     return lo;
@@ -71,7 +71,7 @@ struct Place {
 __device__ __forceinline__ Place row_place(const Kv4View &c, int hd, const int *cu, const int *start, const int *seqs,
                                            int n, int row) {
     const int i = seq_of_row(cu, n, row);
-    const int first = __ldg(cu + i), end = __ldg(cu + i + 1), at0 = __ldg(start + i), s = seqs ? __ldg(seqs + i) : i;
+    const int first = __ldcg(cu + i), end = __ldcg(cu + i + 1), at0 = __ldcg(start + i), s = seqs ? __ldcg(seqs + i) : i;
     Place p = {-1, 0};
     if (row < first || row >= end || at0 < 0) return p;
     const long long pos = (long long)at0 + (row - first);
@@ -80,7 +80,7 @@ __device__ __forceinline__ Place row_place(const Kv4View &c, int hd, const int *
         return p;
     }
     const int col = (int)pos / c.page_tokens, in_page = (int)pos - col * c.page_tokens;
-    const int page = __ldg(c.tables + (size_t)s * c.max_pages + col);
+    const int page = __ldcg(c.tables + (size_t)s * c.max_pages + col);
     if (page < 0 || page >= c.n_pages) {
         kv4_report(c.status, HOLO_E_ARG);
         return p;
@@ -96,7 +96,7 @@ __device__ __forceinline__ void load8(const T *p, bool wide, float (&x)[8]) {
     if (wide) {
         uint4 w[sizeof(T) / 2];
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = __ldcg(reinterpret_cast<const uint4 *>(p) + i);
         const T *h = reinterpret_cast<const T *>(w);
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = kv4_to_float<T>(h[i]);
@@ -162,11 +162,13 @@ __device__ __forceinline__ void dequantise8(uint32_t codes, __half d, float (&x)
 // = n_kv * HD / 8 threads a row (a multiple of eight), `magic` = ceil(2^32 / lanes).
 template <bool APPEND, typename T, int HD>
 __global__ void __launch_bounds__(ROW_THREADS)
-rows_kernel(const __grid_constant__ Kv4View c, T *__restrict__ k, T *__restrict__ v, long long k_row, long long v_row,
-            int rows, const int *__restrict__ cu, const int *__restrict__ start, const int *__restrict__ seqs, int n,
+rows_kernel(const __grid_constant__ Kv4View c, T *k, T *v, long long k_row, long long v_row,
+            int rows, const int *cu, const int *start, const int *seqs, int n,
             bool wide, int rows_cta, int lanes, uint32_t magic) {
     constexpr int NB = HD / KV4_GROUP, EIGHTS = HD / 8;
     __shared__ Place places[ROW_MAX];
+    early_wait();
+    early_next();
     const int row0 = blockIdx.x * rows_cta, mine = min(rows_cta, rows - row0);
     if ((int)threadIdx.x < mine) places[threadIdx.x] = row_place(c, HD, cu, start, seqs, n, row0 + threadIdx.x);
     __syncthreads();
@@ -231,8 +233,7 @@ void launch_rows(const Rows &r, const Kv4View &view, bool wide, int sms, cudaStr
     const int steps = (rows_cta * lanes + ROW_THREADS - 1) / ROW_THREADS;
     const unsigned y = (unsigned)max(1, min(steps, (int)(4 * sms / x)));
     const uint32_t magic = (uint32_t)((((uint64_t)1 << 32) + lanes - 1) / lanes);
-    rows_kernel<APPEND, T, HD><<<dim3(x, y), ROW_THREADS, 0, st>>>(view, (T *)r.k, (T *)r.v, r.k_row, r.v_row, r.rows, r.cu,
-                                                                  r.start, r.seqs, r.n, wide, rows_cta, lanes, magic);
+    holo_launch_early(rows_kernel<APPEND, T, HD>, dim3(x, y), ROW_THREADS, 0, st, view, (T *)r.k, (T *)r.v, r.k_row, r.v_row, r.rows, r.cu, r.start, r.seqs, r.n, wide, rows_cta, lanes, magic);
 }
 
 template <bool APPEND, typename T>

@@ -79,8 +79,10 @@ __device__ __forceinline__ int pages_of(const Kv4View &c, int len) { return len 
 constexpr int PLAN_SUM_MAX = 1 << 29;
 
 __global__ void __launch_bounds__(PLAN_THREADS, 1)
-extend_kernel(const __grid_constant__ Kv4View c, const int *__restrict__ seqs, const int *__restrict__ counts,
-              int *__restrict__ start, int n, int *__restrict__ list) {
+extend_kernel(const __grid_constant__ Kv4View c, const int *seqs, const int *counts,
+              int *start, int n, int *list) {
+    early_wait();
+    early_next();
     __shared__ int sh[32];
     // pages that the list's sequences need, in order
     int need_all = 0;
@@ -148,7 +150,9 @@ __device__ __forceinline__ void copy_page(uint8_t *pool, size_t page_bytes, int 
 
 __global__ void __launch_bounds__(COPY_THREADS)
 copy_kernel(const __grid_constant__ Kv4View c, size_t page_bytes, size_t layer_bytes, int layers,
-            const int *__restrict__ src, const int *__restrict__ dst, int n) {
+            const int *src, const int *dst, int n) {
+    early_wait();
+    early_next();
     const long long total = (long long)n * layers;
     for (long long u = blockIdx.x; u < total; u += gridDim.x) {
         const int i = (int)(u / layers), layer = (int)(u % layers);
@@ -164,8 +168,10 @@ copy_kernel(const __grid_constant__ Kv4View c, size_t page_bytes, size_t layer_b
 // ---- fork ------------------------------------------------------------------------
 // page[i]: the new page of child i; -1: it needs none, -2: it is left out
 __global__ void __launch_bounds__(PLAN_THREADS, 1)
-fork_plan_kernel(const __grid_constant__ Kv4View c, const int *__restrict__ parents, const int *__restrict__ children,
-                 int n, int *__restrict__ page, int *__restrict__ list) {
+fork_plan_kernel(const __grid_constant__ Kv4View c, const int *parents, const int *children,
+                 int n, int *page, int *list) {
+    early_wait();
+    early_next();
     __shared__ int sh[32];
     int need_all = 0;
     for (int i0 = 0; i0 < n; i0 += PLAN_THREADS) {
@@ -207,7 +213,9 @@ fork_plan_kernel(const __grid_constant__ Kv4View c, const int *__restrict__ pare
 
 __global__ void __launch_bounds__(COPY_THREADS)
 fork_kernel(const __grid_constant__ Kv4View c, size_t page_bytes, size_t layer_bytes, int layers,
-            const int *__restrict__ parents, const int *__restrict__ children, int n, const int *__restrict__ page) {
+            const int *parents, const int *children, int n, const int *page) {
+    early_wait();
+    early_next();
     const long long total = (long long)n * layers;
     for (long long u = blockIdx.x; u < total; u += gridDim.x) {
         const int i = (int)(u / layers), layer = (int)(u % layers);
@@ -241,7 +249,9 @@ fork_kernel(const __grid_constant__ Kv4View c, size_t page_bytes, size_t layer_b
 
 // ---- release ----------------------------------------------------------------------
 __global__ void __launch_bounds__(COPY_THREADS)
-release_kernel(const __grid_constant__ Kv4View c, const int *__restrict__ seqs, int n) {
+release_kernel(const __grid_constant__ Kv4View c, const int *seqs, int n) {
+    early_wait();
+    early_next();
     __shared__ int len_s;
     for (int i = blockIdx.x; i < n; i += gridDim.x) {
         const int s = seqs ? seqs[i] : i;
@@ -268,8 +278,10 @@ release_kernel(const __grid_constant__ Kv4View c, const int *__restrict__ seqs, 
 // ---- compact ------------------------------------------------------------------------
 // plan[0] moves: src, dst (ascending both); to[page]: its number afterwards
 __global__ void __launch_bounds__(PLAN_THREADS, 1)
-compact_plan_kernel(const __grid_constant__ Kv4View c, int *__restrict__ plan, int *__restrict__ src,
-                    int *__restrict__ dst, int *__restrict__ to) {
+compact_plan_kernel(const __grid_constant__ Kv4View c, int *plan, int *src,
+                    int *dst, int *to) {
+    early_wait();
+    early_next();
     __shared__ int sh[32];
     int live = 0;
     for (int p0 = 0; p0 < c.n_pages; p0 += PLAN_STEP) {
@@ -314,8 +326,10 @@ compact_plan_kernel(const __grid_constant__ Kv4View c, int *__restrict__ plan, i
 
 __global__ void __launch_bounds__(COPY_THREADS)
 compact_kernel(const __grid_constant__ Kv4View c, size_t page_bytes, size_t layer_bytes, int layers,
-               const int *__restrict__ plan, const int *__restrict__ src, const int *__restrict__ dst,
-               const int *__restrict__ to) {
+               const int *plan, const int *src, const int *dst,
+               const int *to) {
+    early_wait();
+    early_next();
     const int moves = plan[0];
     if (moves == 0) return;
     const long long me = (long long)blockIdx.x * COPY_THREADS + threadIdx.x, all = (long long)gridDim.x * COPY_THREADS;
@@ -372,7 +386,7 @@ int cuda_kv4_extend(const holo_kv4 *c, const int *seqs, const int *counts, int *
     if (!begin(c, "cuda_kv4_extend", p, true)) return cuda_last_status();
     if (n < 0 || n > c->max_seqs || (n > 0 && (!counts || !start))) return refuse("cuda_kv4_extend");
     if (n == 0) return HOLO_OK;
-    extend_kernel<<<1, PLAN_THREADS, 0, p.st>>>(p.view, seqs, counts, start, n, p.work.plan + PLAN_LISTS);
+    holo_launch_early(extend_kernel, 1, PLAN_THREADS, 0, p.st, p.view, seqs, counts, start, n, p.work.plan + PLAN_LISTS);
     return kv4_end("cuda_kv4_extend");
 }
 
@@ -382,9 +396,8 @@ int cuda_kv4_fork(const holo_kv4 *c, const int *parents, const int *children, in
     if (n < 0 || n > c->max_seqs || (n > 0 && (!parents || !children))) return refuse("cuda_kv4_fork");
     if (n == 0) return HOLO_OK;
     int *page = p.work.plan + PLAN_LISTS, *list = page + c->max_seqs;
-    fork_plan_kernel<<<1, PLAN_THREADS, 0, p.st>>>(p.view, parents, children, n, page, list);
-    fork_kernel<<<copy_grid(p, (long long)n * c->n_layers), COPY_THREADS, 0, p.st>>>(
-        p.view, p.page_bytes, p.layer_bytes, c->n_layers, parents, children, n, page);
+    holo_launch_early(fork_plan_kernel, 1, PLAN_THREADS, 0, p.st, p.view, parents, children, n, page, list);
+    holo_launch_early(fork_kernel, copy_grid(p, (long long)n * c->n_layers), COPY_THREADS, 0, p.st, p.view, p.page_bytes, p.layer_bytes, c->n_layers, parents, children, n, page);
     return kv4_end("cuda_kv4_fork");
 }
 
@@ -393,7 +406,7 @@ int cuda_kv4_release(const holo_kv4 *c, const int *seqs, int n) {
     if (!begin(c, "cuda_kv4_release", p, true)) return cuda_last_status();
     if (n < 0 || n > c->max_seqs) return refuse("cuda_kv4_release");
     if (n == 0) return HOLO_OK;
-    release_kernel<<<copy_grid(p, n), COPY_THREADS, 0, p.st>>>(p.view, seqs, n);
+    holo_launch_early(release_kernel, copy_grid(p, n), COPY_THREADS, 0, p.st, p.view, seqs, n);
     return kv4_end("cuda_kv4_release");
 }
 
@@ -401,9 +414,8 @@ int cuda_kv4_compact(const holo_kv4 *c) {
     Pages p;
     if (!begin(c, "cuda_kv4_compact", p, true)) return cuda_last_status();
     int *src = p.work.plan + PLAN_LISTS, *dst = src + c->n_pages, *to = dst + c->n_pages;
-    compact_plan_kernel<<<1, PLAN_THREADS, 0, p.st>>>(p.view, p.work.plan, src, dst, to);
-    compact_kernel<<<copy_grid(p, (long long)c->n_pages * c->n_layers), COPY_THREADS, 0, p.st>>>(
-        p.view, p.page_bytes, p.layer_bytes, c->n_layers, p.work.plan, src, dst, to);
+    holo_launch_early(compact_plan_kernel, 1, PLAN_THREADS, 0, p.st, p.view, p.work.plan, src, dst, to);
+    holo_launch_early(compact_kernel, copy_grid(p, (long long)c->n_pages * c->n_layers), COPY_THREADS, 0, p.st, p.view, p.page_bytes, p.layer_bytes, c->n_layers, p.work.plan, src, dst, to);
     return kv4_end("cuda_kv4_compact");
 }
 
@@ -412,8 +424,7 @@ int cuda_kv4_copy_pages(const holo_kv4 *c, const int *src, const int *dst, int n
     if (!begin(c, "cuda_kv4_copy_pages", p, false)) return cuda_last_status();
     if (n < 0 || (n > 0 && (!src || !dst))) return refuse("cuda_kv4_copy_pages");
     if (n == 0) return HOLO_OK;
-    copy_kernel<<<copy_grid(p, (long long)n * c->n_layers), COPY_THREADS, 0, p.st>>>(
-        p.view, p.page_bytes, p.layer_bytes, c->n_layers, src, dst, n);
+    holo_launch_early(copy_kernel, copy_grid(p, (long long)n * c->n_layers), COPY_THREADS, 0, p.st, p.view, p.page_bytes, p.layer_bytes, c->n_layers, src, dst, n);
     return kv4_end("cuda_kv4_copy_pages");
 }
 

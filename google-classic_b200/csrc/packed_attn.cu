@@ -60,8 +60,8 @@ struct PackedArgs {
 
 // first row and length of sequence s, inside the rows whatever cu says
 __device__ __forceinline__ void packed_seq(const PackedArgs &a, int s, int &first, int &len) {
-    first = max(0, __ldg(a.cu + s));
-    len = max(0, min(a.total, __ldg(a.cu + s + 1)) - first);
+    first = max(0, __ldcg(a.cu + s));
+    len = max(0, min(a.total, __ldcg(a.cu + s + 1)) - first);
 }
 
 // ---------------------------------------------------------------------------
@@ -77,7 +77,7 @@ packed_simple_kernel(const __grid_constant__ PackedArgs a) {
     int lo = 0, hi = a.n_seqs;   // the last s with cu[s] <= row
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (__ldg(a.cu + mid) <= row) lo = mid;
+        if (__ldcg(a.cu + mid) <= row) lo = mid;
         else hi = mid;
     }
     int first, len;
@@ -286,6 +286,8 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
     uint8_t *skv = sq + 2 * G::TILE;
     const int h = blockIdx.x % a.n_heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+    early_wait();
+    early_next();
     if (warp == 0) {
         int first = 0, len = 0, pair = -1;
         if (!pk_find_work(a, blockIdx.x / a.n_heads, first, len, pair)) pair = -1;
@@ -573,8 +575,7 @@ bool launch_tc(const PackedArgs &a, int type, cudaStream_t st) {
     const long long pairs = ((long long)a.total + 255LL * a.n_seqs) / 256;
     const long long grid = pairs * a.n_heads;
     if (grid > 0x7fffffffLL) return false;
-    packed_tc_kernel<T, HD><<<(unsigned)grid, PK_THREADS, PkGeom<HD>::SMEM, st>>>(a, qm, km, vm);
-    return true;
+    return holo_launch_early(packed_tc_kernel<T, HD>, (unsigned)grid, PK_THREADS, PkGeom<HD>::SMEM, st, a, qm, km, vm) == cudaSuccess;
 }
 
 // whether TMA can address rows of this base and these strides (elements)
