@@ -6,29 +6,34 @@
 // head size 256, whose output does not fit in TMEM beside the scores, take one
 // warp a row and head.
 //
-// Tensor-core kernel: a CTA takes 256 query rows of one head and sequence as
-// two tiles of 128, and walks the sequence's keys 128 at a time up to the
-// diagonal.
+// Tensor-core kernel: persistent CTAs, one an SM; an item of work is 256 query
+// rows of one head and sequence, as two tiles of 128, which walk the sequence's
+// keys 128 at a time up to the diagonal.
 //   S_t = Q_t K^T    tcgen05.mma, Q_t and K from shared memory, S_t in TMEM
 //   P_t = 2^(c S_t - m)   a thread a row: it reads its row of S_t, keeps the
 //                    row's maximum m and sum l, and writes P_t (16 bits) over S_t
 //   O_t += P_t V     tcgen05.mma, P_t from TMEM, V from shared memory as it
 //                    lies (keys by dims: the transposed operand), O_t in TMEM
 // Warps 0-3 and 4-7 are the softmax of tile 0 and 1 (TMEM lane = query row),
-// warp 8 issues the MMAs, warp 9 the TMA loads of K and V into a ring of tiles
-// of 128 keys.  The two tiles alternate, so that the tensor core works on one
-// while the other's exponentials are taken: for head size 128 a pair of tiles
-// is 4 x 128^3 MACs, 2048 cycles of the tensor core, and 2 x 128^2
-// exponentials, 2048 cycles of the special-function units.
+// warps 8 and 9 issue the MMAs of tile 0 and 1, warp 10 the TMA loads of Q and of
+// K and V into a ring of tiles of 128 keys, warp 11 finds the items and checks V
+// (below).  All of them run on into the next item: its loads and first scores
+// are under way while the softmax warps write the rows of the last.
+// The two tiles alternate, so that the tensor core works on one while the
+// other's exponentials are taken: for head size 128 a pair of key tiles is
+// 4 x 128^3 MACs, 2048 cycles of the tensor core, and 2 x 128^2 exponentials,
+// 2048 cycles of the special-function units.  Those would set the pace, so a
+// part of the exponentials is a polynomial on the FMA units.
 // O_t is rescaled only when a row's maximum has grown by more than 2^8 since
 // the last time, which after the first key tiles is rare; P <= 256 loses no
 // precision, its rounding being relative.
 //
-// A masked place never counts: its P is an exact 0, and the values that are not
-// finite in a diagonal tile of V, the only ones with masked places, are set to 0
-// by warps 10 and 11 before the tensor core reads the tile.  The rows that do
-// see such a value, and any whose result is not finite, are taken again alone
-// over their own keys.
+// A masked place never counts.  Its P is an exact 0, which an infinite or NaN
+// value of V would still make NaN: where a row's result is not finite, the CTA
+// goes through its items a second time with care.  Then warp 11 sets the values
+// that are not finite in a diagonal tile of V, the only ones with masked places,
+// to 0 before the tensor core reads the tile, and the rows that do see such a
+// value, and any whose result is not finite still, are taken alone over their own keys.
 #include "holo_common.cuh"
 #include "mv_unit.cuh"
 #include "tc_util.cuh"
@@ -55,6 +60,7 @@ struct PackedArgs {
     int n_seqs, total, n_heads, group;
     float scale;
     long long q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;
+    int item_rows;                     // 256, or 128: one tile an item, where that many items are wanted
     int *status;
 };
 
@@ -128,7 +134,7 @@ constexpr int PK_ROWS = 128;           // query rows a tile (MMA M), keys a tile
 constexpr int PK_THREADS = 384;        // three warpgroups
 // registers a thread, of 384 * 168 at launch: 2 * 208 + 80 <= 3 * 168
 constexpr int PK_SOFTMAX_REGS = 208, PK_OTHER_REGS = 80;
-constexpr uint32_t PK_TMEM_COLS = 512; // S_0, S_1, O_0, O_1: 128 columns each
+constexpr uint32_t PK_TMEM_COLS = 512; // S_0, S_1, O_0, O_1: 128 columns each; all there are, so they begin at 0
 constexpr float PK_GROWTH = 8.0f;      // log2 of what a row's maximum may grow by before its O is rescaled
 constexpr int PK_STAGES = 5;           // ring of K and V tiles
 
@@ -137,11 +143,18 @@ template <int HD> struct PkGeom {
     static constexpr size_t SMEM = 1024 + (size_t)(2 + PK_STAGES) * TILE;
 };
 
+struct PkWork {
+    int first, len, row0, head;        // the sequence's first row and length; the item's first row in it; len 0: no more
+    int careful;
+};
+
 struct PkBars {
-    uint64_t q_full[2], s_full[2], p_full[2], o_done[2], kv_full[PK_STAGES], kv_empty[PK_STAGES], v_here[2], v_checked[2], drain;
+    uint64_t work_full[2], work_empty[2], q_full[2], q_empty[2], s_full[2], p_half[2], p_full[2], o_done[2], turn[2];
+    uint64_t kv_full[PK_STAGES], kv_empty[PK_STAGES], kv_checked[PK_STAGES], bad_known[2], drain[2];
+    PkWork work[2];
+    int bad_from[2];                   // of an item: first key of the diagonal tiles with a value that is not finite
+    int again;                         // a row's result was not finite
     uint32_t tmem;
-    int first, len, pair;              // the CTA's work: its sequence's first row and length, and 256-row tile
-    int bad_from;                      // first key of the diagonal tiles with a value that is not finite
 };
 
 __device__ __forceinline__ void pk_tma_load(void *dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar) {
@@ -150,12 +163,18 @@ __device__ __forceinline__ void pk_tma_load(void *dst, const CUtensorMap *map, i
         :: "r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar)) : "memory");
 }
 
-// descriptor of an MN-major, 128-byte-swizzled operand of 128 K rows: a K row
-// is 128 bytes (64 MN values), 8 of them 1024 bytes (SBO), the next 64 MN
-// values 128 rows on (LBO)
-__device__ __forceinline__ uint64_t pk_desc_mn(const void *smem) {
-    return (uint64_t)((smem_addr(smem) >> 4) & 0x3FFFu) | ((uint64_t)(PK_ROWS * 128 >> 4) << 16) |
-           ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+// Shared-memory descriptors without the address.  K-major (Q and K): as
+// sw128_desc.  MN-major, 128-byte-swizzled, of 128 K rows (V): a K row is 128
+// bytes (64 MN values), 8 of them 1024 bytes (SBO), the next 64 MN values 128
+// rows on (LBO).
+constexpr uint64_t PK_DESC_K = ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+constexpr uint64_t PK_DESC_MN = ((uint64_t)(PK_ROWS * 128 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
+                                ((uint64_t)2 << 61);
+
+__device__ __forceinline__ bool pk_elect() {
+    uint32_t p;
+    asm volatile("{.reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p;}" : "=r"(p));
+    return p != 0;
 }
 
 template <typename T> struct PkType;
@@ -228,25 +247,30 @@ __device__ __noinline__ void pk_row_alone(const PackedArgs &a, int row, int firs
     if (a.lse) a.lse[(size_t)h * a.total + row] = m + logf(l);
 }
 
-// The work of CTA group r (heads apart), longest first: the 256-row tiles of
-// all sequences in the order of their index, the highest first, and of the
-// sequences.  One warp; false if there are no more than r.
-__device__ __forceinline__ bool pk_find_work(const PackedArgs &a, int r, int &first, int &len, int &pair) {
-    const int lane = threadIdx.x & 31;
+// Item r of all, heads apart, longest first: the tiles of item_rows rows of all
+// sequences in the order of their index, the highest first, and of the
+// sequences.  One warp; false if there are no more than r.  `kept`: the lengths of the
+// first 256 sequences, eight a lane; `first0`: the first rows of the first 32.
+constexpr int PK_KEPT = 8;
+__device__ __forceinline__ int pk_len(const PackedArgs &a, int s) {
+    int first, len = 0;
+    if (s < a.n_seqs) packed_seq(a, s, first, len);
+    return len;
+}
+__device__ __forceinline__ bool pk_find_work(const PackedArgs &a, const int (&kept)[PK_KEPT], int first0, int r, PkWork &w) {
+    const int lane = threadIdx.x & 31, shift = a.item_rows == 2 * PK_ROWS ? 8 : 7;
+    auto tiles = [&](int len) { return (len + a.item_rows - 1) >> shift; };
     int longest = 0;
-    for (int s = lane; s < a.n_seqs; s += 32) {
-        packed_seq(a, s, first, len);
-        longest = max(longest, (len + 255) >> 8);
-    }
-    longest = __reduce_max_sync(0xffffffffu, longest);
+#pragma unroll
+    for (int i = 0; i < PK_KEPT; ++i) longest = max(longest, kept[i]);
+    for (int s = 32 * PK_KEPT + lane; s < a.n_seqs; s += 32) longest = max(longest, pk_len(a, s));
+    longest = tiles(__reduce_max_sync(0xffffffffu, longest));
     // tiles of index t or above, over all sequences
     auto from = [&](int t) {
         int n = 0;
-        for (int s = lane; s < a.n_seqs; s += 32) {
-            int f, l;
-            packed_seq(a, s, f, l);
-            n += max(0, ((l + 255) >> 8) - t);
-        }
+#pragma unroll
+        for (int i = 0; i < PK_KEPT; ++i) n += max(0, tiles(kept[i]) - t);
+        for (int s = 32 * PK_KEPT + lane; s < a.n_seqs; s += 32) n += max(0, tiles(pk_len(a, s)) - t);
         return __reduce_add_sync(0xffffffffu, n);
     };
     if (from(0) <= r) return false;
@@ -257,22 +281,38 @@ __device__ __forceinline__ bool pk_find_work(const PackedArgs &a, int r, int &fi
         if (n > r) lo = mid;
         else hi = mid, above = n;
     }
-    pair = lo;
+    w.row0 = lo << shift;
     int skip = r - above;       // of the sequences with a tile `lo`
     for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
-        int f = 0, l = 0;
-        if (s0 + lane < a.n_seqs) packed_seq(a, s0 + lane, f, l);
-        const unsigned has = __ballot_sync(0xffffffffu, ((l + 255) >> 8) > lo);
+        int mine = 0;
+        if (s0 < 32 * PK_KEPT) {
+#pragma unroll
+            for (int i = 0; i < PK_KEPT; ++i)
+                if (s0 == 32 * i) mine = kept[i];
+        } else {
+            mine = pk_len(a, s0 + lane);
+        }
+        const unsigned has = __ballot_sync(0xffffffffu, tiles(mine) > lo);
         const int n = __popc(has);
         if (skip < n) {
             const int src = __fns(has, 0, skip + 1);
-            first = __shfl_sync(0xffffffffu, f, src);
-            len = __shfl_sync(0xffffffffu, l, src);
+            if (s0 == 0) {
+                w.first = __shfl_sync(0xffffffffu, first0, src);
+                w.len = __shfl_sync(0xffffffffu, mine, src);
+            } else {
+                packed_seq(a, s0 + src, w.first, w.len);
+            }
             return true;
         }
         skip -= n;
     }
     return false;
+}
+
+__device__ __forceinline__ float pk_max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 
 template <typename T, int HD>
@@ -284,239 +324,402 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
     __shared__ PkBars B;
     uint8_t *sq = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(pk_smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t *skv = sq + 2 * G::TILE;
-    const int h = blockIdx.x % a.n_heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    early_wait();
-    early_next();
     if (warp == 0) {
-        int first = 0, len = 0, pair = -1;
-        if (!pk_find_work(a, blockIdx.x / a.n_heads, first, len, pair)) pair = -1;
-        if (lane == 0) B.first = first, B.len = len, B.pair = pair;
-        if (pair >= 0) tc_alloc(&B.tmem, PK_TMEM_COLS);
+        tc_alloc(&B.tmem, PK_TMEM_COLS);
     } else if (warp == 1 && lane == 0) {
         for (int t = 0; t < 2; ++t) {
+            mbar_init(&B.work_full[t], 1);
+            mbar_init(&B.work_empty[t], 11);   // warps 8-10 and the softmax's eight
             mbar_init(&B.q_full[t], 1);
+            mbar_init(&B.q_empty[t], 1);
             mbar_init(&B.s_full[t], 1);
+            mbar_init(&B.p_half[t], 128);
             mbar_init(&B.p_full[t], 128);
             mbar_init(&B.o_done[t], 1);
-            mbar_init(&B.v_here[t], 1);
-            mbar_init(&B.v_checked[t], 64);
+            mbar_init(&B.turn[t], 128);
+            mbar_init(&B.bad_known[t], 1);
+            mbar_init(&B.drain[t], 1);
         }
-        B.bad_from = 0x7fffffff;
         for (int i = 0; i < PK_STAGES; ++i) {
             mbar_init(&B.kv_full[i], 1);
-            mbar_init(&B.kv_empty[i], 1);
+            mbar_init(&B.kv_empty[i], 3);      // warps 8, 9 and 11 are through with it
+            mbar_init(&B.kv_checked[i], 1);
         }
-        mbar_init(&B.drain, 1);
+        B.again = 0;
         fence_barrier_init();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (B.pair < 0) return;
-    const int first = B.first, len = B.len, row0 = 256 * B.pair;       // rows of the sequence from row0 on
-    const int n0 = 2 * B.pair + 1, n1 = len > row0 + PK_ROWS ? n0 + 1 : 0;   // key tiles of the two query tiles
-    const int n = max(n0, n1);
     const uint32_t tmem = B.tmem;
+    early_wait();
+    early_next();
+
+    bool ok = true;
+    auto wait = [&](uint64_t *bar, int parity) {
+        ok = ok && mbar_wait_bounded(bar, parity & 1, a.status, HOLO_E_TIMEOUT);
+        return ok;
+    };
+    // item k's work, and the key tiles of its two query tiles
+    PkWork w;
+    int n0, n1, n;
+    auto next = [&](int k) {
+        if (!wait(&B.work_full[k & 1], k >> 1)) return false;
+        w = B.work[k & 1];
+        if (w.len == 0) return false;
+        n0 = w.row0 / PK_ROWS + 1;
+        n1 = a.item_rows > PK_ROWS && w.len > w.row0 + PK_ROWS ? n0 + 1 : 0;
+        n = max(n0, n1);
+        return true;
+    };
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PK_OTHER_REGS));
-        if (warp == 9 && lane == 0) {
+        if (warp == 10 && lane == 0) {
             // ---- loads: Q_0, K_0, Q_1, V_0, K_1, V_1, ... ----
-            const int kvh = h / a.group;
             auto load = [&](uint8_t *dst, const CUtensorMap *map, int head, int row, uint64_t *bar) {
                 mbar_arrive_expect_tx(bar, G::TILE);
 #pragma unroll
                 for (int x = 0; x < HD; x += 64) pk_tma_load(dst + x / 64 * (PK_ROWS * 128), map, x, head, row, bar);
             };
-            load(sq, &qmap, h, first + row0, &B.q_full[0]);
-            int i = 0;
-            bool ok = true;
-            for (; i < 2 * n; ++i) {
-                const int slot = i % PK_STAGES;
-                ok = mbar_wait_bounded(&B.kv_empty[slot], (i / PK_STAGES & 1) ^ 1, a.status, HOLO_E_TIMEOUT);
-                if (!ok) break;
-                load(skv + slot * G::TILE, i & 1 ? &vmap : &kmap, kvh, first + (i >> 1) * PK_ROWS, &B.kv_full[slot]);
-                if (i == 0 && n1) load(sq + G::TILE, &qmap, h, first + row0 + PK_ROWS, &B.q_full[1]);
+            int q[2] = {0, 0}, slot = 0, phase = 0, ahead = 0;   // Q tiles loaded, ring position, its tiles loaded in all
+            for (int k = 0; next(k); ++k) {
+                const int kvh = w.head / a.group;
+                auto load_q = [&](int t) {
+                    if (q[t] > 0 && !wait(&B.q_empty[t], q[t] + 1)) return;
+                    load(sq + t * G::TILE, &qmap, w.head, w.first + w.row0 + t * PK_ROWS, &B.q_full[t]);
+                    ++q[t];
+                };
+                load_q(0);
+                for (int i = 0; i < 2 * n && ok; ++i) {
+                    if (!wait(&B.kv_empty[slot], phase + 1)) break;
+                    load(skv + slot * G::TILE, i & 1 ? &vmap : &kmap, kvh, w.first + (i >> 1) * PK_ROWS, &B.kv_full[slot]);
+                    ++ahead;
+                    if (++slot == PK_STAGES) slot = 0, phase ^= 1;
+                    if (i == 0 && n1) load_q(1);
+                }
+                mbar_arrive(&B.work_empty[k & 1]);
             }
-            if (!ok)   // the loads in flight land before the CTA leaves
-                for (int k = max(0, i - PK_STAGES); k < i; ++k)
+            if (!ok) {   // the loads in flight land before the CTA leaves
+                for (int k = max(0, ahead - PK_STAGES); k < ahead; ++k)
                     mbar_wait_bounded(&B.kv_full[k % PK_STAGES], k / PK_STAGES & 1, a.status, HOLO_E_TIMEOUT);
-        } else if (warp == 8 && lane == 0) {
-            // ---- MMAs ----
+                for (int t = 0; t < 2; ++t)
+                    if (q[t] > 0) mbar_wait_bounded(&B.q_full[t], (q[t] - 1) & 1, a.status, HOLO_E_TIMEOUT);
+            }
+        } else if (warp < 10) {
+            // ---- MMAs of tile t ----
+            // The whole warp walks the items together, so that the descriptors stay uniform (a thread of its own would
+            // move each into uniform registers, at about the cost of the MMA); one lane issues.
             constexpr uint32_t id_s = tc_idesc_f16(PK_ROWS, PK_ROWS) | PkType<T>::AB;
             constexpr uint32_t id_o = tc_idesc_f16(PK_ROWS, HD) | PkType<T>::AB | 1u << 16;   // B transposed
-            bool ok = true;
-            auto wait = [&](uint64_t *bar, int parity) {
-                ok = ok && mbar_wait_bounded(bar, parity, a.status, HOLO_E_TIMEOUT);
-                tc_fence_after();
+            const int t = warp - 8;
+            const bool leader = pk_elect();
+            const uint32_t sq_at = __shfl_sync(0xffffffffu, smem_addr(sq) >> 4, 0), skv_at = sq_at + (2 * G::TILE >> 4);
+            int q = 0, it = 0;                     // Q tiles, key tiles so far
+            int slot = 0, phase = 0;               // of the next ring tile
+            auto wait_all = [&](uint64_t *bar, int parity) {
+                wait(bar, parity);
+                ok = __all_sync(0xffffffffu, ok);
                 return ok;
             };
-            auto wait_kv = [&](int i) { return wait(&B.kv_full[i % PK_STAGES], i / PK_STAGES & 1); };
-            auto scores = [&](int t, int j) {   // S_t = Q_t K_j^T
-                const uint64_t q = sw128_desc(sq + t * G::TILE), k = sw128_desc(skv + 2 * j % PK_STAGES * G::TILE);
-#pragma unroll
-                for (int s = 0; s < HD / 16; ++s) {
-                    const uint64_t off = (uint64_t)(((s >> 2) * (PK_ROWS * 128) + (s & 3) * 32) >> 4);
-                    tc_mma(tmem + t * 128, q + off, k + off, id_s, s > 0);
-                }
-                tc_commit(&B.s_full[t]);
+            auto commit = [&](uint64_t *bar) {
+                if (leader) tc_commit(bar);
             };
-            if (wait(&B.q_full[0], 0) && wait_kv(0)) scores(0, 0);
-            if (n1 && wait(&B.q_full[1], 0)) scores(1, 0);
-            if (ok) tc_commit(&B.kv_empty[0]);
-            for (int j = 0; j < n && ok; ++j) {
-                wait_kv(2 * j + 1);
-                if (j >= n0 - 1) mbar_arrive(&B.v_here[j - (n0 - 1)]);   // for its check
-#pragma unroll 1
-                for (int t = 0; t < 2; ++t) {
-                    const int nt = t ? n1 : n0;
-                    if (j >= nt) continue;
-                    if (j >= n0 - 1) wait(&B.v_checked[j - (n0 - 1)], 0);
-                    if (!wait(&B.p_full[t], j & 1)) break;
-                    const uint64_t v = pk_desc_mn(skv + (2 * j + 1) % PK_STAGES * G::TILE);
+            auto advance = [&]() {
+                if (++slot == PK_STAGES) slot = 0, phase ^= 1;
+            };
+            // S_t = Q_t K^T with the ring's next tile, once the last P_t, in the same columns, has been read
+            auto scores = [&]() {
+                if (!wait_all(&B.kv_full[slot], phase) || (it > 0 && !wait_all(&B.o_done[t], it + 1))) return;
+                tc_fence_after();
+                const uint64_t qd = PK_DESC_K | (uint64_t)(sq_at + t * (G::TILE >> 4));
+                const uint64_t kd = PK_DESC_K | (uint64_t)(skv_at + slot * (G::TILE >> 4));
+                if (leader) {
 #pragma unroll
-                    for (int s = 0; s < PK_ROWS / 16; ++s)   // 16 keys: 8 columns of P, 16 rows of V
-                        tc_mma_ts(tmem + 256 + t * 128, tmem + t * 128 + 8 * s, v + (uint64_t)(s * 2048 >> 4), id_o,
-                                  j > 0 || s > 0);
-                    tc_commit(&B.o_done[t]);
-                    if (t == 1 || !n1) tc_commit(&B.kv_empty[(2 * j + 1) % PK_STAGES]);
-                    if (j + 1 < nt) {
-                        // P_t and the next S_t share columns: P_t has been read first
-                        if (!wait_kv(2 * j + 2) || !wait(&B.o_done[t], j & 1)) break;
-                        scores(t, j + 1);
+                    for (int s = 0; s < HD / 16; ++s) {
+                        const uint64_t off = (uint64_t)(((s >> 2) * (PK_ROWS * 128) + (s & 3) * 32) >> 4);
+                        tc_mma(t * 128, qd + off, kd + off, id_s, s > 0);
                     }
-                    if ((t == 1 || !n1) && j + 1 < n) tc_commit(&B.kv_empty[(2 * j + 2) % PK_STAGES]);
+                    tc_commit(&B.s_full[t]);
+                    tc_commit(&B.kv_empty[slot]);
                 }
+                __syncwarp();
+                advance();
+            };
+            auto skip = [&]() {                    // a tile that only the other query tile reads
+                if (!wait_all(&B.kv_full[slot], phase)) return;
+                if (leader) mbar_arrive(&B.kv_empty[slot]);
+                advance();
+            };
+            for (int k = 0; ok; ++k) {
+                const bool more = next(k);
+                if (!__all_sync(0xffffffffu, more)) break;
+                const int nt = __shfl_sync(0xffffffffu, t ? n1 : n0, 0), tiles = __shfl_sync(0xffffffffu, n, 0);
+                // K_0, then V_j and K_(j+1) for every j
+                if (nt > 0) {
+                    if (!wait_all(&B.q_full[t], q++)) break;
+                    scores();
+                    if (nt == 1) commit(&B.q_empty[t]);
+                }
+                for (int j = 0; j < nt && ok; ++j) {
+                    const int v_slot = slot, v_phase = phase;
+                    advance();
+                    if (!wait_all(&B.kv_full[v_slot], v_phase)) break;
+                    if (w.careful && j >= n0 - 1 && !wait_all(&B.kv_checked[v_slot], v_phase)) break;
+                    const uint64_t v = PK_DESC_MN | (uint64_t)(skv_at + v_slot * (G::TILE >> 4));
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        if (!wait_all(half ? &B.p_full[t] : &B.p_half[t], it)) break;
+                        tc_fence_after();
+                        if (leader) {
+#pragma unroll
+                            for (int s = 4 * half; s < 4 * half + 4; ++s)   // 16 keys: 8 columns of P, 16 rows of V
+                                tc_mma_ts(256 + t * 128, t * 128 + 8 * s, v + (uint64_t)(s * 2048 >> 4), id_o, j > 0 || s > 0);
+                        }
+                        __syncwarp();
+                    }
+                    if (!ok) break;
+                    commit(&B.o_done[t]);
+                    commit(&B.kv_empty[v_slot]);
+                    ++it;
+                    if (j + 1 < nt) {
+                        scores();
+                        if (j + 2 == nt) commit(&B.q_empty[t]);
+                    }
+                }
+                for (int i = nt > 0 ? 2 * nt : 0; i < 2 * tiles && ok; ++i) skip();
+                if (lane == 0) mbar_arrive(&B.work_empty[k & 1]);
             }
             if (!ok) {   // the MMAs in flight end before the CTA leaves
-                tc_commit(&B.drain);
-                mbar_wait_bounded(&B.drain, 0, a.status, HOLO_E_TIMEOUT);
+                commit(&B.drain[t]);
+                mbar_wait_bounded(&B.drain[t], 0, a.status, HOLO_E_TIMEOUT);
             }
-        }
-        if (warp >= 10) {
-            // ---- diagonal tiles of V: no value that is not finite in a masked place ----
-            for (int j = n0 - 1; j < n; ++j) {
-                // (the ring's barrier alone would not do: its phase may be several before this tile's)
-                const int i = 2 * j + 1;
-                const bool ok = mbar_wait_bounded(&B.v_here[j - (n0 - 1)], 0, a.status, HOLO_E_TIMEOUT);
-                uint4 *tile = reinterpret_cast<uint4 *>(skv + i % PK_STAGES * G::TILE);
-                for (int e = threadIdx.x - 320; e < G::TILE / 16 && ok; e += 64) {
-                    uint4 w = tile[e];
-                    constexpr uint32_t X = PkType<T>::EXPONENT;
-                    const uint32_t b[4] = {__vcmpeq2(w.x & X, X), __vcmpeq2(w.y & X, X), __vcmpeq2(w.z & X, X),
-                                           __vcmpeq2(w.w & X, X)};
-                    if (b[0] | b[1] | b[2] | b[3]) {
-                        tile[e] = make_uint4(w.x & ~b[0], w.y & ~b[1], w.z & ~b[2], w.w & ~b[3]);
-                        const int key = j * PK_ROWS + (e & (PK_ROWS * 8 - 1)) / 8;   // 8 pieces of 16 bytes a key
-                        if (key < len) atomicMin(&B.bad_from, key);
+        } else if (warp == 11) {
+            // ---- items: every gridDim.x-th, the order turned round each time so that the sums are even ----
+            int kept[PK_KEPT], first0 = 0;
+            kept[0] = 0;
+            if (lane < a.n_seqs) packed_seq(a, lane, first0, kept[0]);
+#pragma unroll
+            for (int i = 1; i < PK_KEPT; ++i) kept[i] = pk_len(a, 32 * i + lane);
+            int published = 0, base = 0;           // items so far, and of them before this pass
+            bool more = true, careful = false;
+            auto publish = [&](PkWork &mine) {
+                if (published >= 2) wait(&B.work_empty[published & 1], (published >> 1) + 1);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) return;
+                mine.careful = careful;
+                if (lane == 0) {
+                    B.work[published & 1] = mine;
+                    B.bad_from[published & 1] = 0x7fffffff;
+                    mbar_arrive(&B.work_full[published & 1]);
+                }
+                __syncwarp();
+                ++published;
+            };
+            auto find = [&]() {
+                if (!more) return;
+                const int round = published - base;
+                const long long r = (long long)round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+                const int tile = (int)(r / a.n_heads);
+                PkWork mine;
+                mine.head = (int)(r - (long long)tile * a.n_heads);
+                more = pk_find_work(a, kept, first0, tile, mine);   // past the end: none follows
+                if (more) publish(mine);
+            };
+            find();
+            find();
+            int slot = 0, phase = 0;
+            for (int k = 0; ok; ++k) {
+                if (k == published) {
+                    // The end of a pass.  Once the last item is through: is one with care wanted?
+                    if (k > 0 && !careful) {
+                        wait(&B.work_empty[(k - 1) & 1], (k - 1) >> 1);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (ok && *(volatile int *)&B.again) {
+                            careful = more = true;
+                            base = published;
+                            find();
+                            find();
+                        }
+                    }
+                    if (k == published) {
+                        PkWork none = {0, 0, 0, 0, 0};
+                        publish(none);
+                        break;
                     }
                 }
-                holo_mv::fence_proxy_async_smem();
-                mbar_arrive(&B.v_checked[j - (n0 - 1)]);
+                if (!next(k)) break;
+                for (int i = 0; i < 2 * n; ++i) {   // every tile of the ring, so that no phase is missed
+                    wait(&B.kv_full[slot], phase);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    const int j = i >> 1;
+                    if (careful && (i & 1) && j >= n0 - 1) {
+                        // a diagonal tile of V: no value that is not finite in a masked place
+                        uint4 *tile = reinterpret_cast<uint4 *>(skv + slot * G::TILE);
+                        constexpr uint32_t X = PkType<T>::EXPONENT;
+#pragma unroll 4
+                        for (int e = lane; e < G::TILE / 16; e += 32) {
+                            const uint4 v = tile[e];
+                            const uint32_t b[4] = {__vcmpeq2(v.x & X, X), __vcmpeq2(v.y & X, X), __vcmpeq2(v.z & X, X),
+                                                   __vcmpeq2(v.w & X, X)};
+                            if (b[0] | b[1] | b[2] | b[3]) {
+                                tile[e] = make_uint4(v.x & ~b[0], v.y & ~b[1], v.z & ~b[2], v.w & ~b[3]);
+                                const int key = j * PK_ROWS + (e & (PK_ROWS * 8 - 1)) / 8;   // 8 pieces of 16 bytes a key
+                                if (key < w.len) atomicMin(&B.bad_from[k & 1], key);
+                            }
+                        }
+                        holo_mv::fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                    if (lane == 0) {
+                        mbar_arrive(&B.kv_checked[slot]);
+                        mbar_arrive(&B.kv_empty[slot]);
+                    }
+                    if (++slot == PK_STAGES) slot = 0, phase ^= 1;
+                }
+                if (lane == 0) mbar_arrive(&B.bad_known[k & 1]);
+                if (ok) find();
             }
         }
         __syncwarp();
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PK_SOFTMAX_REGS));
-        const int t = warp >> 2, r = threadIdx.x & 127, nt = t ? n1 : n0;   // tile, row of the tile
+        const int t = warp >> 2, r = threadIdx.x & 127;   // tile, row of the tile
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t ts = tmem + t * 128 + lanes, to = tmem + 256 + t * 128 + lanes;
         const float c = a.scale * 1.4426950408889634f;
-        float m = -INFINITY;   // log2 of what P is scaled by
-        float l = 0.0f;
-        bool ok = true;
-        for (int j = 0; j < nt; ++j) {
-            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&B.s_full[t], j & 1, a.status, HOLO_E_TIMEOUT));
-            if (!ok) break;
-            tc_fence_after();
-            uint32_t s[2][64];
-            tc_ld64(ts, s[0]);
-            tc_ld64(ts + 64, s[1]);
-            if (j == nt - 1) {   // the diagonal: row r sees keys 0 .. r of the tile
-#pragma unroll
-                for (int i = 0; i < 128; ++i)
-                    if (i > r) s[i >> 6][i & 63] = 0xff800000u;
-            }
-            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int i = 0; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(s[i >> 6][i & 63]));
-            const float mn = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c);
-            const bool grow = mn > m + PK_GROWTH;
-            if (j == 0) {
-                m = mn;
-            } else if (__any_sync(0xffffffffu, grow)) {
-                const float fix = grow ? pk_ex2(m - mn) : 1.0f;
-                if (grow) m = mn;
-                l *= fix;
-                ok = __all_sync(0xffffffffu, mbar_wait_bounded(&B.o_done[t], (j - 1) & 1, a.status, HOLO_E_TIMEOUT));
-                if (!ok) break;
-                tc_fence_after();
-#pragma unroll 1
-                for (int cb = 0; cb < HD; cb += 32) {
-                    uint32_t o[32];
-                    tc_ld32(to + cb, o);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fix);
-                    tc_st32(to + cb, o);
-                }
-            }
-            const float sub = m == -INFINITY ? 0.0f : m;   // nothing but -inf so far: weights 0
-            const uint64_t c2 = pk_pair(c, c), sub2 = pk_pair(-sub, -sub);
-            uint64_t sum[2] = {0, 0};
-            uint32_t p[64];
-#pragma unroll
-            for (int i = 0; i < 64; ++i) {
-                float x, y;
-                pk_split(pk_fma2(pk_pair(__uint_as_float(s[i >> 5][2 * i & 63]), __uint_as_float(s[i >> 5][(2 * i + 1) & 63])), c2,
-                                 sub2), x, y);
-                x = pk_ex2(x);
-                y = pk_ex2(y);
-                sum[i & 1] = pk_add2(sum[i & 1], pk_pair(x, y));
-                p[i] = PkType<T>::pack(x, y);
-            }
-            tc_st32(ts, p);
-            tc_st32(ts + 32, p + 32);
-            float x, y;
-            pk_split(pk_add2(sum[0], sum[1]), x, y);
-            l += x + y;
-            tc_fence_before();
-            mbar_arrive(&B.p_full[t]);
-        }
-        // ---- O_t / l to the rows ----
-        if (nt > 0 && ok) {
-            ok = mbar_wait_bounded(&B.o_done[t], (nt - 1) & 1, a.status, HOLO_E_TIMEOUT);
-            for (int i = 0; i < nt - (n0 - 1) && ok; ++i)
-                ok = mbar_wait_bounded(&B.v_checked[i], 0, a.status, HOLO_E_TIMEOUT);
+        int it = 0, turns = 0;             // key tiles, and turns of the exponentials, so far
+        // a wait of the whole warp
+        auto wait_warp = [&](uint64_t *bar, int parity) {
+            wait(bar, parity);
             ok = __all_sync(0xffffffffu, ok);
-        }
-        if (nt > 0 && ok) {
             tc_fence_after();
-            const int i = row0 + t * PK_ROWS + r, row = first + i;
-            const bool mine = i < len;
-            const float inv = 1.0f / l;
-            T *o = (T *)a.out + (mine ? row * a.out_row : 0) + h * a.out_head;
-            bool finite = i < B.bad_from;
+            return ok;
+        };
+        for (int k = 0;; ++k) {
+            const bool more = next(k);
+            if (!__all_sync(0xffffffffu, more)) break;
+            const int nt = t ? n1 : n0;
+            float m = -INFINITY;           // log2 of what P is scaled by
+            float l = 0.0f;
+            for (int j = 0; j < nt; ++j, ++it) {
+                if (!wait_warp(&B.s_full[t], it)) break;
+                uint32_t s[2][64];
+                tc_ld64(ts, s[0]);
+                tc_ld64(ts + 64, s[1]);
+                if (j == nt - 1) {         // the diagonal: row r sees keys 0 .. r of the tile
 #pragma unroll
-            for (int cb = 0; cb < HD; cb += 32) {
-                uint32_t v[32];
-                tc_ld32(to + cb, v);
-#pragma unroll
-                for (int k = 0; k < 32; k += 8) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float x = __uint_as_float(v[k + 2 * e]) * inv, y = __uint_as_float(v[k + 2 * e + 1]) * inv;
-                        finite = finite && isfinite(x) && isfinite(y);
-                        w[e] = PkType<T>::pack(x, y);
-                    }
-                    if (mine) *reinterpret_cast<uint4 *>(o + cb + k) = make_uint4(w[0], w[1], w[2], w[3]);
+                    for (int i = 0; i < 128; ++i)
+                        if (i > r) s[i >> 6][i & 63] = 0xff800000u;
                 }
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < 128; i += 2)
+                    top[i / 2 & 3] = pk_max3(top[i / 2 & 3], __uint_as_float(s[i >> 6][i & 63]),
+                                             __uint_as_float(s[i >> 6][(i + 1) & 63]));
+                const float mn = fmaxf(m, pk_max3(fmaxf(top[0], top[1]), top[2], top[3]) * c);
+                const bool grow = mn > m + PK_GROWTH;
+                if (j == 0) {
+                    m = mn;
+                } else if (__any_sync(0xffffffffu, grow)) {
+                    const float fix = grow ? pk_ex2(m - mn) : 1.0f;
+                    if (grow) m = mn;
+                    l *= fix;
+                    if (!wait_warp(&B.o_done[t], it + 1)) break;   // (of the tile before)
+#pragma unroll 1
+                    for (int cb = 0; cb < HD; cb += 32) {
+                        uint32_t o[32];
+                        tc_ld32(to + cb, o);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fix);
+                        tc_st32(to + cb, o);
+                    }
+                }
+                const float sub = m == -INFINITY ? 0.0f : m;   // nothing but -inf so far: weights 0
+                const uint64_t c2 = pk_pair(c, c);
+                uint64_t sub2 = pk_pair(-sub, -sub), sum[2] = {0, 0};
+                // The two tiles take turns at the exponentials, so that one's run beside the other's MMAs: left alone, the
+                // two fall into step, and the units into turns.
+                const bool paired = n1 > 0 && j < n0;
+                if (paired && (t == 1 || turns > 0) && !wait_warp(&B.turn[t], turns + t + 1)) break;
+                asm volatile("" : "+l"(sub2));   // not before the turn has come
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t p[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const uint64_t z = pk_fma2(pk_pair(__uint_as_float(s[half][2 * i]), __uint_as_float(s[half][2 * i + 1])), c2, sub2);
+                        float x, y;
+                        pk_split(z, x, y);
+                        x = pk_ex2(x);
+                        y = pk_ex2(y);
+                        sum[i & 1] = pk_add2(sum[i & 1], pk_pair(x, y));
+                        p[i] = PkType<T>::pack(x, y);
+                    }
+                    tc_st32(ts + 32 * half, p);
+                    if (half && paired) {          // (after the store, which needs them all)
+                        mbar_arrive(&B.turn[t ^ 1]);
+                        ++turns;
+                    }
+                    tc_fence_before();
+                    mbar_arrive(half ? &B.p_full[t] : &B.p_half[t]);
+                }
+                float x, y;
+                pk_split(pk_add2(sum[0], sum[1]), x, y);
+                l += x + y;
             }
-            if (mine) {
-                if (!finite) pk_row_alone<T, HD>(a, row, first, h);
-                else if (a.lse) a.lse[(size_t)h * a.total + row] = (m + log2f(l)) * 0.6931471805599453f;
+            if (!ok) break;
+            // ---- O_t / l to the rows ----
+            if (nt > 0) {
+                if (w.careful) wait(&B.bad_known[k & 1], k >> 1);
+                if (!wait_warp(&B.o_done[t], it + 1)) break;
+                const int i = w.row0 + t * PK_ROWS + r;   // of the sequence
+                const float inv = 1.0f / l;
+                bool finite = !w.careful || i < B.bad_from[k & 1];
+                // 32 values a lane at a time; four lanes turn their 16-byte pieces round, so that they store 64 bytes of a row
+                const int part = lane & 3, i4 = i - part, n4 = w.len - i4;   // the first row of the four, rows from it on
+                T *o = (T *)a.out + (size_t)(w.first + min(i4, w.len - 1)) * a.out_row + (size_t)w.head * a.out_head + 8 * part;
+#pragma unroll
+                for (int cb = 0; cb < HD; cb += 32) {
+                    uint32_t v[32];
+                    tc_ld32(to + cb, v);
+                    uint32_t u[4][4];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float x = __uint_as_float(v[2 * e]) * inv, y = __uint_as_float(v[2 * e + 1]) * inv;
+                        finite = finite && isfinite(x) && isfinite(y);
+                        u[e >> 2][e & 3] = PkType<T>::pack(x, y);
+                    }
+#pragma unroll
+                    for (int bit = 1; bit < 4; bit <<= 1)
+#pragma unroll
+                        for (int p = 0; p < 4; ++p)
+                            if (!(p & bit)) {
+                                const bool up = (lane & bit) != 0;
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? u[p][e] : u[p | bit][e], bit);
+                                    if (up) u[p][e] = got;
+                                    else u[p | bit][e] = got;
+                                }
+                            }
+#pragma unroll
+                    for (int p = 0; p < 4; ++p)
+                        if (p < n4) *reinterpret_cast<uint4 *>(o + p * a.out_row + cb) = make_uint4(u[p][0], u[p][1], u[p][2], u[p][3]);
+                }
+                __syncwarp();              // a row is written by four lanes
+                if (i < w.len) {
+                    if (!finite && !w.careful) B.again = 1;
+                    else if (!finite) pk_row_alone<T, HD>(a, w.first + i, w.first, w.head);
+                    if (finite && a.lse) a.lse[(size_t)w.head * a.total + w.first + i] = (m + log2f(l)) * 0.6931471805599453f;
+                }
+                __syncwarp();
             }
+            tc_fence_before();             // O_t has been read before the next item's P_t is announced
+            if (lane == 0) mbar_arrive(&B.work_empty[k & 1]);
         }
     }
     tc_fence_before();
@@ -571,11 +774,13 @@ bool launch_tc(const PackedArgs &a, int type, cudaStream_t st) {
             return false;
         if (dev < 16) configured[dev] = true;
     }
-    // at most this many 256-row tiles over all sequences; a CTA without one leaves
-    const long long pairs = ((long long)a.total + 255LL * a.n_seqs) / 256;
-    const long long grid = pairs * a.n_heads;
-    if (grid > 0x7fffffffLL) return false;
-    return holo_launch_early(packed_tc_kernel<T, HD>, (unsigned)grid, PK_THREADS, PkGeom<HD>::SMEM, st, a, qm, km, vm) == cudaSuccess;
+    // at most this many items; where pairs of tiles would leave SMs without one, single tiles
+    PackedArgs w = a;
+    const int sms = holo_dev()->sms;
+    auto items = [&](int rows) { return ((long long)a.total + (long long)(rows - 1) * a.n_seqs) / rows * a.n_heads; };
+    w.item_rows = items(2 * PK_ROWS) >= sms ? 2 * PK_ROWS : PK_ROWS;
+    const unsigned grid = (unsigned)min((long long)sms, items(w.item_rows));
+    return holo_launch_early(packed_tc_kernel<T, HD>, grid, PK_THREADS, PkGeom<HD>::SMEM, st, w, qm, km, vm) == cudaSuccess;
 }
 
 // whether TMA can address rows of this base and these strides (elements)
