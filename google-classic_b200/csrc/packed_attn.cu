@@ -8,22 +8,24 @@
 //
 // Tensor-core kernel: persistent CTAs, one an SM; an item of work is 256 query
 // rows of one head and sequence, as two tiles of 128, which walk the sequence's
-// keys 128 at a time up to the diagonal.
+// keys in steps of 64 up to the diagonal.
 //   S_t = Q_t K^T    tcgen05.mma, Q_t and K from shared memory, S_t in TMEM
 //   P_t = 2^(c S_t - m)   a thread a row: it reads its row of S_t, keeps the
 //                    row's maximum m and sum l, and writes P_t (16 bits) over S_t
 //   O_t += P_t V     tcgen05.mma, P_t from TMEM, V from shared memory as it
 //                    lies (keys by dims: the transposed operand), O_t in TMEM
+// TMEM holds O_0, O_1 and two S of 64 keys for each tile, so that a step's
+// scores are there before the softmax of the step before ends, and neither the
+// softmax nor the tensor core waits through the other's latency.  (Steps of 128
+// keys leave room for one S a tile: then each tile's chain, softmax 2000 cycles, P V,
+// 290 to its end, Q K^T, 350 to its reader, sets the pace, 4100 cycles a pair of
+// tiles; their MMAs are 2048.  At N = 64 Q K^T is bound by shared memory, 48 cycles
+// an MMA and not 32: 2560 cycles.)
 // Warps 0-3 and 4-7 are the softmax of tile 0 and 1 (TMEM lane = query row),
 // warps 8 and 9 issue the MMAs of tile 0 and 1, warp 10 the TMA loads of Q and of
 // K and V into a ring of tiles of 128 keys, warp 11 finds the items and checks V
 // (below).  All of them run on into the next item: its loads and first scores
 // are under way while the softmax warps write the rows of the last.
-// The two tiles alternate, so that the tensor core works on one while the
-// other's exponentials are taken: for head size 128 a pair of key tiles is
-// 4 x 128^3 MACs, 2048 cycles of the tensor core, and 2 x 128^2 exponentials,
-// 2048 cycles of the special-function units.  Those would set the pace, so a
-// part of the exponentials is a polynomial on the FMA units.
 // O_t is rescaled only when a row's maximum has grown by more than 2^8 since
 // the last time, which after the first key tiles is rare; P <= 256 loses no
 // precision, its rounding being relative.
@@ -130,11 +132,12 @@ void launch_simple(const PackedArgs &a, int hd, cudaStream_t st) {
 // ---------------------------------------------------------------------------
 // tensor-core kernel
 // ---------------------------------------------------------------------------
-constexpr int PK_ROWS = 128;           // query rows a tile (MMA M), keys a tile (MMA N of S, K of P V)
+constexpr int PK_ROWS = 128;           // query rows a tile (MMA M), keys a tile of the ring
+constexpr int PK_STEP = 64;            // keys a step (MMA N of S, K of P V)
 constexpr int PK_THREADS = 384;        // three warpgroups
 // registers a thread, of 384 * 168 at launch: 2 * 208 + 80 <= 3 * 168
 constexpr int PK_SOFTMAX_REGS = 208, PK_OTHER_REGS = 80;
-constexpr uint32_t PK_TMEM_COLS = 512; // S_0, S_1, O_0, O_1: 128 columns each; all there are, so they begin at 0
+constexpr uint32_t PK_TMEM_COLS = 512; // two S_0, two S_1 (64 columns each), O_0, O_1 (128): all, so they begin at 0
 constexpr float PK_GROWTH = 8.0f;      // log2 of what a row's maximum may grow by before its O is rescaled
 constexpr int PK_STAGES = 5;           // ring of K and V tiles
 
@@ -149,7 +152,7 @@ struct PkWork {
 };
 
 struct PkBars {
-    uint64_t work_full[2], work_empty[2], q_full[2], q_empty[2], s_full[2], p_half[2], p_full[2], o_done[2], turn[2];
+    uint64_t work_full[2], work_empty[2], q_full[2], q_empty[2], s_full[2][2], p_full[2][2], o_done[2][2];
     uint64_t kv_full[PK_STAGES], kv_empty[PK_STAGES], kv_checked[PK_STAGES], bad_known[2], drain[2];
     PkWork work[2];
     int bad_from[2];                   // of an item: first key of the diagonal tiles with a value that is not finite
@@ -334,11 +337,11 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
             mbar_init(&B.work_empty[t], 11);   // warps 8-10 and the softmax's eight
             mbar_init(&B.q_full[t], 1);
             mbar_init(&B.q_empty[t], 1);
-            mbar_init(&B.s_full[t], 1);
-            mbar_init(&B.p_half[t], 128);
-            mbar_init(&B.p_full[t], 128);
-            mbar_init(&B.o_done[t], 1);
-            mbar_init(&B.turn[t], 128);
+            for (int b = 0; b < 2; ++b) {
+                mbar_init(&B.s_full[t][b], 1);
+                mbar_init(&B.p_full[t][b], 128);
+                mbar_init(&B.o_done[t][b], 1);
+            }
             mbar_init(&B.bad_known[t], 1);
             mbar_init(&B.drain[t], 1);
         }
@@ -358,13 +361,19 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
     early_next();
 
     bool ok = true;
+    // waits for a phase by its parity: it is the barrier's last but, at most, the one under way
     auto wait = [&](uint64_t *bar, int parity) {
         ok = ok && mbar_wait_bounded(bar, parity & 1, a.status, HOLO_E_TIMEOUT);
         return ok;
     };
     // item k's work, and the key tiles of its two query tiles
-    PkWork w;
-    int n0, n1, n;
+    PkWork w = {};
+    int n0 = 0, n1 = 0, n = 0;
+    // steps of query tile t: the diagonal key tile's second half is for its rows from 64 on
+    auto steps = [&](int t) {
+        const int nt = t ? n1 : n0;
+        return nt == 0 ? 0 : 2 * nt - (w.len - w.row0 - t * PK_ROWS <= PK_STEP);
+    };
     auto next = [&](int k) {
         if (!wait(&B.work_full[k & 1], k >> 1)) return false;
         w = B.work[k & 1];
@@ -412,12 +421,13 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
             // ---- MMAs of tile t ----
             // The whole warp walks the items together, so that the descriptors stay uniform (a thread of its own would
             // move each into uniform registers, at about the cost of the MMA); one lane issues.
-            constexpr uint32_t id_s = tc_idesc_f16(PK_ROWS, PK_ROWS) | PkType<T>::AB;
+            constexpr uint32_t id_s = tc_idesc_f16(PK_ROWS, PK_STEP) | PkType<T>::AB;
             constexpr uint32_t id_o = tc_idesc_f16(PK_ROWS, HD) | PkType<T>::AB | 1u << 16;   // B transposed
+            constexpr uint32_t HALF = PK_STEP * 128 >> 4;   // 64 rows of a 128-byte-wide tile, in a descriptor
             const int t = warp - 8;
             const bool leader = pk_elect();
             const uint32_t sq_at = __shfl_sync(0xffffffffu, smem_addr(sq) >> 4, 0), skv_at = sq_at + (2 * G::TILE >> 4);
-            int q = 0, it = 0;                     // Q tiles, key tiles so far
+            int q = 0, it = 0;                     // Q tiles, steps so far
             int slot = 0, phase = 0;               // of the next ring tile
             auto wait_all = [&](uint64_t *bar, int parity) {
                 wait(bar, parity);
@@ -430,66 +440,80 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
             auto advance = [&]() {
                 if (++slot == PK_STAGES) slot = 0, phase ^= 1;
             };
-            // S_t = Q_t K^T with the ring's next tile, once the last P_t, in the same columns, has been read
-            auto scores = [&]() {
-                if (!wait_all(&B.kv_full[slot], phase) || (it > 0 && !wait_all(&B.o_done[t], it + 1))) return;
+            // S of step x of all: Q_t and half h of the K tile in slot kv
+            auto scores = [&](int x, int kv, int h) {
                 tc_fence_after();
                 const uint64_t qd = PK_DESC_K | (uint64_t)(sq_at + t * (G::TILE >> 4));
-                const uint64_t kd = PK_DESC_K | (uint64_t)(skv_at + slot * (G::TILE >> 4));
+                const uint64_t kd = PK_DESC_K | (uint64_t)(skv_at + kv * (G::TILE >> 4) + h * HALF);
                 if (leader) {
 #pragma unroll
                     for (int s = 0; s < HD / 16; ++s) {
                         const uint64_t off = (uint64_t)(((s >> 2) * (PK_ROWS * 128) + (s & 3) * 32) >> 4);
-                        tc_mma(t * 128, qd + off, kd + off, id_s, s > 0);
+                        tc_mma(t * 128 + (x & 1) * PK_STEP, qd + off, kd + off, id_s, s > 0);
                     }
-                    tc_commit(&B.s_full[t]);
-                    tc_commit(&B.kv_empty[slot]);
+                    tc_commit(&B.s_full[t][x & 1]);
                 }
                 __syncwarp();
-                advance();
-            };
-            auto skip = [&]() {                    // a tile that only the other query tile reads
-                if (!wait_all(&B.kv_full[slot], phase)) return;
-                if (leader) mbar_arrive(&B.kv_empty[slot]);
-                advance();
             };
             for (int k = 0; ok; ++k) {
                 const bool more = next(k);
                 if (!__all_sync(0xffffffffu, more)) break;
-                const int nt = __shfl_sync(0xffffffffu, t ? n1 : n0, 0), tiles = __shfl_sync(0xffffffffu, n, 0);
+                const int ns = __shfl_sync(0xffffffffu, steps(t), 0), tiles = __shfl_sync(0xffffffffu, n, 0);
+                int k_slot = 0, v_slot = 0;
                 // K_0, then V_j and K_(j+1) for every j
-                if (nt > 0) {
-                    if (!wait_all(&B.q_full[t], q++)) break;
-                    scores();
-                    if (nt == 1) commit(&B.q_empty[t]);
-                }
-                for (int j = 0; j < nt && ok; ++j) {
-                    const int v_slot = slot, v_phase = phase;
+                if (ns > 0) {
+                    if (!wait_all(&B.q_full[t], q++) || !wait_all(&B.kv_full[slot], phase)) break;
+                    k_slot = slot;
+                    // the S that these write were read, as P, by the last steps of the item before
+                    if (it > 1 && !wait_all(&B.o_done[t][it & 1], (it >> 1) + 1)) break;
+                    scores(it, k_slot, 0);
+                    if (ns > 1) {
+                        if (it > 0 && !wait_all(&B.o_done[t][(it + 1) & 1], ((it + 1) >> 1) + 1)) break;
+                        scores(it + 1, k_slot, 1);
+                    }
+                    commit(&B.kv_empty[k_slot]);
+                    if (ns <= 2) commit(&B.q_empty[t]);
                     advance();
-                    if (!wait_all(&B.kv_full[v_slot], v_phase)) break;
-                    if (w.careful && j >= n0 - 1 && !wait_all(&B.kv_checked[v_slot], v_phase)) break;
-                    const uint64_t v = PK_DESC_MN | (uint64_t)(skv_at + v_slot * (G::TILE >> 4));
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        if (!wait_all(half ? &B.p_full[t] : &B.p_half[t], it)) break;
-                        tc_fence_after();
-                        if (leader) {
-#pragma unroll
-                            for (int s = 4 * half; s < 4 * half + 4; ++s)   // 16 keys: 8 columns of P, 16 rows of V
-                                tc_mma_ts(256 + t * 128, t * 128 + 8 * s, v + (uint64_t)(s * 2048 >> 4), id_o, j > 0 || s > 0);
-                        }
-                        __syncwarp();
+                }
+                for (int x = 0; x < ns && ok; ++x, ++it) {
+                    const int h = x & 1;
+                    if (h == 0) {
+                        v_slot = slot;
+                        if (!wait_all(&B.kv_full[v_slot], phase)) break;
+                        if (w.careful && x / 2 >= n0 - 1 && !wait_all(&B.kv_checked[v_slot], phase)) break;
+                        advance();
                     }
-                    if (!ok) break;
-                    commit(&B.o_done[t]);
-                    commit(&B.kv_empty[v_slot]);
-                    ++it;
-                    if (j + 1 < nt) {
-                        scores();
-                        if (j + 2 == nt) commit(&B.q_empty[t]);
+                    if (!wait_all(&B.p_full[t][it & 1], it >> 1)) break;
+                    tc_fence_after();
+                    const uint64_t v = PK_DESC_MN | (uint64_t)(skv_at + v_slot * (G::TILE >> 4) + h * HALF);
+                    if (leader) {
+#pragma unroll
+                        for (int s = 0; s < PK_STEP / 16; ++s)   // 16 keys: 8 columns of P, 16 rows of V
+                            tc_mma_ts(256 + t * 128, t * 128 + (it & 1) * PK_STEP + 8 * s, v + (uint64_t)(s * 2048 >> 4), id_o,
+                                      x > 0 || s > 0);
+                        tc_commit(&B.o_done[t][it & 1]);
+                        if (h || x + 1 == ns) tc_commit(&B.kv_empty[v_slot]);
+                    }
+                    __syncwarp();
+                    if (x + 2 < ns) {
+                        if (h == 0) {
+                            k_slot = slot;
+                            if (!wait_all(&B.kv_full[k_slot], phase)) break;
+                            advance();
+                        }
+                        // P of this step and the next S but one share columns: P has been read first
+                        if (!wait_all(&B.o_done[t][it & 1], it >> 1)) break;
+                        scores(it, k_slot, h);
+                        if (h || x + 3 == ns) commit(&B.kv_empty[k_slot]);
+                        if (x + 3 == ns) commit(&B.q_empty[t]);
                     }
                 }
-                for (int i = nt > 0 ? 2 * nt : 0; i < 2 * tiles && ok; ++i) skip();
+                // tiles that only the other query tile reads
+                for (int i = 2 * ((ns + 1) / 2); i < 2 * tiles && ok; ++i) {
+                    if (!wait_all(&B.kv_full[slot], phase)) break;
+                    if (leader) mbar_arrive(&B.kv_empty[slot]);
+                    advance();
+                }
                 if (lane == 0) mbar_arrive(&B.work_empty[k & 1]);
             }
             if (!ok) {   // the MMAs in flight end before the CTA leaves
@@ -591,7 +615,7 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t ts = tmem + t * 128 + lanes, to = tmem + 256 + t * 128 + lanes;
         const float c = a.scale * 1.4426950408889634f;
-        int it = 0, turns = 0;             // key tiles, and turns of the exponentials, so far
+        int it = 0;                        // steps so far
         // a wait of the whole warp
         auto wait_warp = [&](uint64_t *bar, int parity) {
             wait(bar, parity);
@@ -602,33 +626,34 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
         for (int k = 0;; ++k) {
             const bool more = next(k);
             if (!__all_sync(0xffffffffu, more)) break;
-            const int nt = t ? n1 : n0;
+            const int ns = steps(t);
             float m = -INFINITY;           // log2 of what P is scaled by
             float l = 0.0f;
-            for (int j = 0; j < nt; ++j, ++it) {
-                if (!wait_warp(&B.s_full[t], it)) break;
-                uint32_t s[2][64];
-                tc_ld64(ts, s[0]);
-                tc_ld64(ts + 64, s[1]);
-                if (j == nt - 1) {         // the diagonal: row r sees keys 0 .. r of the tile
+            for (int x = 0; x < ns; ++x, ++it) {
+                const uint32_t tb = ts + (it & 1) * PK_STEP;
+                if (!wait_warp(&B.s_full[t][it & 1], it >> 1)) break;
+                uint32_t s[PK_STEP];
+                tc_ld64(tb, s);
+                // the diagonal: row r sees keys 0 .. r of the tile
+                const int seen = r - (x * PK_STEP - (t ? n1 - 1 : n0 - 1) * PK_ROWS);
+                if (x / 2 == (t ? n1 : n0) - 1) {
 #pragma unroll
-                    for (int i = 0; i < 128; ++i)
-                        if (i > r) s[i >> 6][i & 63] = 0xff800000u;
+                    for (int i = 0; i < PK_STEP; ++i)
+                        if (i > seen) s[i] = 0xff800000u;
                 }
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int i = 0; i < 128; i += 2)
-                    top[i / 2 & 3] = pk_max3(top[i / 2 & 3], __uint_as_float(s[i >> 6][i & 63]),
-                                             __uint_as_float(s[i >> 6][(i + 1) & 63]));
+                for (int i = 0; i < PK_STEP; i += 2)
+                    top[i / 2 & 3] = pk_max3(top[i / 2 & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
                 const float mn = fmaxf(m, pk_max3(fmaxf(top[0], top[1]), top[2], top[3]) * c);
                 const bool grow = mn > m + PK_GROWTH;
-                if (j == 0) {
+                if (x == 0) {
                     m = mn;
                 } else if (__any_sync(0xffffffffu, grow)) {
                     const float fix = grow ? pk_ex2(m - mn) : 1.0f;
                     if (grow) m = mn;
                     l *= fix;
-                    if (!wait_warp(&B.o_done[t], it + 1)) break;   // (of the tile before)
+                    if (!wait_warp(&B.o_done[t][(it + 1) & 1], (it - 1) >> 1)) break;   // of the step before
 #pragma unroll 1
                     for (int cb = 0; cb < HD; cb += 32) {
                         uint32_t o[32];
@@ -639,43 +664,31 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
                     }
                 }
                 const float sub = m == -INFINITY ? 0.0f : m;   // nothing but -inf so far: weights 0
-                const uint64_t c2 = pk_pair(c, c);
-                uint64_t sub2 = pk_pair(-sub, -sub), sum[2] = {0, 0};
-                // The two tiles take turns at the exponentials, so that one's run beside the other's MMAs: left alone, the
-                // two fall into step, and the units into turns.
-                const bool paired = n1 > 0 && j < n0;
-                if (paired && (t == 1 || turns > 0) && !wait_warp(&B.turn[t], turns + t + 1)) break;
-                asm volatile("" : "+l"(sub2));   // not before the turn has come
+                const uint64_t c2 = pk_pair(c, c), sub2 = pk_pair(-sub, -sub);
+                uint64_t sum[2] = {0, 0};
+                uint32_t p[PK_STEP / 2];
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    uint32_t p[32];
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const uint64_t z = pk_fma2(pk_pair(__uint_as_float(s[half][2 * i]), __uint_as_float(s[half][2 * i + 1])), c2, sub2);
-                        float x, y;
-                        pk_split(z, x, y);
-                        x = pk_ex2(x);
-                        y = pk_ex2(y);
-                        sum[i & 1] = pk_add2(sum[i & 1], pk_pair(x, y));
-                        p[i] = PkType<T>::pack(x, y);
-                    }
-                    tc_st32(ts + 32 * half, p);
-                    if (half && paired) {          // (after the store, which needs them all)
-                        mbar_arrive(&B.turn[t ^ 1]);
-                        ++turns;
-                    }
-                    tc_fence_before();
-                    mbar_arrive(half ? &B.p_full[t] : &B.p_half[t]);
+                for (int i = 0; i < PK_STEP / 2; ++i) {
+                    const uint64_t z = pk_fma2(pk_pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), c2, sub2);
+                    float y0, y1;
+                    pk_split(z, y0, y1);
+                    y0 = pk_ex2(y0);
+                    y1 = pk_ex2(y1);
+                    sum[i & 1] = pk_add2(sum[i & 1], pk_pair(y0, y1));
+                    p[i] = PkType<T>::pack(y0, y1);
                 }
-                float x, y;
-                pk_split(pk_add2(sum[0], sum[1]), x, y);
-                l += x + y;
+                tc_st32(tb, p);
+                tc_fence_before();
+                mbar_arrive(&B.p_full[t][it & 1]);
+                float y0, y1;
+                pk_split(pk_add2(sum[0], sum[1]), y0, y1);
+                l += y0 + y1;
             }
             if (!ok) break;
             // ---- O_t / l to the rows ----
-            if (nt > 0) {
+            if (ns > 0) {
                 if (w.careful) wait(&B.bad_known[k & 1], k >> 1);
-                if (!wait_warp(&B.o_done[t], it + 1)) break;
+                if (!wait_warp(&B.o_done[t][(it + 1) & 1], (it - 1) >> 1)) break;
                 const int i = w.row0 + t * PK_ROWS + r;   // of the sequence
                 const float inv = 1.0f / l;
                 bool finite = !w.careful || i < B.bad_from[k & 1];
