@@ -33,21 +33,23 @@
 namespace {
 
 constexpr int AT_WARPS = 4, AT_THREADS = 32 * AT_WARPS;
-constexpr int AT_UNIT = 2;                     // blocks of 16 positions a unit
+constexpr int AT_UNIT = 4;                     // blocks of 16 positions a unit
 constexpr int AT_UNIT_POS = AT_UNIT * KV4_BLOCK;
-constexpr int AT_WHOLE = 16;                   // items of up to so many units are not cut
+constexpr int AT_WHOLE = 8;                    // items of up to so many units are not cut
+constexpr int AT_MIN = 4;                      // units a CTA: fewer cost more to join than they save
+constexpr int AT_ITEM = 4;                     // the cost of an item where CTAs take several
 constexpr float AT_GROWTH = 6.0f;              // log2 of what a maximum may grow by before the sums are rescaled
 constexpr int AT_SHIFT = 8;                    // weights times scales lie below 2 to this and AT_GROWTH: 2^14
 
 template <int HD> struct AtGeom {
     static constexpr int NB = HD / KV4_GROUP;
     static constexpr int BLOCK_BYTES = kv4_block_bytes(HD);
-    static constexpr int STAGES = HD == 64 ? 4 : 3;
+    static constexpr int STAGES = HD == 64 ? 3 : 2;
     static constexpr int RING = AT_WARPS * STAGES * AT_UNIT * BLOCK_BYTES;
     static constexpr int ROW = HD + 4;          // floats of a head in the join: its lanes' 16-byte stores spread over all banks
     static constexpr int JOIN = AT_WARPS * KV4_HEADS * ROW * 4;
     static constexpr int SMEM = RING + JOIN;
-    static constexpr int CTAS = HD == 256 ? 1 : 3;   // an SM
+    static constexpr int CTAS = HD == 256 ? 1 : HD == 128 ? 2 : 3;   // an SM
     static constexpr int SLOT = KV4_HEADS * (HD + 2);   // floats of a partial result: m and l of the heads, then the outputs
 };
 
@@ -57,6 +59,7 @@ struct AtArgs {
     long long q_row, out_row;
     const int *seqs;
     int n, n_heads, group, chunks;             // chunks of KV4_HEADS query heads a KV head
+    int item_cost;                             // what an item costs besides its units, in units: its q, the join
     float scale;
     uint32_t page_magic;                       // ceil(2^32 / page_blocks); 0 for 1
     bool wide;                                 // rows of out are 16-byte aligned
@@ -78,7 +81,9 @@ __device__ __forceinline__ void at_mma(float (&d)[4], uint32_t a0, uint32_t a1, 
 }
 __device__ __forceinline__ void at_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
-    at_mma(d, a0, a1, a2, a3, b0, b1, d[0], d[1], d[2], d[3]);
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t at_transpose(uint32_t x) {
     uint32_t y;
@@ -103,13 +108,14 @@ template <int N> __device__ __forceinline__ AtWords<N> at_lds(const uint8_t *p) 
     return r;
 }
 
-// The list of units: of every sequence, every (KV head, chunk of heads), its
-// units.  A walk through the CTA's part, item by item.
+// The list: of every sequence, every (KV head, chunk of heads), its units after
+// item_cost places that stand for the rest of its work.  A walk through the CTA's
+// part, item by item.
 struct Walk {
     int i, s, len, units;      // sequence: its place in the list, number, positions, units an item
     int item;                  // KV head * chunks + chunk
-    int first, take;           // units of the item in the part
-    int rest;                  // units of the part from `first` on
+    int start;                 // of the item in the list
+    int first, take;           // its units in the part
 };
 
 __device__ __forceinline__ int at_units(const Kv4View &c, const AtArgs &a, int i, int &s, int &len) {
@@ -122,23 +128,27 @@ __device__ __forceinline__ int at_units(const Kv4View &c, const AtArgs &a, int i
     len = max(0, min(__ldcg(c.lens + s), c.max_pages * c.page_tokens));
     return (len + AT_UNIT_POS - 1) / AT_UNIT_POS;
 }
-__device__ __forceinline__ void at_clip(Walk &w) { w.take = min(w.units - w.first, w.rest); }
-// the next item of the part; rest 0 at its end
-__device__ __forceinline__ void at_next(const Kv4View &c, const AtArgs &a, Walk &w) {
-    w.rest -= w.take;
-    w.first = w.take = 0;
-    if (w.rest <= 0) return;
-    if (++w.item == c.n_kv * a.chunks) {
-        w.item = 0;
-        do {
-            if (++w.i >= a.n) {
-                w.rest = 0;
-                return;
-            }
-            w.units = at_units(c, a, w.i, w.s, w.len);
-        } while (w.units == 0);
-    }
-    at_clip(w);
+// the item's units in [from, to) of the list
+__device__ __forceinline__ void at_clip(const AtArgs &a, Walk &w, int from, int to) {
+    w.first = max(0, from - w.start - a.item_cost);
+    w.take = max(0, min(w.units, to - w.start - a.item_cost) - w.first);
+}
+// the next item of the part [from, to) that has units in it; false: none
+__device__ __forceinline__ bool at_next(const Kv4View &c, const AtArgs &a, Walk &w, int from, int to) {
+    do {
+        w.start += w.units + a.item_cost;
+        w.first = w.take = 0;
+        if (w.start >= to) return false;
+        if (++w.item == c.n_kv * a.chunks) {
+            w.item = 0;
+            do {
+                if (++w.i >= a.n) return false;
+                w.units = at_units(c, a, w.i, w.s, w.len);
+            } while (w.units == 0);
+        }
+        at_clip(a, w, from, to);
+    } while (w.take == 0);
+    return true;
 }
 
 // inclusive sum over the CTA
@@ -161,14 +171,11 @@ __device__ __forceinline__ int at_scan(int v, int *sh, int &total) {
     return v;
 }
 
-// The list cut over `ctas` parts: the first `more` of them have one unit more than the others.
+// the list of `all` places cut evenly over `parts`
 struct Cuts {
-    int size, more;
-    __device__ __forceinline__ int begin(int part) const { return part * size + min(part, more); }
-    __device__ __forceinline__ int part_of(int unit) const {
-        const int big = more * (size + 1);
-        return unit < big ? unit / (size + 1) : more + (unit - big) / size;
-    }
+    int all, parts;
+    __device__ __forceinline__ int begin(int part) const { return (int)((long long)all * part / parts); }
+    __device__ __forceinline__ int part_of(int place) const { return (int)((((long long)place + 1) * parts - 1) / all); }
 };
 
 template <typename T>
@@ -222,7 +229,8 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
 
     // ---- the CTA's part of the list ----
     const int items = c.n_kv * a.chunks;
-    int all = 0, s0 = -1, len0 = 0, u0 = 0, end0 = 0;   // of thread's sequence in the last step of the sum
+    int all = 0, held = 0, s0 = -1, len0 = 0, u0 = 0, end0 = 0;   // s0 .. end0: of the thread's sequence in the last step
+    auto places = [&](int units) { return units ? (units + a.item_cost) * items : 0; };
     for (int i0 = 0; i0 < a.n; i0 += AT_THREADS) {
         const int i = i0 + threadIdx.x;
         u0 = 0, s0 = -1, len0 = 0;
@@ -231,18 +239,20 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
             if (s0 < 0 && blockIdx.x == 0) kv4_report(c.status, HOLO_E_ARG);
         }
         int total;
-        end0 = all + at_scan(u0 * items, scan, total);
+        end0 = all + at_scan(places(u0), scan, total);
         all += total;
+        held += __syncthreads_count(u0 > 0);
     }
-    // no more CTAs than leave each warp a unit
-    const int ctas = min((int)gridDim.x, max(1, (all + AT_WARPS - 1) / AT_WARPS));
+    // a CTA an item, or more where they keep AT_MIN units each
+    const int units = all - held * items * a.item_cost;
+    const int ctas = max(1, min(min((int)gridDim.x, units), max(held * items, units / AT_MIN)));
     if ((int)blockIdx.x >= ctas) {
         zeros();
         return;
     }
-    // Its part: the even cuts of the list, moved down to the item's start
+    // Its part: the cuts of the list, moved down to the item's start
     // where the item is short.  Cuts inside longer items stay, so that the parts that an item spans follow from them.
-    const Cuts cuts = {all / ctas, all % ctas};
+    const Cuts cuts = {all, ctas};
     const int cut0 = cuts.begin(blockIdx.x), cut1 = cuts.begin(blockIdx.x + 1);
     if (threadIdx.x == 0) part_start = 0, part_end = blockIdx.x + 1 == ctas ? all : 0;
     __syncthreads();
@@ -254,30 +264,34 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
                 u0 = 0, s0 = -1, len0 = 0;
                 if (i < a.n) u0 = at_units(c, a, i, s0, len0);
                 int total;
-                end0 = before + at_scan(u0 * items, scan, total);
+                end0 = before + at_scan(places(u0), scan, total);
                 before += total;
             }
-            const int start = end0 - u0 * items;
+            const int start = end0 - places(u0), item_places = u0 + a.item_cost;
             if (start <= cut0 && cut0 < end0) {
                 Walk w;
                 w.i = i0 + threadIdx.x, w.s = s0, w.len = len0, w.units = u0;
-                w.item = (cut0 - start) / u0;
-                w.first = u0 > AT_WHOLE ? cut0 - start - w.item * u0 : 0;
+                w.item = (cut0 - start) / item_places;
+                w.start = start + w.item * item_places;
                 begin = w;
-                part_start = start + w.item * u0 + w.first;
+                part_start = u0 > AT_WHOLE ? cut0 : w.start;
             }
-            if (start <= cut1 && cut1 < end0) part_end = u0 > AT_WHOLE ? cut1 : start + (cut1 - start) / u0 * u0;
+            if (start <= cut1 && cut1 < end0)
+                part_end = u0 > AT_WHOLE ? cut1 : start + (cut1 - start) / item_places * item_places;
         }
         __syncthreads();
     }
     const int from = part_start, to = part_end;
-    if (from >= to) {
+    Walk head = begin;
+    bool any = from < to;
+    if (any) {
+        at_clip(a, head, from, to);
+        if (head.take == 0) any = at_next(c, a, head, from, to);
+    }
+    if (!any) {
         zeros();
         return;
     }
-    Walk head = begin;
-    head.rest = to - from;
-    at_clip(head);
 
     // ---- the warp's loads: unit `unit` of item `load` ----
     // The walks lie in shared memory (one a warp each): only an item's change reads them.
@@ -291,20 +305,21 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
     const uint32_t page_bytes = (uint32_t)c.n_kv * c.page_blocks * G::BLOCK_BYTES;
     auto settle = [&]() {                     // to the next unit that there is, and its item
         Walk x = load;
-        while (x.rest > 0 && unit >= x.first + x.take) {
-            at_next(c, a, x);
+        bool more = true;
+        while (more && unit >= x.first + x.take) {
+            more = at_next(c, a, x, from, to);
             unit = x.first + warp;
         }
         __syncwarp();
         if (lane == 0) load = x;
         __syncwarp();
-        unit_end = x.rest > 0 ? x.first + x.take : 0;
+        unit_end = more ? x.first + x.take : 0;
         load_len = x.len;
         load_base = c.pool + (uint32_t)(x.item / a.chunks * c.page_blocks * G::BLOCK_BYTES);
         load_table = c.tables + (size_t)max(0, x.s) * c.max_pages;
     };
     settle();
-    int entry = -1, in_page = 0;              // lanes 0 and 1: the page of their block of it, and the block there
+    int entry = -1, in_page = 0;              // the first lanes: the page of their block of it, and the block there
     auto look_up = [&]() {
         const int block = unit * AT_UNIT + lane;
         if (unit < unit_end && lane < AT_UNIT && block * KV4_BLOCK < load_len) {
@@ -343,7 +358,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
     // ---- items ----
     int slot = 0, phase = 0;                  // the slot of the next unit to take and its barrier's phase
     bool ok = true;
-    while (w.rest > 0) {
+    for (bool more = true; more;) {
         const int len = w.len, u_end = w.first + w.take;
         const int kvh = w.item / a.chunks, head0 = kvh * a.group + (w.item % a.chunks) * KV4_HEADS;
         const int heads = min(KV4_HEADS, (kvh + 1) * a.group - head0);
@@ -621,34 +636,55 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
         }
         if (!whole) {
             // the item's units lie in parts p0 .. p1; the last part to come joins their results, in order
-            const int begins = w.first > 0 ? from - w.first : to - w.rest;
+            const int begins = w.start + a.item_cost;
             const int p0 = cuts.part_of(begins), p1 = cuts.part_of(begins + w.units - 1);
             int *counter = a.counters + (size_t)w.i * items + w.item;
-            __threadfence();
             __syncthreads();
-            if (threadIdx.x == 0) last = atomicAdd(counter, 1) == p1 - p0;
+            if (threadIdx.x == 0) {           // of all the CTA's writes, and before its reads
+                __threadfence();
+                last = atomicAdd(counter, 1) == p1 - p0;
+                if (last) {
+                    *counter = 0;
+                    __threadfence();
+                }
+            }
             __syncthreads();
             if (last) {
-                __threadfence();
-                if (threadIdx.x == 0) *counter = 0;
                 const float *part = a.partial + ((size_t)p0 * 2 + 1) * G::SLOT;   // then every second one, one less
-                auto at = [&](int k) { return part + (size_t)(k ? 2 * k - 1 : 0) * G::SLOT; };
+                const int parts = p1 - p0 + 1;
+                constexpr int BATCH = 8;      // parts loaded together: few would wait for the memory, one after another
                 for (int d = 4 * threadIdx.x; d < heads * HD; d += 4 * AT_THREADS) {
-                    const int h = d / HD, n = p1 - p0 + 1;
+                    const int h = d / HD;
                     float top = -INFINITY, den = 0.0f;
-#pragma unroll 8
-                    for (int k = 0; k < n; ++k) {
-                        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(at(k)) + h);
-                        if (ml.y != 0.0f) top = fmaxf(top, ml.x);
-                    }
                     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-                    for (int k = 0; k < n; ++k) {
-                        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(at(k)) + h);
-                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(at(k) + 2 * KV4_HEADS + d));
-                        const float f = ml.y != 0.0f ? at_ex2(ml.x - top) : 0.0f;
-                        den = fmaf(ml.y, f, den);
-                        sum.x = fmaf(v.x, f, sum.x), sum.y = fmaf(v.y, f, sum.y), sum.z = fmaf(v.z, f, sum.z), sum.w = fmaf(v.w, f, sum.w);
+                    for (int k0 = 0; k0 < parts; k0 += BATCH) {
+                        float2 ml[BATCH];
+                        float4 v[BATCH];
+#pragma unroll
+                        for (int i = 0; i < BATCH; ++i) {
+                            const int k = min(k0 + i, parts - 1);
+                            const float *p = part + (size_t)(k ? 2 * k - 1 : 0) * G::SLOT;
+                            ml[i] = __ldcg(reinterpret_cast<const float2 *>(p) + h);
+                            v[i] = __ldcg(reinterpret_cast<const float4 *>(p + 2 * KV4_HEADS + d));
+                            if (k0 + i >= parts) ml[i].y = 0.0f;
+                        }
+                        float to = top;
+#pragma unroll
+                        for (int i = 0; i < BATCH; ++i)
+                            if (ml[i].y != 0.0f) to = fmaxf(to, ml[i].x);
+                        const float fix = den != 0.0f ? at_ex2(top - to) : 0.0f;
+                        top = to;
+                        den *= fix;
+                        sum.x *= fix, sum.y *= fix, sum.z *= fix, sum.w *= fix;
+#pragma unroll
+                        for (int i = 0; i < BATCH; ++i) {
+                            const float f = at_ex2(ml[i].x - top);
+                            if (ml[i].y != 0.0f) {
+                                den = fmaf(ml[i].y, f, den);
+                                sum.x = fmaf(v[i].x, f, sum.x), sum.y = fmaf(v[i].y, f, sum.y);
+                                sum.z = fmaf(v[i].z, f, sum.z), sum.w = fmaf(v[i].w, f, sum.w);
+                            }
+                        }
                     }
                     at_store4<T>(out + d, a.wide, sum.x / den, sum.y / den, sum.z / den, sum.w / den);
                 }
@@ -656,7 +692,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
         }
         __syncthreads();                      // the join's memory is free again
         Walk x = w;
-        at_next(c, a, x);
+        more = at_next(c, a, x, from, to);
         __syncwarp();
         if (lane == 0) w = x;
         __syncwarp();
@@ -721,12 +757,14 @@ extern "C" int cuda_kv4_attention(const holo_kv4 *c, int layer, void *out, const
     a.out = out, a.q = q, a.q_row = q_row, a.out_row = out_row, a.seqs = seqs;
     a.n = n, a.n_heads = n_heads, a.group = group, a.chunks = (group + KV4_HEADS - 1) / KV4_HEADS;
     a.scale = scale == 0.0f ? 1.0f / sqrtf((float)c->head_dim) : scale;
-    // units of the list, at most: counted in an int
-    const long long units = ((long long)c->max_pages * c->page_tokens + AT_UNIT_POS - 1) / AT_UNIT_POS;
+    // places of the list, at most: counted in an int
+    const long long units = ((long long)c->max_pages * c->page_tokens + AT_UNIT_POS - 1) / AT_UNIT_POS + AT_ITEM;
     if (units * n * c->n_kv_heads * a.chunks > 0x40000000LL) return refuse(HOLO_E_UNSUPPORTED);
     a.page_magic = view.page_blocks == 1 ? 0 : (uint32_t)((((uint64_t)1 << 32) + view.page_blocks - 1) / view.page_blocks);
     a.wide = (uintptr_t)out % 16 == 0 && out_row * size % 16 == 0;
     a.counters = work.counters, a.partial = work.partial;
+    // where there may be fewer items than CTAs, each CTA has one at most and its cost is the same for all
+    a.item_cost = (long long)n * c->n_kv_heads * a.chunks >= holo_dev()->sms * 2 ? AT_ITEM : 0;
     const int sms = holo_dev()->sms;
     bool done;
     switch (type) {
