@@ -11,6 +11,7 @@
 #include "kv4.cuh"
 
 #include <mutex>
+#include <type_traits>
 
 namespace {
 
@@ -107,30 +108,34 @@ __device__ __forceinline__ void load8(const T *p, bool wide, float (&x)[8]) {
 }
 
 template <typename T>
-__device__ __forceinline__ void store8(T *p, bool wide, const float (&x)[8]) {
+__device__ __forceinline__ void store8(T *p, bool wide, const T (&x)[8]) {
     if (wide) {
         uint4 w[sizeof(T) / 2];
         T *h = reinterpret_cast<T *>(w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) h[i] = kv4_from_float<T>(x[i]);
+        for (int i = 0; i < 8; ++i) h[i] = x[i];
 #pragma unroll
         for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4 *>(p)[i] = w[i];
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = kv4_from_float<T>(x[i]);
+        for (int i = 0; i < 8; ++i) p[i] = x[i];
     }
 }
 
-// eight codes of a lane and the scale of its group, over the four lanes that
+// Eight codes of a lane and the scale of its group, over the four lanes that
 // hold it: d = fp16(m / -8), code = rint(x / d) + 8 in 0..15 (fp32 arithmetic,
-// each operation rounded once), NaN as the scale where a value is not finite
+// each operation rounded once), NaN as the scale where a value is not finite.
+// The quotient is the rounded one without a division: from the rounded
+// reciprocal r, t = x r and t + (x - t d) r, each a fused operation, which rounds
+// x / d correctly (Markstein, IBM J. Res. Dev. 34, 1990); where the remainder could
+// underflow the quotient is far below 1/2.  The rounding to a whole number is
+// the addition of 1.5 * 2^23 + 8, whose low bits are then the code.
 __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], __half &d) {
-    float m = x[0];
-    bool finite = isfinite(x[0]);
+    float m = x[0], zero = x[0] * 0.0f;
 #pragma unroll
     for (int i = 1; i < 8; ++i) {
         if (fabsf(x[i]) > fabsf(m)) m = x[i];
-        finite = finite && isfinite(x[i]);
+        zero = fmaf(x[i], 0.0f, zero);        // NaN where a value is not finite
     }
     // of two equal magnitudes the lower lane's stays
 #pragma unroll
@@ -139,23 +144,44 @@ __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], __half &d) {
         const bool lower = (threadIdx.x & o) != 0;   // the other lane is the lower one
         if (fabsf(other) > fabsf(m) || (lower && fabsf(other) == fabsf(m))) m = other;
     }
-    const unsigned all = __ballot_sync(0xffffffffu, finite);
+    const unsigned all = __ballot_sync(0xffffffffu, zero == 0.0f);
     const unsigned mine = 0xfu << (threadIdx.x & 28);
-    d = (all & mine) == mine ? __float2half_rn(m * -0.125f) : __ushort_as_half(0x7e00);
+    const bool finite = (all & mine) == mine;
+    d = finite ? __float2half_rn(m * -0.125f) : __ushort_as_half(0x7e00);
     const float w = __half2float(d);
+    const bool usable = w != 0.0f && fabsf(w) <= 65504.0f;   // a scale to divide by: else code 8
+    const float r = usable ? __frcp_rn(w) : 0.0f;
     uint32_t codes = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int q = w == 0.0f ? 0 : __float2int_rn(__fdiv_rn(x[i], w));
-        codes |= (uint32_t)max(0, min(15, q + 8)) << (4 * i);
+    for (int i = 7; i >= 0; --i) {
+        const float t = __fmul_rn(x[i], r);
+        const float q = fminf(fmaxf(fmaf(fmaf(-t, w, x[i]), r, t), -8.0f), 7.0f);
+        codes = codes << 4 | (__float_as_uint(__fadd_rn(q, 12582920.0f)) & 15u);
     }
-    return codes;
+    return usable ? codes : 0x88888888u;
 }
 
-__device__ __forceinline__ void dequantise8(uint32_t codes, __half d, float (&x)[8]) {
+// pair p (0..3) of eight codes, p and p + 4, as fp16 code - 8: 1024 + code, less 1032
+__device__ __forceinline__ __half2 code_pair(uint32_t codes, int p) {
+    const uint32_t w = (codes >> (4 * p) & 0x000f000fu) | 0x64006400u;
+    return __hsub2(*reinterpret_cast<const __half2 *>(&w), __half2half2(__ushort_as_half(0x6408)));
+}
+
+// the values of eight codes, rounded once to the rows' type
+template <typename T>
+__device__ __forceinline__ void dequantise8(uint32_t codes, __half d, T (&x)[8]) {
     const float w = __half2float(d);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = w * (float)((int)((codes >> (4 * i)) & 15u) - 8);
+    for (int p = 0; p < 4; ++p) {
+        const __half2 c = code_pair(codes, p);
+        if constexpr (std::is_same<T, __half>::value) {   // the product has 15 bits: one rounding here too
+            const __half2 v = __hmul2(c, __half2half2(d));
+            x[p] = __low2half(v), x[p + 4] = __high2half(v);
+        } else {
+            const float2 v = __half22float2(c);
+            x[p] = kv4_from_float<T>(v.x * w), x[p + 4] = kv4_from_float<T>(v.y * w);
+        }
+    }
 }
 
 // Thread = (row, head, group b, eight values t), of the CTA's rows.  `lanes`
@@ -187,8 +213,8 @@ rows_kernel(const __grid_constant__ Kv4View c, T *k, T *v, long long k_row, long
         uint16_t *half1 = reinterpret_cast<uint16_t *>(blk + kv4_off_v(HD) + kv4_v_half(HD, p.slot, 2 * t + 1, b));
         __half *scale_k = reinterpret_cast<__half *>(blk + kv4_off_dk(HD) + 2 * (p.slot * NB + b));
         __half *scale_v = reinterpret_cast<__half *>(blk + kv4_off_dv(HD) + 2 * (p.slot * NB + b));
-        float xk[8] = {}, xv[8] = {};
         if (APPEND) {
+            float xk[8] = {}, xv[8] = {};
             if (ok) {
                 load8(k + at_k, wide, xk);
                 load8(v + at_v, wide, xv);
@@ -202,10 +228,12 @@ rows_kernel(const __grid_constant__ Kv4View c, T *k, T *v, long long k_row, long
                 if (t == 0) *scale_k = dk, *scale_v = dv;
             }
         } else if (in) {
-            if (ok) {
-                dequantise8(*word, *scale_k, xk);
-                dequantise8(*half0 | (uint32_t)*half1 << 16, *scale_v, xv);
-            }
+            // (a row without a place: code 8 throughout, zeros)
+            const uint32_t ck = ok ? *word : 0x88888888u, cv = ok ? *half0 | (uint32_t)*half1 << 16 : 0x88888888u;
+            const __half dk = ok ? *scale_k : __ushort_as_half(0), dv = ok ? *scale_v : __ushort_as_half(0);
+            T xk[8], xv[8];
+            dequantise8(ck, dk, xk);
+            dequantise8(cv, dv, xv);
             store8(k + at_k, wide, xk);
             store8(v + at_v, wide, xv);
         }
