@@ -125,40 +125,65 @@ __device__ __forceinline__ void store8(T *p, bool wide, const T (&x)[8]) {
 // Eight codes of a lane and the scale of its group, over the four lanes that
 // hold it: d = fp16(m / -8), code = rint(x / d) + 8 in 0..15 (fp32 arithmetic,
 // each operation rounded once), NaN as the scale where a value is not finite.
-// The quotient is the rounded one without a division: from the rounded
-// reciprocal r, t = x r and t + (x - t d) r, each a fused operation, which rounds
-// x / d correctly (Markstein, IBM J. Res. Dev. 34, 1990); where the remainder could
-// underflow the quotient is far below 1/2.  The rounding to a whole number is
-// the addition of 1.5 * 2^23 + 8, whose low bits are then the code.
+// Bound by instructions (an append of many rows: 0.78 of the issue slots at 2.9
+// TB/s), so the work is put on the FMA pipe, which takes one a cycle:
+//   m         from the group's largest and smallest value; where they are equal
+//             in size, or zero, from a second look for the first of them
+//   x / d     the rounded quotient without a division: from the rounded
+//             reciprocal r, t = x r and t + (x - t d) r, fused operations, which
+//             rounds x / d correctly (Markstein, IBM J. Res. Dev. 34, 1990); where
+//             the remainder could underflow the quotient is far below 1/2
+//   codes     rounded to whole numbers by adding and taking away 1.5 * 2^23, and
+//             put together four at a time as the digits, base 16, of an exact float
 __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], __half &d) {
-    float m = x[0], zero = x[0] * 0.0f;
+    float high = x[0], low = x[0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) {
-        if (fabsf(x[i]) > fabsf(m)) m = x[i];
-        zero = fmaf(x[i], 0.0f, zero);        // NaN where a value is not finite
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(high) : "f"(x[i]));
+        low = fminf(low, x[i]);
     }
-    // of two equal magnitudes the lower lane's stays
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
-        const float other = __shfl_xor_sync(0xffffffffu, m, o, 4);
-        const bool lower = (threadIdx.x & o) != 0;   // the other lane is the lower one
-        if (fabsf(other) > fabsf(m) || (lower && fabsf(other) == fabsf(m))) m = other;
+        const float h = __shfl_xor_sync(0xffffffffu, high, o), l = __shfl_xor_sync(0xffffffffu, low, o);
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(high) : "f"(h));
+        low = fminf(low, l);
     }
-    const unsigned all = __ballot_sync(0xffffffffu, zero == 0.0f);
-    const unsigned mine = 0xfu << (threadIdx.x & 28);
-    const bool finite = (all & mine) == mine;
+    float m = high > -low ? high : low;
+    const bool tie = high == -low;
+    if (__any_sync(0xffffffffu, tie)) {
+        // the first value of that size: its place in the group, and the value
+        int place = 32;
+        float v = m;
+#pragma unroll
+        for (int i = 7; i >= 0; --i)
+            if (fabsf(x[i]) == high) place = (threadIdx.x & 3) * 8 + i, v = x[i];
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+            const int p = __shfl_xor_sync(0xffffffffu, place, o);
+            const float u = __shfl_xor_sync(0xffffffffu, v, o);
+            if (p < place) place = p, v = u;
+        }
+        if (tie) m = v;
+    }
+    const bool finite = high < INFINITY && low > -INFINITY;   // high is NaN where a value is
     d = finite ? __float2half_rn(m * -0.125f) : __ushort_as_half(0x7e00);
     const float w = __half2float(d);
     const bool usable = w != 0.0f && fabsf(w) <= 65504.0f;   // a scale to divide by: else code 8
     const float r = usable ? __frcp_rn(w) : 0.0f;
-    uint32_t codes = 0;
+    const float magic = 12582912.0f;
+    uint32_t codes[2];
 #pragma unroll
-    for (int i = 7; i >= 0; --i) {
-        const float t = __fmul_rn(x[i], r);
-        const float q = fminf(fmaxf(fmaf(fmaf(-t, w, x[i]), r, t), -8.0f), 7.0f);
-        codes = codes << 4 | (__float_as_uint(__fadd_rn(q, 12582920.0f)) & 15u);
+    for (int half = 0; half < 2; ++half) {
+        float digits = 0.0f;
+#pragma unroll
+        for (int i = 4 * half + 3; i >= 4 * half; --i) {
+            const float t = __fmul_rn(x[i], r);
+            const float q = fminf(fmaxf(fmaf(fmaf(-t, w, x[i]), r, t), -8.0f), 7.0f);
+            digits = fmaf(digits, 16.0f, __fadd_rn(__fadd_rn(q, magic), 8.0f - magic));
+        }
+        codes[half] = __float_as_uint(__fadd_rn(digits, 8388608.0f));   // 2^23: the digits are the low bits
     }
-    return usable ? codes : 0x88888888u;
+    return usable ? __byte_perm(codes[0], codes[1], 0x5410) : 0x88888888u;
 }
 
 // pair p (0..3) of eight codes, p and p + 4, as fp16 code - 8: 1024 + code, less 1032
