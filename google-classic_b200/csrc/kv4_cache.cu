@@ -209,13 +209,13 @@ __device__ __forceinline__ void dequantise8(uint32_t codes, __half d, T (&x)[8])
     }
 }
 
-// Thread = (row, head, group b, eight values t), of the CTA's rows.  `lanes`
-// = n_kv * HD / 8 threads a row (a multiple of eight), `magic` = ceil(2^32 / lanes).
+// Thread = (row, head, group b, eight values t), of the CTA's rows.  A row is
+// `lanes` = n_kv * HD / 8 threads; 1 << shift of them, the largest power of two in
+// it, stand side by side, so that a thread keeps its place in the row from row to row.
 template <bool APPEND, typename T, int HD>
 __global__ void __launch_bounds__(ROW_THREADS)
-rows_kernel(const __grid_constant__ Kv4View c, T *k, T *v, long long k_row, long long v_row,
-            int rows, const int *cu, const int *start, const int *seqs, int n,
-            bool wide, int rows_cta, int lanes, uint32_t magic) {
+rows_kernel(const __grid_constant__ Kv4View c, T *k, T *v, long long k_row, long long v_row, int rows, const int *cu,
+            const int *start, const int *seqs, int n, bool wide, int rows_cta, int lanes, int shift) {
     constexpr int NB = HD / KV4_GROUP, EIGHTS = HD / 8;
     __shared__ Place places[ROW_MAX];
     early_wait();
@@ -223,47 +223,52 @@ rows_kernel(const __grid_constant__ Kv4View c, T *k, T *v, long long k_row, long
     const int row0 = blockIdx.x * rows_cta, mine = min(rows_cta, rows - row0);
     if ((int)threadIdx.x < mine) places[threadIdx.x] = row_place(c, HD, cu, start, seqs, n, row0 + threadIdx.x);
     __syncthreads();
-    const int total = mine * lanes;
-    for (int e0 = blockIdx.y * ROW_THREADS; e0 < total; e0 += gridDim.y * ROW_THREADS) {
-        const int e = e0 + threadIdx.x;
-        const int r = min((int)__umulhi((uint32_t)e, magic), mine - 1), in_row = e - r * lanes;
-        const int kvh = in_row / EIGHTS, eight = in_row % EIGHTS, b = eight >> 2, t = eight & 3;
-        const Place p = places[r];
-        const bool in = e < total, ok = in && p.at >= 0;
-        const size_t at_k = (size_t)(row0 + r) * k_row + (size_t)kvh * HD + 8 * eight;
-        const size_t at_v = (size_t)(row0 + r) * v_row + (size_t)kvh * HD + 8 * eight;
-        uint8_t *blk = c.pool + p.at + (size_t)kvh * c.page_blocks * kv4_block_bytes(HD);
-        uint32_t *word = reinterpret_cast<uint32_t *>(blk + kv4_k_half(HD, p.slot, 2 * t, b));
-        uint16_t *half0 = reinterpret_cast<uint16_t *>(blk + kv4_off_v(HD) + kv4_v_half(HD, p.slot, 2 * t, b));
-        uint16_t *half1 = reinterpret_cast<uint16_t *>(blk + kv4_off_v(HD) + kv4_v_half(HD, p.slot, 2 * t + 1, b));
-        __half *scale_k = reinterpret_cast<__half *>(blk + kv4_off_dk(HD) + 2 * (p.slot * NB + b));
-        __half *scale_v = reinterpret_cast<__half *>(blk + kv4_off_dv(HD) + 2 * (p.slot * NB + b));
-        if (APPEND) {
-            float xk[8] = {}, xv[8] = {};
-            if (ok) {
-                load8(k + at_k, wide, xk);
-                load8(v + at_v, wide, xv);
+    const int across = 1 << shift, down = ROW_THREADS >> shift, r0 = threadIdx.x >> shift;
+    for (int col0 = blockIdx.y << shift; col0 < lanes; col0 += gridDim.y << shift) {
+        const int col = col0 + (threadIdx.x & (across - 1));
+        const int kvh = col / EIGHTS, eight = col % EIGHTS, b = eight >> 2, t = eight & 3;
+        const long long off = (long long)kvh * c.page_blocks * kv4_block_bytes(HD);
+        T *kp = k + (size_t)(row0 + r0) * k_row + 8 * col, *vp = v + (size_t)(row0 + r0) * v_row + 8 * col;
+        // (all threads of the CTA go round alike: the shuffles)
+        for (int i = 0; i < mine; i += down, kp += down * k_row, vp += down * v_row) {
+            const bool in = i + r0 < mine;
+            const Place p = places[in ? i + r0 : 0];
+            const bool ok = in && p.at >= 0;
+            uint8_t *blk = c.pool + (p.at + off);
+            const int pair = p.slot >> 1, odd = p.slot & 1;
+            uint32_t *word = reinterpret_cast<uint32_t *>(blk + kv4_k_half(HD, 0, 2 * t, b) + p.slot * (HD / 2));
+            uint8_t *value = blk + kv4_off_v(HD) + kv4_v_half(HD, 0, 2 * t, b) + pair * (8 * NB) + odd * (2 * NB);
+            uint16_t *half0 = reinterpret_cast<uint16_t *>(value), *half1 = reinterpret_cast<uint16_t *>(value + 4 * NB);
+            __half *scale_k = reinterpret_cast<__half *>(blk + kv4_off_dk(HD) + 2 * b + p.slot * (2 * NB));
+            __half *scale_v = scale_k + HD / 2;
+            if (APPEND) {
+                float xk[8] = {}, xv[8] = {};
+                if (ok) {
+                    load8(kp, wide, xk);
+                    load8(vp, wide, xv);
+                }
+                __half dk, dv;
+                const uint32_t ck = quantise8(xk, dk), cv = quantise8(xv, dv);
+                if (ok) {
+                    *word = ck;
+                    *half0 = (uint16_t)cv;
+                    *half1 = (uint16_t)(cv >> 16);
+                    if (t == 0) *scale_k = dk, *scale_v = dv;
+                }
+            } else if (in) {
+                // (a row without a place: code 8 throughout, zeros)
+                const uint32_t ck = ok ? *word : 0x88888888u, cv = ok ? *half0 | (uint32_t)*half1 << 16 : 0x88888888u;
+                const __half dk = ok ? *scale_k : __ushort_as_half(0), dv = ok ? *scale_v : __ushort_as_half(0);
+                T xk[8], xv[8];
+                dequantise8(ck, dk, xk);
+                dequantise8(cv, dv, xv);
+                store8(kp, wide, xk);
+                store8(vp, wide, xv);
             }
-            __half dk, dv;
-            const uint32_t ck = quantise8(xk, dk), cv = quantise8(xv, dv);
-            if (ok) {
-                *word = ck;
-                *half0 = (uint16_t)cv;
-                *half1 = (uint16_t)(cv >> 16);
-                if (t == 0) *scale_k = dk, *scale_v = dv;
-            }
-        } else if (in) {
-            // (a row without a place: code 8 throughout, zeros)
-            const uint32_t ck = ok ? *word : 0x88888888u, cv = ok ? *half0 | (uint32_t)*half1 << 16 : 0x88888888u;
-            const __half dk = ok ? *scale_k : __ushort_as_half(0), dv = ok ? *scale_v : __ushort_as_half(0);
-            T xk[8], xv[8];
-            dequantise8(ck, dk, xk);
-            dequantise8(cv, dv, xv);
-            store8(k + at_k, wide, xk);
-            store8(v + at_v, wide, xv);
         }
     }
 }
+static_assert(kv4_v_half(128, 0, 1, 0) == 4 * 4 && kv4_v_half(64, 3, 0, 0) == 8 * 2 + 2 * 2, "a value's place in its block");
 
 int type_bytes(int type) { return type == HOLO_DT_F32 ? 4 : 2; }
 
@@ -278,15 +283,16 @@ struct Rows {
 
 template <bool APPEND, typename T, int HD>
 void launch_rows(const Rows &r, const Kv4View &view, bool wide, int sms, cudaStream_t st) {
-    // 16 rows a CTA where that still makes four CTAs an SM, else fewer, and the heads of
-    // one row over several CTAs where one row is all there is for each SM
+    // 16 rows a CTA where that still makes four CTAs an SM, else fewer, and the columns of
+    // a row over several CTAs where one row is all there is for each SM
     const int lanes = view.n_kv * (HD / 8);
     const int rows_cta = max(1, min(ROW_MAX, r.rows / (4 * sms)));
+    int shift = 3;                            // lanes is a multiple of eight
+    while (shift < 8 && lanes % (2 << shift) == 0) ++shift;
     const unsigned x = (unsigned)((r.rows + rows_cta - 1) / rows_cta);
-    const int steps = (rows_cta * lanes + ROW_THREADS - 1) / ROW_THREADS;
-    const unsigned y = (unsigned)max(1, min(steps, (int)(4 * sms / x)));
-    const uint32_t magic = (uint32_t)((((uint64_t)1 << 32) + lanes - 1) / lanes);
-    holo_launch_early(rows_kernel<APPEND, T, HD>, dim3(x, y), ROW_THREADS, 0, st, view, (T *)r.k, (T *)r.v, r.k_row, r.v_row, r.rows, r.cu, r.start, r.seqs, r.n, wide, rows_cta, lanes, magic);
+    const unsigned y = (unsigned)max(1, min(lanes >> shift, (int)(4 * sms / x)));
+    holo_launch_early(rows_kernel<APPEND, T, HD>, dim3(x, y), ROW_THREADS, 0, st, view, (T *)r.k, (T *)r.v, r.k_row, r.v_row,
+                      r.rows, r.cu, r.start, r.seqs, r.n, wide, rows_cta, lanes, shift);
 }
 
 template <bool APPEND, typename T>
