@@ -1,10 +1,10 @@
 // kv4_pages.cu -- pages of the paged 4-bit KV cache: allocation, forks,
 // release, compaction and copies, all decided on the device.
 //
-// Each call that needs free pages, or a new order of the pages, is two launches: one CTA
-// makes the plan (prefix sums over refs, 4096 pages a step: the lowest free
-// pages, or the pairs to move), then a grid over all SMs copies the pages in
-// every layer and rewrites tables and refs.  Free pages go to the sequences in
+// A fork or a compaction is two launches: one CTA makes the plan (prefix sums
+// over refs, 4096 pages a step: the lowest free pages, or the pairs to move),
+// then a grid over all SMs copies the pages in every layer and rewrites tables
+// and refs; where there is little to copy the one CTA does that too.  Free pages go to the sequences in
 // the order of the list, so the result does not depend on timing.  The copies
 // read and write each moved byte once.
 #include "kv4.cuh"
@@ -140,12 +140,28 @@ extend_kernel(const __grid_constant__ Kv4View c, const int *seqs, const int *cou
 }
 
 // ---- copies ---------------------------------------------------------------------
-// All layers of `pairs` pages: the unit of a CTA is one page of one layer.
-__device__ __forceinline__ void copy_page(uint8_t *pool, size_t page_bytes, int src, int dst, int t, int threads) {
+// The threads that share a unit of work, one of `teams`: a CTA of a grid, or a
+// warp of the one CTA that does everything.
+struct Team {
+    int team, teams, thread, threads;
+};
+__device__ __forceinline__ Team cta_team() { return {(int)blockIdx.x, (int)gridDim.x, (int)threadIdx.x, (int)blockDim.x}; }
+__device__ __forceinline__ Team warp_team() { return {(int)threadIdx.x / 32, PLAN_THREADS / 32, (int)threadIdx.x % 32, 32}; }
+
+// One page of one layer; four loads under way a thread.
+__device__ __forceinline__ void copy_page(const Team &t, uint8_t *pool, size_t page_bytes, int src, int dst) {
     const uint4 *s = reinterpret_cast<const uint4 *>(pool + (size_t)src * page_bytes);
     uint4 *d = reinterpret_cast<uint4 *>(pool + (size_t)dst * page_bytes);
-    const int words = (int)(page_bytes / 16);
-    for (int i = t; i < words; i += threads) d[i] = s[i];
+    const int words = (int)(page_bytes / 16), step = t.threads;
+    int i = t.thread;
+    for (; i + 3 * step < words; i += 4 * step) {
+        uint4 v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = __ldcs(s + i + k * step);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) __stcs(d + i + k * step, v[k]);
+    }
+    for (; i < words; i += step) d[i] = s[i];
 }
 
 __global__ void __launch_bounds__(COPY_THREADS)
@@ -161,15 +177,51 @@ copy_kernel(const __grid_constant__ Kv4View c, size_t page_bytes, size_t layer_b
             if (threadIdx.x == 0) kv4_report(c.status, HOLO_E_ARG);
             continue;
         }
-        copy_page(c.pool + layer * layer_bytes, page_bytes, s, d, threadIdx.x, COPY_THREADS);
+        copy_page(cta_team(), c.pool + layer * layer_bytes, page_bytes, s, d);
     }
 }
 
 // ---- fork ------------------------------------------------------------------------
-// page[i]: the new page of child i; -1: it needs none, -2: it is left out
+// the children's rows, the pages' counts and the copies
+__device__ __forceinline__ void fork_apply(const Kv4View &c, size_t page_bytes, size_t layer_bytes, int layers,
+                                           const int *parents, const int *children, int n, const int *page, const Team &t) {
+    const long long total = (long long)n * layers;
+    for (long long u = t.team; u < total; u += t.teams) {
+        const int i = (int)(u / layers), layer = (int)(u % layers);
+        const int fresh = page[i];
+        if (fresh == -2) continue;
+        const int p = parents[i], k = children[i], len = c.lens[p], full = len / c.page_tokens;
+        const int *from = c.tables + (size_t)p * c.max_pages;
+        if (layer == 0) {   // the child's row and the pages' counts, once
+            int *to = c.tables + (size_t)k * c.max_pages;
+            for (int j = t.thread; j < c.max_pages; j += t.threads) {
+                int e = -1;
+                if (j < full) {
+                    e = from[j];
+                    if (e >= 0 && e < c.n_pages) atomicAdd(c.refs + e, 1);
+                    else kv4_report(c.status, HOLO_E_ARG);
+                } else if (j == full) {
+                    e = fresh;   // -1: the parent ends with a full page
+                    if (e >= 0) c.refs[e] = 1;
+                }
+                to[j] = e;
+            }
+            if (t.thread == 0) c.lens[k] = len;
+        }
+        if (fresh >= 0) {
+            const int s = from[full];
+            if (s >= 0 && s < c.n_pages) copy_page(t, c.pool + layer * layer_bytes, page_bytes, s, fresh);
+            else if (t.thread == 0) kv4_report(c.status, HOLO_E_ARG);
+        }
+    }
+}
+
+// page[i]: the new page of child i; -1: it needs none, -2: it is left out.
+// ALL: the rest of the work too, where it is little
+template <bool ALL>
 __global__ void __launch_bounds__(PLAN_THREADS, 1)
-fork_plan_kernel(const __grid_constant__ Kv4View c, const int *parents, const int *children,
-                 int n, int *page, int *list) {
+fork_plan_kernel(const __grid_constant__ Kv4View c, size_t page_bytes, size_t layer_bytes, int layers, const int *parents,
+                 const int *children, int n, int *page, int *list) {
     early_wait();
     early_next();
     __shared__ int sh[32];
@@ -209,42 +261,18 @@ fork_plan_kernel(const __grid_constant__ Kv4View c, const int *parents, const in
             }
         }
     }
+    if (ALL) {
+        __syncthreads();
+        fork_apply(c, page_bytes, layer_bytes, layers, parents, children, n, page, warp_team());
+    }
 }
 
 __global__ void __launch_bounds__(COPY_THREADS)
-fork_kernel(const __grid_constant__ Kv4View c, size_t page_bytes, size_t layer_bytes, int layers,
-            const int *parents, const int *children, int n, const int *page) {
+fork_kernel(const __grid_constant__ Kv4View c, size_t page_bytes, size_t layer_bytes, int layers, const int *parents,
+            const int *children, int n, const int *page) {
     early_wait();
     early_next();
-    const long long total = (long long)n * layers;
-    for (long long u = blockIdx.x; u < total; u += gridDim.x) {
-        const int i = (int)(u / layers), layer = (int)(u % layers);
-        const int fresh = page[i];
-        if (fresh == -2) continue;
-        const int p = parents[i], k = children[i], len = c.lens[p], full = len / c.page_tokens;
-        const int *from = c.tables + (size_t)p * c.max_pages;
-        if (layer == 0) {   // the child's row and the pages' counts, once
-            int *to = c.tables + (size_t)k * c.max_pages;
-            for (int j = threadIdx.x; j < c.max_pages; j += COPY_THREADS) {
-                int e = -1;
-                if (j < full) {
-                    e = from[j];
-                    if (e >= 0 && e < c.n_pages) atomicAdd(c.refs + e, 1);
-                    else kv4_report(c.status, HOLO_E_ARG);
-                } else if (j == full) {
-                    e = fresh;   // -1: the parent ends with a full page
-                    if (e >= 0) c.refs[e] = 1;
-                }
-                to[j] = e;
-            }
-            if (threadIdx.x == 0) c.lens[k] = len;
-        }
-        if (fresh >= 0) {
-            const int s = from[full];
-            if (s >= 0 && s < c.n_pages) copy_page(c.pool + layer * layer_bytes, page_bytes, s, fresh, threadIdx.x, COPY_THREADS);
-            else if (threadIdx.x == 0) kv4_report(c.status, HOLO_E_ARG);
-        }
-    }
+    fork_apply(c, page_bytes, layer_bytes, layers, parents, children, n, page, cta_team());
 }
 
 // ---- release ----------------------------------------------------------------------
@@ -276,17 +304,38 @@ release_kernel(const __grid_constant__ Kv4View c, const int *seqs, int n) {
 }
 
 // ---- compact ------------------------------------------------------------------------
-// plan[0] moves: src, dst (ascending both); to[page]: its number afterwards
+// the counts, the tables and the copies
+__device__ __forceinline__ void compact_apply(const Kv4View &c, size_t page_bytes, size_t layer_bytes, int layers, int moves,
+                                              const int *src, const int *dst, const int *to, const Team &t) {
+    if (moves == 0) return;
+    const long long me = (long long)t.team * t.threads + t.thread, all = (long long)t.teams * t.threads;
+    for (long long i = me; i < moves; i += all) {   // sources and targets are disjoint
+        c.refs[dst[i]] = c.refs[src[i]];
+        c.refs[src[i]] = 0;
+    }
+    for (long long i = me; i < (long long)c.max_seqs * c.max_pages; i += all) {
+        const int e = c.tables[i];
+        if (e >= 0 && e < c.n_pages && to[e] != e) c.tables[i] = to[e];
+    }
+    const long long total = (long long)moves * layers;
+    for (long long u = t.team; u < total; u += t.teams)
+        copy_page(t, c.pool + (u % layers) * layer_bytes, page_bytes, src[u / layers], dst[u / layers]);
+}
+
+// plan[0] moves: src, dst (ascending both); to[page]: its number afterwards.
+// ALL: the rest of the work too, where it is little
+template <bool ALL>
 __global__ void __launch_bounds__(PLAN_THREADS, 1)
-compact_plan_kernel(const __grid_constant__ Kv4View c, int *plan, int *src,
+compact_plan_kernel(const __grid_constant__ Kv4View c, size_t page_bytes, size_t layer_bytes, int layers, int *plan, int *src,
                     int *dst, int *to) {
     early_wait();
     early_next();
     __shared__ int sh[32];
     int live = 0;
+    int4 r;                                   // (a pool of one step is read once)
     for (int p0 = 0; p0 < c.n_pages; p0 += PLAN_STEP) {
         const int p = p0 + 4 * threadIdx.x;
-        const int4 r = four_refs(c, p);
+        r = four_refs(c, p);
         const int held[4] = {r.x != 0 && p < c.n_pages, r.y != 0 && p + 1 < c.n_pages, r.z != 0 && p + 2 < c.n_pages,
                              r.w != 0 && p + 3 < c.n_pages};
         int total;
@@ -296,7 +345,7 @@ compact_plan_kernel(const __grid_constant__ Kv4View c, int *plan, int *src,
     int movers = 0, holes = 0;
     for (int p0 = 0; p0 < c.n_pages; p0 += PLAN_STEP) {
         const int p = p0 + 4 * threadIdx.x;
-        const int4 r = four_refs(c, p);
+        if (c.n_pages > PLAN_STEP) r = four_refs(c, p);
         const int ref[4] = {r.x, r.y, r.z, r.w};
         // movers in the low half of a sum, holes in the high half
         int mine = 0;
@@ -322,29 +371,18 @@ compact_plan_kernel(const __grid_constant__ Kv4View c, int *plan, int *src,
     __syncthreads();
     for (int i = threadIdx.x; i < movers; i += PLAN_THREADS) to[src[i]] = dst[i];
     if (threadIdx.x == 0) plan[0] = movers;   // as many holes as movers
+    if (ALL) {
+        __syncthreads();
+        compact_apply(c, page_bytes, layer_bytes, layers, movers, src, dst, to, warp_team());
+    }
 }
 
 __global__ void __launch_bounds__(COPY_THREADS)
-compact_kernel(const __grid_constant__ Kv4View c, size_t page_bytes, size_t layer_bytes, int layers,
-               const int *plan, const int *src, const int *dst,
-               const int *to) {
+compact_kernel(const __grid_constant__ Kv4View c, size_t page_bytes, size_t layer_bytes, int layers, const int *plan,
+               const int *src, const int *dst, const int *to) {
     early_wait();
     early_next();
-    const int moves = plan[0];
-    if (moves == 0) return;
-    const long long me = (long long)blockIdx.x * COPY_THREADS + threadIdx.x, all = (long long)gridDim.x * COPY_THREADS;
-    for (long long i = me; i < moves; i += all) {   // sources and targets are disjoint
-        c.refs[dst[i]] = c.refs[src[i]];
-        c.refs[src[i]] = 0;
-    }
-    for (long long i = me; i < (long long)c.max_seqs * c.max_pages; i += all) {
-        const int e = c.tables[i];
-        if (e >= 0 && e < c.n_pages && to[e] != e) c.tables[i] = to[e];
-    }
-    const long long total = (long long)moves * layers;
-    for (long long u = blockIdx.x; u < total; u += gridDim.x)
-        copy_page(c.pool + (u % layers) * layer_bytes, page_bytes, src[u / layers], dst[u / layers], threadIdx.x,
-                  COPY_THREADS);
+    compact_apply(c, page_bytes, layer_bytes, layers, plan[0], src, dst, to, cta_team());
 }
 
 struct Pages {
@@ -372,6 +410,9 @@ int refuse(const char *what) {
     return HOLO_E_ARG;
 }
 
+// so little to copy (page-layers) that one CTA does it sooner than a second launch would begin
+bool little(const Pages &p, long long units) { return units * (long long)p.page_bytes <= (512 << 10); }
+
 unsigned copy_grid(const Pages &p, long long units) {
     const long long most = (long long)p.sms * 8;
     return (unsigned)(units < 1 ? 1 : units < most ? units : most);
@@ -396,8 +437,15 @@ int cuda_kv4_fork(const holo_kv4 *c, const int *parents, const int *children, in
     if (n < 0 || n > c->max_seqs || (n > 0 && (!parents || !children))) return refuse("cuda_kv4_fork");
     if (n == 0) return HOLO_OK;
     int *page = p.work.plan + PLAN_LISTS, *list = page + c->max_seqs;
-    holo_launch_early(fork_plan_kernel, 1, PLAN_THREADS, 0, p.st, p.view, parents, children, n, page, list);
-    holo_launch_early(fork_kernel, copy_grid(p, (long long)n * c->n_layers), COPY_THREADS, 0, p.st, p.view, p.page_bytes, p.layer_bytes, c->n_layers, parents, children, n, page);
+    if (little(p, (long long)n * c->n_layers)) {
+        holo_launch_early(fork_plan_kernel<true>, 1, PLAN_THREADS, 0, p.st, p.view, p.page_bytes, p.layer_bytes, c->n_layers,
+                          parents, children, n, page, list);
+    } else {
+        holo_launch_early(fork_plan_kernel<false>, 1, PLAN_THREADS, 0, p.st, p.view, p.page_bytes, p.layer_bytes,
+                          c->n_layers, parents, children, n, page, list);
+        holo_launch_early(fork_kernel, copy_grid(p, (long long)n * c->n_layers), COPY_THREADS, 0, p.st, p.view, p.page_bytes,
+                          p.layer_bytes, c->n_layers, parents, children, n, page);
+    }
     return kv4_end("cuda_kv4_fork");
 }
 
@@ -414,8 +462,16 @@ int cuda_kv4_compact(const holo_kv4 *c) {
     Pages p;
     if (!begin(c, "cuda_kv4_compact", p, true)) return cuda_last_status();
     int *src = p.work.plan + PLAN_LISTS, *dst = src + c->n_pages, *to = dst + c->n_pages;
-    holo_launch_early(compact_plan_kernel, 1, PLAN_THREADS, 0, p.st, p.view, p.work.plan, src, dst, to);
-    holo_launch_early(compact_kernel, copy_grid(p, (long long)c->n_pages * c->n_layers), COPY_THREADS, 0, p.st, p.view, p.page_bytes, p.layer_bytes, c->n_layers, p.work.plan, src, dst, to);
+    // at most half of the pages move
+    if (little(p, (long long)(c->n_pages / 2) * c->n_layers) && (long long)c->max_seqs * c->max_pages <= 64 * PLAN_THREADS) {
+        holo_launch_early(compact_plan_kernel<true>, 1, PLAN_THREADS, 0, p.st, p.view, p.page_bytes, p.layer_bytes,
+                          c->n_layers, p.work.plan, src, dst, to);
+    } else {
+        holo_launch_early(compact_plan_kernel<false>, 1, PLAN_THREADS, 0, p.st, p.view, p.page_bytes, p.layer_bytes,
+                          c->n_layers, p.work.plan, src, dst, to);
+        holo_launch_early(compact_kernel, copy_grid(p, (long long)c->n_pages * c->n_layers), COPY_THREADS, 0, p.st, p.view,
+                          p.page_bytes, p.layer_bytes, c->n_layers, p.work.plan, src, dst, to);
+    }
     return kv4_end("cuda_kv4_compact");
 }
 
