@@ -14,10 +14,16 @@
 //            times the position's scale of the group, transposed by movmatrix.
 //            One more MMA with A all -8 * 2^-24 makes the codes signed 16
 //            positions at a time, before the sum could grow by them.
-// Only the weights are rounded (to fp16; for fp32 rows a second fp16 term
-// carries the rest, as for q).  So that they use fp16's range whatever the
-// values' size, they are scaled by a power of two that follows the largest
+// Only the weights are rounded, to fp16.  So that they use fp16's range whatever
+// the values' size, they are scaled by a power of two that follows the largest
 // scale seen; a head's q is scaled by the power of two of its largest value.
+//   fp32 rows  q and the weights have a second fp16 term that carries the rest.
+//            The tensor core lines products up by their operands' exponents, a
+//            subnormal's being 2^-14 whatever it holds, and drops what falls below: a sum of
+//            subnormals keeps 2^-18 of itself.  That is enough for rows of 16
+//            bits and not here, so the codes become normal numbers n - 8, an
+//            instruction more an operand but no MMA for the signs; and as its sums are
+//            cut towards 0, a block's sum of values is added to the others outside of it.
 //
 // The units of work, 32 positions of 8 heads of one KV head, of all sequences form one
 // list that is cut evenly over the CTAs (ragged batches stay balanced).  Each warp
@@ -96,6 +102,15 @@ __device__ __forceinline__ uint32_t at_pack(float lo, float hi) {
     return r;
 }
 __device__ __forceinline__ float2 at_unpack(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2 *>(&x)); }
+// Codes n and their fp16 operands.  Plain: the subnormals n 2^-24, by a mask.
+// Signed: n - 8, an exponent set beside the code and taken off again.  Of odd codes, 16 times these.
+constexpr uint32_t AT_EVEN = 0x000f000fu, AT_ODD = 0x00f000f0u;
+template <uint32_t CODES, bool SIGNED> __device__ __forceinline__ uint32_t at_codes(uint32_t w) {
+    if (!SIGNED) return w & CODES;
+    const uint32_t x = (w & CODES) | 0x64006400u;   // 1024 + n; 1024 + 16 n
+    const __half2 y = __hsub2(*reinterpret_cast<const __half2 *>(&x), __float2half2_rn(CODES == AT_EVEN ? 1032.0f : 1152.0f));
+    return *reinterpret_cast<const uint32_t *>(&y);
+}
 template <int N> struct AtWords { uint32_t w[N]; };
 template <int N> __device__ __forceinline__ AtWords<N> at_lds(const uint8_t *p) {
     AtWords<N> r;
@@ -201,6 +216,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
     constexpr int NB = G::NB, STAGES = G::STAGES;
     constexpr bool FINE = sizeof(T) == 4;      // fp32 rows: second terms of q and of the weights
     constexpr int TERMS = FINE ? 2 : 1;
+    constexpr float UNIT = FINE ? 1.0f : 16777216.0f;   // 1 / a code's operand
     extern __shared__ __align__(128) uint8_t at_smem[];
     __shared__ uint64_t full[AT_WARPS][STAGES];
     __shared__ int scan[AT_WARPS];
@@ -380,7 +396,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
             // 2^(11 - exponent) brings the largest to [2^11, 2^12)
             const int e0 = max(12, (int)(__float_as_uint(top) >> 23));
             const float up = __uint_as_float((uint32_t)(265 - e0) << 23);
-            const float down = __uint_as_float((uint32_t)(e0 - 11) << 23) * a.scale * 1.4426950408889634f * 16777216.0f;
+            const float down = __uint_as_float((uint32_t)(e0 - 11) << 23) * a.scale * 1.4426950408889634f * UNIT;
             float sum[NB];
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
@@ -445,24 +461,30 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
                 dv[k][0] = at_lds<NB / 2>(blk + kv4_off_dv(HD) + g * 2 * NB);
                 dv[k][1] = at_lds<NB / 2>(blk + kv4_off_dv(HD) + (g + 8) * 2 * NB);
                 float acc[NB][4];
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-                    at_mma(acc[b], w0.w[b] & 0x000f000fu, w1.w[b] & 0x000f000fu, w0.w[b] >> 8 & 0x000f000fu,
-                           w1.w[b] >> 8 & 0x000f000fu, qf[0][b][0][0], qf[0][b][0][1], start[b][0], start[b][1], start[b][0],
-                           start[b][1]);
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-                    at_mma(acc[b], w0.w[b] & 0x00f000f0u, w1.w[b] & 0x00f000f0u, w0.w[b] >> 8 & 0x00f000f0u,
-                           w1.w[b] >> 8 & 0x00f000f0u, qf[0][b][1][0], qf[0][b][1][1]);
-                if (FINE) {
+                if (!FINE) {
 #pragma unroll
                     for (int b = 0; b < NB; ++b)
-                        at_mma(acc[b], w0.w[b] & 0x000f000fu, w1.w[b] & 0x000f000fu, w0.w[b] >> 8 & 0x000f000fu,
-                               w1.w[b] >> 8 & 0x000f000fu, qf[TERMS - 1][b][0][0], qf[TERMS - 1][b][0][1]);
+                        at_mma(acc[b], w0.w[b] & AT_EVEN, w1.w[b] & AT_EVEN, w0.w[b] >> 8 & AT_EVEN, w1.w[b] >> 8 & AT_EVEN,
+                               qf[0][b][0][0], qf[0][b][0][1], start[b][0], start[b][1], start[b][0], start[b][1]);
 #pragma unroll
                     for (int b = 0; b < NB; ++b)
-                        at_mma(acc[b], w0.w[b] & 0x00f000f0u, w1.w[b] & 0x00f000f0u, w0.w[b] >> 8 & 0x00f000f0u,
-                               w1.w[b] >> 8 & 0x00f000f0u, qf[TERMS - 1][b][1][0], qf[TERMS - 1][b][1][1]);
+                        at_mma(acc[b], w0.w[b] & AT_ODD, w1.w[b] & AT_ODD, w0.w[b] >> 8 & AT_ODD, w1.w[b] >> 8 & AT_ODD,
+                               qf[0][b][1][0], qf[0][b][1][1]);
+                } else {
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        const uint32_t w[4] = {w0.w[b], w1.w[b], w0.w[b] >> 8, w1.w[b] >> 8};
+                        uint32_t even[4], odd[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) even[i] = at_codes<AT_EVEN, FINE>(w[i]), odd[i] = at_codes<AT_ODD, FINE>(w[i]);
+#pragma unroll
+                        for (int f = TERMS - 1; f >= 0; --f) {
+                            if (f == TERMS - 1)
+                                at_mma(acc[b], even[0], even[1], even[2], even[3], qf[f][b][0][0], qf[f][b][0][1], 0.0f, 0.0f, 0.0f, 0.0f);
+                            else at_mma(acc[b], even[0], even[1], even[2], even[3], qf[f][b][0][0], qf[f][b][0][1]);
+                            at_mma(acc[b], odd[0], odd[1], odd[2], odd[3], qf[f][b][1][0], qf[f][b][1][1]);
+                        }
+                    }
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[k][e] = 0.0f;
@@ -564,16 +586,20 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
                     const uint32_t x1 = __byte_perm(v1.w[b >> 1], v1.w[NB / 2 + (b >> 1)], pick);
                     // rows g and g + 8: codes 2 x and, 16 times as large, 2 x + 1; then -8 of each
 #pragma unroll
-                    for (int x = 0; x < 2; ++x)
+                    for (int x = 0; x < 2; ++x) {
+                        const uint32_t c[4] = {at_codes<AT_EVEN, FINE>(x0 >> (8 * x)), at_codes<AT_ODD, FINE>(x0 >> (8 * x)),
+                                               at_codes<AT_EVEN, FINE>(x1 >> (8 * x)), at_codes<AT_ODD, FINE>(x1 >> (8 * x))};
+                        if (!FINE) {
+                            at_mma(o[b][x], c[0], c[1], c[2], c[3], pf[0][0], pf[0][1]);
+                            at_mma(o[b][x], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, pf[0][0], pf[0][1]);
+                        } else {      // a block's sum, added with rounding
+                            float part[4];
+                            at_mma(part, c[0], c[1], c[2], c[3], pf[TERMS - 1][0], pf[TERMS - 1][1], 0.0f, 0.0f, 0.0f, 0.0f);
+                            at_mma(part, c[0], c[1], c[2], c[3], pf[0][0], pf[0][1]);
 #pragma unroll
-                        for (int f = 0; f < TERMS; ++f)
-                            at_mma(o[b][x], x0 >> (8 * x) & 0x000f000fu, x0 >> (8 * x) & 0x00f000f0u,
-                                   x1 >> (8 * x) & 0x000f000fu, x1 >> (8 * x) & 0x00f000f0u, pf[f][0], pf[f][1]);
-#pragma unroll
-                    for (int x = 0; x < 2; ++x)
-#pragma unroll
-                        for (int f = 0; f < TERMS; ++f)
-                            at_mma(o[b][x], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, pf[f][0], pf[f][1]);
+                            for (int i = 0; i < 4; ++i) o[b][x][i] += part[i];
+                        }
+                    }
                 }
             }
             __syncwarp();                     // the slot has been read
@@ -585,7 +611,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
         for (int x = 0; x < 2; ++x)
 #pragma unroll
             for (int i = 4; i < 32; i <<= 1) l[x] += __shfl_xor_sync(0xffffffffu, l[x], i);
-        // l and o hold 2^(AT_SHIFT - power) too; o's codes 2^-24, odd ones 16 times as large
+        // l and o hold 2^(AT_SHIFT - power) too; o's codes 1 / UNIT, odd ones 16 times as large
         const float scaled = (float)(AT_SHIFT - power);
         if (g == 0) {
             join_m[warp][2 * t] = m[0] - scaled, join_m[warp][2 * t + 1] = m[1] - scaled;
@@ -596,8 +622,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
 #pragma unroll
             for (int e = 0; e < 2; ++e)       // values 32 b + 4 g .. + 3 of head 2 t + e
                 *reinterpret_cast<float4 *>(join + (warp * KV4_HEADS + 2 * t + e) * G::ROW + 32 * b + 4 * g) =
-                    make_float4(o[b][0][e] * 16777216.0f, o[b][0][e + 2] * 1048576.0f, o[b][1][e] * 16777216.0f,
-                                o[b][1][e + 2] * 1048576.0f);
+                    make_float4(o[b][0][e] * UNIT, o[b][0][e + 2] * (UNIT / 16), o[b][1][e] * UNIT, o[b][1][e + 2] * (UNIT / 16));
         __syncthreads();
         const bool whole = w.first == 0 && w.take == w.units;
         float *mine = a.partial + ((size_t)blockIdx.x * 2 + (w.first > 0 ? 0 : 1)) * G::SLOT;
