@@ -132,19 +132,35 @@ void launch_simple(const PackedArgs &a, int hd, cudaStream_t st) {
 // ---------------------------------------------------------------------------
 // tensor-core kernel
 // ---------------------------------------------------------------------------
-constexpr int PK_ROWS = 128;           // query rows a tile (MMA M), keys a tile of the ring
+constexpr int PK_ROWS = 128;           // query rows a tile (MMA M)
 constexpr int PK_STEP = 64;            // keys a step (MMA N of S, K of P V)
 constexpr int PK_THREADS = 384;        // three warpgroups
 // registers a thread, of 384 * 168 at launch: 2 * 208 + 80 <= 3 * 168
 constexpr int PK_SOFTMAX_REGS = 208, PK_OTHER_REGS = 80;
-constexpr uint32_t PK_TMEM_COLS = 512; // two S_0, two S_1 (64 columns each), O_0, O_1 (128): all, so they begin at 0
+constexpr uint32_t PK_TMEM_COLS = 512; // two S_0, two S_1 (64 columns each), O_0, O_1 (128; O_0 256): all, so they begin at 0
 constexpr float PK_GROWTH = 8.0f;      // log2 of what a row's maximum may grow by before its O is rescaled
 constexpr int PK_STAGES = 5;           // ring of K and V tiles
 
 template <int HD> struct PkGeom {
-    static constexpr int TILE = PK_ROWS * HD * 2;   // bytes of a Q, K or V tile
-    static constexpr size_t SMEM = 1024 + (size_t)(2 + PK_STAGES) * TILE;
+    static constexpr int TILES = HD == 256 ? 1 : 2;   // query tiles an item: a second O of 256 columns has no room
+    static constexpr int KEYS = HD == 256 ? 64 : 128; // keys a tile of the ring
+    static constexpr int STEPS = KEYS / PK_STEP;      // steps a tile of the ring
+    static constexpr int Q_TILE = PK_ROWS * HD * 2, KV_TILE = KEYS * HD * 2;   // bytes
+    static constexpr size_t SMEM = 1024 + (size_t)TILES * Q_TILE + (size_t)PK_STAGES * KV_TILE;
 };
+
+// Load i of an item of n ring tiles of K and of V: which side, and its tile j.
+// Tiles of two steps come as K_0, V_0, K_1, V_1, ...; of one step as K_0, K_1,
+// V_0, K_2, V_1, ..., since scores are taken two steps ahead.
+template <int STEPS> __device__ __forceinline__ bool pk_is_value(int i, int n, int &j) {
+    if (STEPS == 2) {
+        j = i >> 1;
+        return i & 1;
+    }
+    const bool v = i == 2 * n - 1 || (i >= 2 && (i & 1) == 0);
+    j = i == 2 * n - 1 ? n - 1 : v ? i / 2 - 1 : i < 2 ? i : (i + 1) / 2;
+    return v;
+}
 
 struct PkWork {
     int first, len, row0, head;        // the sequence's first row and length; the item's first row in it; len 0: no more
@@ -167,12 +183,13 @@ __device__ __forceinline__ void pk_tma_load(void *dst, const CUtensorMap *map, i
 }
 
 // Shared-memory descriptors without the address.  K-major (Q and K): as
-// sw128_desc.  MN-major, 128-byte-swizzled, of 128 K rows (V): a K row is 128
-// bytes (64 MN values), 8 of them 1024 bytes (SBO), the next 64 MN values 128
+// sw128_desc.  MN-major, 128-byte-swizzled, of `keys` K rows (V): a K row is 128
+// bytes (64 MN values), 8 of them 1024 bytes (SBO), the next 64 MN values `keys`
 // rows on (LBO).
 constexpr uint64_t PK_DESC_K = ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-constexpr uint64_t PK_DESC_MN = ((uint64_t)(PK_ROWS * 128 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
-                                ((uint64_t)2 << 61);
+constexpr uint64_t pk_desc_mn(int keys) {
+    return ((uint64_t)(keys * 128 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
 
 __device__ __forceinline__ bool pk_elect() {
     uint32_t p;
@@ -326,7 +343,7 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
     extern __shared__ uint8_t pk_smem_raw[];
     __shared__ PkBars B;
     uint8_t *sq = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(pk_smem_raw) + 1023) & ~(uintptr_t)1023);
-    uint8_t *skv = sq + 2 * G::TILE;
+    uint8_t *skv = sq + G::TILES * G::Q_TILE;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (warp == 0) {
@@ -366,7 +383,7 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
         ok = ok && mbar_wait_bounded(bar, parity & 1, a.status, HOLO_E_TIMEOUT);
         return ok;
     };
-    // item k's work, and the key tiles of its two query tiles
+    // item k's work, the key tiles of 128 of its two query tiles, and the tiles of the ring
     PkWork w = {};
     int n0 = 0, n1 = 0, n = 0;
     // steps of query tile t: the diagonal key tile's second half is for its rows from 64 on
@@ -379,32 +396,34 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
         w = B.work[k & 1];
         if (w.len == 0) return false;
         n0 = w.row0 / PK_ROWS + 1;
-        n1 = a.item_rows > PK_ROWS && w.len > w.row0 + PK_ROWS ? n0 + 1 : 0;
-        n = max(n0, n1);
+        n1 = G::TILES > 1 && a.item_rows > PK_ROWS && w.len > w.row0 + PK_ROWS ? n0 + 1 : 0;
+        n = G::STEPS == 2 ? max(n0, n1) : steps(0);
         return true;
     };
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PK_OTHER_REGS));
         if (warp == 10 && lane == 0) {
-            // ---- loads: Q_0, K_0, Q_1, V_0, K_1, V_1, ... ----
-            auto load = [&](uint8_t *dst, const CUtensorMap *map, int head, int row, uint64_t *bar) {
-                mbar_arrive_expect_tx(bar, G::TILE);
+            // ---- loads: Q_0, K_0, Q_1, then V and K ----
+            auto load = [&](uint8_t *dst, const CUtensorMap *map, int rows, int head, int row, uint64_t *bar) {
+                mbar_arrive_expect_tx(bar, rows * HD * 2);
 #pragma unroll
-                for (int x = 0; x < HD; x += 64) pk_tma_load(dst + x / 64 * (PK_ROWS * 128), map, x, head, row, bar);
+                for (int x = 0; x < HD; x += 64) pk_tma_load(dst + x / 64 * (rows * 128), map, x, head, row, bar);
             };
             int q[2] = {0, 0}, slot = 0, phase = 0, ahead = 0;   // Q tiles loaded, ring position, its tiles loaded in all
             for (int k = 0; next(k); ++k) {
                 const int kvh = w.head / a.group;
                 auto load_q = [&](int t) {
                     if (q[t] > 0 && !wait(&B.q_empty[t], q[t] + 1)) return;
-                    load(sq + t * G::TILE, &qmap, w.head, w.first + w.row0 + t * PK_ROWS, &B.q_full[t]);
+                    load(sq + t * G::Q_TILE, &qmap, PK_ROWS, w.head, w.first + w.row0 + t * PK_ROWS, &B.q_full[t]);
                     ++q[t];
                 };
                 load_q(0);
                 for (int i = 0; i < 2 * n && ok; ++i) {
                     if (!wait(&B.kv_empty[slot], phase + 1)) break;
-                    load(skv + slot * G::TILE, i & 1 ? &vmap : &kmap, kvh, w.first + (i >> 1) * PK_ROWS, &B.kv_full[slot]);
+                    int j;
+                    const bool v = pk_is_value<G::STEPS>(i, n, j);
+                    load(skv + slot * G::KV_TILE, v ? &vmap : &kmap, G::KEYS, kvh, w.first + j * G::KEYS, &B.kv_full[slot]);
                     ++ahead;
                     if (++slot == PK_STAGES) slot = 0, phase ^= 1;
                     if (i == 0 && n1) load_q(1);
@@ -426,7 +445,7 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
             constexpr uint32_t HALF = PK_STEP * 128 >> 4;   // 64 rows of a 128-byte-wide tile, in a descriptor
             const int t = warp - 8;
             const bool leader = pk_elect();
-            const uint32_t sq_at = __shfl_sync(0xffffffffu, smem_addr(sq) >> 4, 0), skv_at = sq_at + (2 * G::TILE >> 4);
+            const uint32_t sq_at = __shfl_sync(0xffffffffu, smem_addr(sq) >> 4, 0), skv_at = sq_at + (G::TILES * G::Q_TILE >> 4);
             int q = 0, it = 0;                     // Q tiles, steps so far
             int slot = 0, phase = 0;               // of the next ring tile
             auto wait_all = [&](uint64_t *bar, int parity) {
@@ -440,16 +459,17 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
             auto advance = [&]() {
                 if (++slot == PK_STAGES) slot = 0, phase ^= 1;
             };
-            // S of step x of all: Q_t and half h of the K tile in slot kv
+            // S of step x of all: Q_t and part h of the K tile in slot kv
             auto scores = [&](int x, int kv, int h) {
                 tc_fence_after();
-                const uint64_t qd = PK_DESC_K | (uint64_t)(sq_at + t * (G::TILE >> 4));
-                const uint64_t kd = PK_DESC_K | (uint64_t)(skv_at + kv * (G::TILE >> 4) + h * HALF);
+                const uint64_t qd = PK_DESC_K | (uint64_t)(sq_at + t * (G::Q_TILE >> 4));
+                const uint64_t kd = PK_DESC_K | (uint64_t)(skv_at + kv * (G::KV_TILE >> 4) + h * HALF);
                 if (leader) {
 #pragma unroll
                     for (int s = 0; s < HD / 16; ++s) {
-                        const uint64_t off = (uint64_t)(((s >> 2) * (PK_ROWS * 128) + (s & 3) * 32) >> 4);
-                        tc_mma(t * 128 + (x & 1) * PK_STEP, qd + off, kd + off, id_s, s > 0);
+                        const uint64_t qo = (uint64_t)(((s >> 2) * (PK_ROWS * 128) + (s & 3) * 32) >> 4);
+                        const uint64_t ko = (uint64_t)(((s >> 2) * (G::KEYS * 128) + (s & 3) * 32) >> 4);
+                        tc_mma(t * 128 + (x & 1) * PK_STEP, qd + qo, kd + ko, id_s, s > 0);
                     }
                     tc_commit(&B.s_full[t][x & 1]);
                 }
@@ -460,7 +480,7 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
                 if (!__all_sync(0xffffffffu, more)) break;
                 const int ns = __shfl_sync(0xffffffffu, steps(t), 0), tiles = __shfl_sync(0xffffffffu, n, 0);
                 int k_slot = 0, v_slot = 0;
-                // K_0, then V_j and K_(j+1) for every j
+                // the ring's tiles in the order of their loads
                 if (ns > 0) {
                     if (!wait_all(&B.q_full[t], q++) || !wait_all(&B.kv_full[slot], phase)) break;
                     k_slot = slot;
@@ -468,15 +488,22 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
                     if (it > 1 && !wait_all(&B.o_done[t][it & 1], (it >> 1) + 1)) break;
                     scores(it, k_slot, 0);
                     if (ns > 1) {
+                        if (G::STEPS == 1) {
+                            commit(&B.kv_empty[k_slot]);
+                            advance();
+                            if (!wait_all(&B.kv_full[slot], phase)) break;
+                            k_slot = slot;
+                        }
                         if (it > 0 && !wait_all(&B.o_done[t][(it + 1) & 1], ((it + 1) >> 1) + 1)) break;
-                        scores(it + 1, k_slot, 1);
+                        scores(it + 1, k_slot, G::STEPS - 1);
                     }
                     commit(&B.kv_empty[k_slot]);
                     if (ns <= 2) commit(&B.q_empty[t]);
                     advance();
                 }
                 for (int x = 0; x < ns && ok; ++x, ++it) {
-                    const int h = x & 1;
+                    const int h = x & (G::STEPS - 1);
+                    const bool last = h == G::STEPS - 1;   // of its ring tile
                     if (h == 0) {
                         v_slot = slot;
                         if (!wait_all(&B.kv_full[v_slot], phase)) break;
@@ -485,14 +512,14 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
                     }
                     if (!wait_all(&B.p_full[t][it & 1], it >> 1)) break;
                     tc_fence_after();
-                    const uint64_t v = PK_DESC_MN | (uint64_t)(skv_at + v_slot * (G::TILE >> 4) + h * HALF);
+                    const uint64_t v = pk_desc_mn(G::KEYS) | (uint64_t)(skv_at + v_slot * (G::KV_TILE >> 4) + h * HALF);
                     if (leader) {
 #pragma unroll
                         for (int s = 0; s < PK_STEP / 16; ++s)   // 16 keys: 8 columns of P, 16 rows of V
                             tc_mma_ts(256 + t * 128, t * 128 + (it & 1) * PK_STEP + 8 * s, v + (uint64_t)(s * 2048 >> 4), id_o,
                                       x > 0 || s > 0);
                         tc_commit(&B.o_done[t][it & 1]);
-                        if (h || x + 1 == ns) tc_commit(&B.kv_empty[v_slot]);
+                        if (last || x + 1 == ns) tc_commit(&B.kv_empty[v_slot]);
                     }
                     __syncwarp();
                     if (x + 2 < ns) {
@@ -504,12 +531,12 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
                         // P of this step and the next S but one share columns: P has been read first
                         if (!wait_all(&B.o_done[t][it & 1], it >> 1)) break;
                         scores(it, k_slot, h);
-                        if (h || x + 3 == ns) commit(&B.kv_empty[k_slot]);
+                        if (last || x + 3 == ns) commit(&B.kv_empty[k_slot]);
                         if (x + 3 == ns) commit(&B.q_empty[t]);
                     }
                 }
                 // tiles that only the other query tile reads
-                for (int i = 2 * ((ns + 1) / 2); i < 2 * tiles && ok; ++i) {
+                for (int i = 2 * ((ns + G::STEPS - 1) / G::STEPS); i < 2 * tiles && ok; ++i) {
                     if (!wait_all(&B.kv_full[slot], phase)) break;
                     if (leader) mbar_arrive(&B.kv_empty[slot]);
                     advance();
@@ -579,19 +606,19 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
                     wait(&B.kv_full[slot], phase);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
-                    const int j = i >> 1;
-                    if (careful && (i & 1) && j >= n0 - 1) {
+                    int j;
+                    if (pk_is_value<G::STEPS>(i, n, j) && careful && j * G::KEYS >= w.row0) {
                         // a diagonal tile of V: no value that is not finite in a masked place
-                        uint4 *tile = reinterpret_cast<uint4 *>(skv + slot * G::TILE);
+                        uint4 *tile = reinterpret_cast<uint4 *>(skv + slot * G::KV_TILE);
                         constexpr uint32_t X = PkType<T>::EXPONENT;
 #pragma unroll 4
-                        for (int e = lane; e < G::TILE / 16; e += 32) {
+                        for (int e = lane; e < G::KV_TILE / 16; e += 32) {
                             const uint4 v = tile[e];
                             const uint32_t b[4] = {__vcmpeq2(v.x & X, X), __vcmpeq2(v.y & X, X), __vcmpeq2(v.z & X, X),
                                                    __vcmpeq2(v.w & X, X)};
                             if (b[0] | b[1] | b[2] | b[3]) {
                                 tile[e] = make_uint4(v.x & ~b[0], v.y & ~b[1], v.z & ~b[2], v.w & ~b[3]);
-                                const int key = j * PK_ROWS + (e & (PK_ROWS * 8 - 1)) / 8;   // 8 pieces of 16 bytes a key
+                                const int key = j * G::KEYS + (e & (G::KEYS * 8 - 1)) / 8;   // 8 pieces of 16 bytes a key
                                 if (key < w.len) atomicMin(&B.bad_from[k & 1], key);
                             }
                         }
@@ -695,7 +722,7 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
                 // 32 values a lane at a time; four lanes turn their 16-byte pieces round, so that they store 64 bytes of a row
                 const int part = lane & 3, i4 = i - part, n4 = w.len - i4;   // the first row of the four, rows from it on
                 T *o = (T *)a.out + (size_t)(w.first + min(i4, w.len - 1)) * a.out_row + (size_t)w.head * a.out_head + 8 * part;
-#pragma unroll
+#pragma unroll (HD == 256 ? 2 : HD / 32)
                 for (int cb = 0; cb < HD; cb += 32) {
                     uint32_t v[32];
                     tc_ld32(to + cb, v);
@@ -758,12 +785,13 @@ EncodeTiled encode_tiled() {
     return fn;
 }
 
-// [rows][heads][hd] as boxes of 128 rows of one head, 64 values wide; rows past
+// [rows][heads][hd] as boxes of `tall` rows of one head, 64 values wide; rows past
 // the end read as zeros.  A stride that one row or head leaves open is any valid one.
-bool make_map(CUtensorMap *map, int type, const void *p, int hd, int heads, int rows, long long row, long long head) {
+bool make_map(CUtensorMap *map, int type, const void *p, int hd, int heads, int rows, long long row, long long head,
+              int tall) {
     const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)heads, (cuuint64_t)rows};
     const cuuint64_t strides[2] = {(cuuint64_t)head * 2, (cuuint64_t)row * 2};
-    const cuuint32_t box[3] = {64, 1, PK_ROWS}, one[3] = {1, 1, 1};
+    const cuuint32_t box[3] = {64, 1, (cuuint32_t)tall}, one[3] = {1, 1, 1};
     const CUtensorMapDataType dt = type == HOLO_DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     return encode_tiled()(map, dt, 3, const_cast<void *>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -774,9 +802,9 @@ template <typename T, int HD>
 bool launch_tc(const PackedArgs &a, int type, cudaStream_t st) {
     CUtensorMap qm, km, vm;
     const int kv = a.n_heads / a.group;
-    if (!make_map(&qm, type, a.q, HD, a.n_heads, a.total, a.q_row, a.q_head) ||
-        !make_map(&km, type, a.k, HD, kv, a.total, a.k_row, a.k_head) ||
-        !make_map(&vm, type, a.v, HD, kv, a.total, a.v_row, a.v_head))
+    if (!make_map(&qm, type, a.q, HD, a.n_heads, a.total, a.q_row, a.q_head, PK_ROWS) ||
+        !make_map(&km, type, a.k, HD, kv, a.total, a.k_row, a.k_head, PkGeom<HD>::KEYS) ||
+        !make_map(&vm, type, a.v, HD, kv, a.total, a.v_row, a.v_head, PkGeom<HD>::KEYS))
         return false;
     static bool configured[16] = {false};
     int dev = 0;
@@ -791,9 +819,14 @@ bool launch_tc(const PackedArgs &a, int type, cudaStream_t st) {
     PackedArgs w = a;
     const int sms = holo_dev()->sms;
     auto items = [&](int rows) { return ((long long)a.total + (long long)(rows - 1) * a.n_seqs) / rows * a.n_heads; };
-    w.item_rows = items(2 * PK_ROWS) >= sms ? 2 * PK_ROWS : PK_ROWS;
+    w.item_rows = PkGeom<HD>::TILES == 2 && items(2 * PK_ROWS) >= sms ? 2 * PK_ROWS : PK_ROWS;
     const unsigned grid = (unsigned)min((long long)sms, items(w.item_rows));
     return holo_launch_early(packed_tc_kernel<T, HD>, grid, PK_THREADS, PkGeom<HD>::SMEM, st, w, qm, km, vm) == cudaSuccess;
+}
+
+template <typename T>
+bool launch_tc(const PackedArgs &a, int hd, int type, cudaStream_t st) {
+    return hd == 64 ? launch_tc<T, 64>(a, type, st) : hd == 128 ? launch_tc<T, 128>(a, type, st) : launch_tc<T, 256>(a, type, st);
 }
 
 // whether TMA can address rows of this base and these strides (elements)
@@ -837,11 +870,10 @@ extern "C" int cuda_attention_packed(const holo_packed_desc *d, void *out, const
         return refuse(HOLO_E_ARG);
     cudaStream_t st = d->stream ? (cudaStream_t)d->stream : holo_stream();
     bool done = false;
-    if (hd <= 128 && tma_rows(q, a.q_row, a.q_head) && tma_rows(k, a.k_row, a.k_head) && tma_rows(v, a.v_row, a.v_head) &&
-        tma_rows(out, a.out_row, a.out_head) && encode_tiled()) {
-        if (d->type == HOLO_DT_F16) done = hd == 64 ? launch_tc<__half, 64>(a, d->type, st) : launch_tc<__half, 128>(a, d->type, st);
-        else done = hd == 64 ? launch_tc<__nv_bfloat16, 64>(a, d->type, st) : launch_tc<__nv_bfloat16, 128>(a, d->type, st);
-    }
+    if (tma_rows(q, a.q_row, a.q_head) && tma_rows(k, a.k_row, a.k_head) && tma_rows(v, a.v_row, a.v_head) &&
+        tma_rows(out, a.out_row, a.out_head) && encode_tiled())
+        done = d->type == HOLO_DT_F16 ? launch_tc<__half>(a, d->head_dim, d->type, st)
+                                      : launch_tc<__nv_bfloat16>(a, d->head_dim, d->type, st);
     if (!done) {
         if (d->type == HOLO_DT_F16) launch_simple<__half>(a, d->head_dim, st);
         else launch_simple<__nv_bfloat16>(a, d->head_dim, st);

@@ -102,6 +102,26 @@ def test_values_in_masked_places_of_a_long_sequence(packed, n):
         assert torch.equal(packed(q, k, v, cu), want)
 
 
+@pytest.mark.parametrize("lens", [[64, 65, 1, 192], [1500, 77]])
+def test_wide_heads(packed, lens):
+    """Head size 256: its key tiles of 64, their edges, and many of them."""
+    check(packed, lens, 4, 2, 256, "bf16", 11, spread=2.0)
+
+
+@pytest.mark.parametrize("n", [60, 130, 321, 700])
+def test_values_in_masked_places_of_wide_heads(packed, n):
+    q, k, v = rows([n, 200], 2, 1, 256, "f16", n)
+    cu = cu_of([n, 200])
+    want = packed(q, k, v, cu).clone()
+    k2, v2 = k.clone(), v.clone()
+    v2[n:], k2[n:] = float("nan"), float("nan")
+    v2[n - 20:n], k2[n - 20:n] = float("inf"), float("nan")
+    for _ in range(3):
+        got = packed(q, k2, v2, cu)
+        assert torch.equal(got[:n - 20], want[:n - 20]) and got[n - 20:].isnan().all()
+        assert torch.equal(packed(q, k, v, cu), want)
+
+
 def test_strides(packed):
     """q, k and v as columns of one matrix of rows, heads before rows, and an odd offset that no wide load takes."""
     lens, heads, n_kv, hd = [130, 30], 4, 2, 64
