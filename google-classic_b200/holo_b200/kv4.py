@@ -17,6 +17,7 @@ from . import load
 from .attention import DTYPES, check, row_stride, stream_of
 
 BLOCK = 16   # positions a block of a page
+INT = torch.int32
 
 
 class Kv4Desc(C.Structure):
@@ -101,30 +102,35 @@ class Kv4Cache:
     def extend(self, counts, seqs=None, start=None):
         """Room for counts[i] more positions of each sequence; returns start,
         their lengths before (-1 where there was no room)."""
-        _ints(counts, "Kv4Cache.extend: counts")
-        p, n = self._seqs(seqs, counts.shape[0])
+        i, n = self._index, counts.numel()
+        p, m = (None, n) if seqs is None else self._seqs(seqs)
         if start is None:
             start = torch.empty_like(counts)
-        if counts.shape != (n,) or _ints(start, "Kv4Cache.extend: start").shape != (n,):
+        if m != n or start.numel() != n:
             raise ValueError("Kv4Cache.extend: one count and start a sequence")
+        if counts.dtype != INT or start.dtype != INT or not counts.is_contiguous() or not start.is_contiguous():
+            raise TypeError("Kv4Cache.extend: counts and start are contiguous int32 vectors")
+        if counts.get_device() != i or start.get_device() != i:
+            raise ValueError("Kv4Cache.extend: a tensor is not on the cache's device")
         self._call("cuda_kv4_extend", self.lib.cuda_kv4_extend, p, counts.data_ptr(), start.data_ptr(), n)
         return start
 
     def _rows(self, what, k, v, cu_rows, start, seqs):
-        shape, n = k.shape, cu_rows.shape[0] - 1
+        shape, n = k.shape, cu_rows.numel() - 1
         p, m = (None, n) if seqs is None else self._seqs(seqs)
-        if shape != v.shape or len(shape) != 3 or shape[1:] != self._heads or m != n or start.shape != (n,):
+        if shape != v.shape or len(shape) != 3 or shape[1:] != self._heads or m != n or start.numel() != n:
             raise ValueError(f"{what}: k {tuple(k.shape)}, v {tuple(v.shape)}, {n} sequences in cu_rows")
         dtype = k.dtype
         if dtype not in DTYPES or v.dtype != dtype:
             raise TypeError(f"{what}: k {k.dtype}, v {v.dtype}")
-        if cu_rows.dtype != torch.int32 or start.dtype != torch.int32 or not cu_rows.is_contiguous() or not start.is_contiguous():
+        if cu_rows.dtype != INT or start.dtype != INT or not cu_rows.is_contiguous() or not start.is_contiguous():
             raise TypeError(f"{what}: cu_rows and start are contiguous int32 vectors")
         i = self._index
         if k.get_device() != i or v.get_device() != i or cu_rows.get_device() != i or start.get_device() != i:
             raise ValueError(f"{what}: a tensor is not on the cache's device")
-        return (k.data_ptr(), v.data_ptr(), DTYPES[dtype], row_stride(k, *self._heads, what), row_stride(v, *self._heads, what),
-                shape[0], cu_rows.data_ptr(), start.data_ptr(), p, n)
+        k_row = 0 if k.is_contiguous() else row_stride(k, *self._heads, what)
+        v_row = 0 if v.is_contiguous() else row_stride(v, *self._heads, what)
+        return (k.data_ptr(), v.data_ptr(), DTYPES[dtype], k_row, v_row, shape[0], cu_rows.data_ptr(), start.data_ptr(), p, n)
 
     def append(self, layer: int, k, v, cu_rows, start, seqs=None):
         """Writes rows cu_rows[i] .. cu_rows[i + 1] of k and v [rows][n_kv_heads]

@@ -439,3 +439,20 @@ def test_kernels_report_what_they_leave_out(kv4):
     with pytest.raises(RuntimeError, match=str(hb.HOLO_E_ARG)):
         cache.check()
     assert torch.equal(cache.pool, before)
+
+
+def test_vectors_of_another_device_are_refused(kv4):
+    cache = kv4.Kv4Cache(1, 1, 64, 16, 4, 2, 2)
+    host, here = torch.ones(1, dtype=torch.int32), ints(1)
+    x = torch.zeros(1, 1, 64, device="cuda")
+    for call in (lambda: cache.extend(host), lambda: cache.extend(here, start=host), lambda: cache.append(0, x, x, cu_of([1]), host),
+                 lambda: cache.append(0, x, x, cu_of([1]).cpu(), here), lambda: cache.append(0, x.cpu(), x, cu_of([1]), here),
+                 lambda: cache.attention(0, x.cpu()), lambda: cache.attention(0, x, out=x.cpu())):
+        with pytest.raises(ValueError):
+            call()
+    for call in (lambda: cache.extend(here, host), lambda: cache.fork(host, here), lambda: cache.release(host),
+                 lambda: cache.copy_pages(here, host)):
+        with pytest.raises(TypeError):
+            call()
+    cache.check()
+    assert cache.lens.tolist() == [0, 0]
