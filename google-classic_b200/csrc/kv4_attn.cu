@@ -234,7 +234,9 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
     early_wait();
     early_next();
 
-    auto zeros = [&]() {                      // sequences without positions (a number out of range: left alone)
+    bool empty = false;                       // there are sequences without positions
+    auto zeros = [&]() {                      // theirs (a number out of range: left alone)
+        if (!empty) return;
         for (int i = blockIdx.x; i < a.n; i += gridDim.x) {
             int s, len;
             if (at_units(c, a, i, s, len) == 0 && s >= 0)
@@ -259,6 +261,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
         all += total;
         held += __syncthreads_count(u0 > 0);
     }
+    empty = held < a.n;
     // a CTA an item, or more where they keep AT_MIN units each
     const int units = all - held * items * a.item_cost;
     const int ctas = max(1, min(min((int)gridDim.x, units), max(held * items, units / AT_MIN)));
@@ -741,7 +744,10 @@ bool launch(const Kv4View &view, AtArgs a, int sms, cudaStream_t st) {
             return false;
         if (dev < 16) configured[dev] = true;
     }
-    const int grid = min(sms * G::CTAS, KV4_MAX_CTAS);
+    // no more CTAs than the sequences could keep busy if their tables were full
+    const long long items = (long long)a.n * view.n_kv * a.chunks;
+    const long long most = ((long long)view.max_pages * view.page_tokens + AT_UNIT_POS * AT_MIN - 1) / (AT_UNIT_POS * AT_MIN);
+    const int grid = (int)min((long long)min(sms * G::CTAS, KV4_MAX_CTAS), items * most);
     return holo_launch_early(kv4_attn_kernel<T, HD>, grid, AT_THREADS, G::SMEM, st, view, a) == cudaSuccess;
 }
 
