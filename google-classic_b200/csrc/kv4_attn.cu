@@ -68,7 +68,7 @@ struct AtArgs {
     int item_cost;                             // what an item costs besides its units, in units: its q, the join
     float scale;
     uint32_t page_magic;                       // ceil(2^32 / page_blocks); 0 for 1
-    bool wide;                                 // rows of out are 16-byte aligned
+    bool wide, q_wide;                         // rows of out, and of q, are 16-byte aligned
     int *counters;
     float *partial;
 };
@@ -186,11 +186,22 @@ __device__ __forceinline__ int at_scan(int v, int *sh, int &total) {
     return v;
 }
 
-// the list of `all` places cut evenly over `parts`
-struct Cuts {
-    int all, parts;
-    __device__ __forceinline__ int begin(int part) const { return (int)((long long)all * part / parts); }
-    __device__ __forceinline__ int part_of(int place) const { return (int)((((long long)place + 1) * parts - 1) / all); }
+// the values of q that a lane holds, as they lie: eight of every group
+template <typename T, int NB> struct AtQ {
+    alignas(16) T v[NB][8];
+    __device__ __forceinline__ void load(const T *q, bool wide, bool there) {
+        constexpr int N = 16 / sizeof(T);
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int e = 0; e < 8; e += N) {
+                if (!there) *reinterpret_cast<uint4 *>(&v[b][e]) = make_uint4(0, 0, 0, 0);
+                else if (wide) *reinterpret_cast<uint4 *>(&v[b][e]) = __ldcg(reinterpret_cast<const uint4 *>(q + 32 * b + e));
+                else
+#pragma unroll
+                    for (int i = 0; i < N; ++i) v[b][e + i] = q[32 * b + e + i];
+            }
+    }
 };
 
 template <typename T>
@@ -269,11 +280,15 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
         zeros();
         return;
     }
-    // Its part: the cuts of the list, moved down to the item's start
+    // Its part: `step` places of the list, the cuts moved down to the item's start
     // where the item is short.  Cuts inside longer items stay, so that the parts that an item spans follow from them.
-    const Cuts cuts = {all, ctas};
-    const int cut0 = cuts.begin(blockIdx.x), cut1 = cuts.begin(blockIdx.x + 1);
-    if (threadIdx.x == 0) part_start = 0, part_end = blockIdx.x + 1 == ctas ? all : 0;
+    const int step = (all + ctas - 1) / ctas;
+    const int cut0 = (int)blockIdx.x * step, cut1 = min(all, cut0 + step);
+    if (cut0 >= all) {                        // rounded up, they took all of it
+        zeros();
+        return;
+    }
+    if (threadIdx.x == 0) part_start = 0, part_end = cut1 == all ? all : 0;
     __syncthreads();
     {
         int before = 0;
@@ -312,6 +327,19 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
         return;
     }
 
+    // q of head g of an item's, quarter t of every group: loaded before it is wanted
+    AtQ<T, NB> raw;
+    auto heads_of = [&](const Walk &x, int &first) {
+        const int kvh = x.item / a.chunks;
+        first = kvh * a.group + (x.item % a.chunks) * KV4_HEADS;
+        return min(KV4_HEADS, (kvh + 1) * a.group - first);
+    };
+    auto load_q = [&](const Walk &x) {
+        int first;
+        const int n = heads_of(x, first);
+        raw.load((const T *)a.q + x.i * a.q_row + (long long)(first + g) * HD + 8 * t, a.q_wide, g < n);
+    };
+    constexpr bool EARLY = HD < 256;          // else its registers would be spilled
     // ---- the warp's loads: unit `unit` of item `load` ----
     // The walks lie in shared memory (one a warp each): only an item's change reads them.
     __shared__ Walk walk_load[AT_WARPS], walk_use[AT_WARPS];
@@ -348,6 +376,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
         }
     };
     look_up();
+    if (EARLY) load_q(head);
     int ahead = 0, fill = 0;                  // units issued and not yet taken, the slot of the next one
     auto issue = [&]() {                      // its copies, and the table entries of the next one
         if (unit >= unit_end) return;
@@ -372,26 +401,26 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
         look_up();
     };
     __syncwarp();
-    for (int k = 0; k < STAGES; ++k) issue();
+    issue();                                  // the others when q has been laid out: their table entries are on the way
 
     // ---- items ----
     int slot = 0, phase = 0;                  // the slot of the next unit to take and its barrier's phase
     bool ok = true;
-    for (bool more = true; more;) {
+    for (bool more = true, begun = false; more; begun = true) {
         const int len = w.len, u_end = w.first + w.take;
-        const int kvh = w.item / a.chunks, head0 = kvh * a.group + (w.item % a.chunks) * KV4_HEADS;
-        const int heads = min(KV4_HEADS, (kvh + 1) * a.group - head0);
-        // q of head g: quarter t of every group, times a power of two; B fragments of the two steps of a group
+        int head0;
+        const int heads = heads_of(w, head0);
+        if (!EARLY) load_q(w);
+        // q, times a power of two; B fragments of the two steps of a group
         uint32_t qf[TERMS][NB][2][2];
         float start[NB][2], factor[2];        // of heads 2 t and 2 t + 1
         {
             float qv[NB][8], top = 0.0f;
-            const T *q = (const T *)a.q + w.i * a.q_row + (long long)(head0 + g) * HD + 8 * t;
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    qv[b][e] = g < heads ? kv4_to_float<T>(q[32 * b + e]) : 0.0f;
+                    qv[b][e] = kv4_to_float<T>(raw.v[b][e]);
                     top = fmaxf(top, fabsf(qv[b][e]));
                 }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -441,6 +470,8 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
         int power = -32;                      // of two: the largest |value scale| lies below it
 
+        if (!begun)
+            for (int k = 1; k < STAGES; ++k) issue();
         for (int u = w.first + warp; u < u_end; u += AT_WARPS) {
             ok = ok && mbar_wait_bounded(&full[warp][slot], phase, c.status, HOLO_E_TIMEOUT);
             ok = __all_sync(0xffffffffu, ok);
@@ -609,6 +640,11 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
             issue();
         }
 
+        // the next item, and its q under way while the warps join
+        Walk after = w;
+        more = at_next(c, a, after, from, to);
+        if (EARLY && more) load_q(after);
+
         // ---- join the warps ----
 #pragma unroll
         for (int x = 0; x < 2; ++x)
@@ -665,7 +701,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
         if (!whole) {
             // the item's units lie in parts p0 .. p1; the last part to come joins their results, in order
             const int begins = w.start + a.item_cost;
-            const int p0 = cuts.part_of(begins), p1 = cuts.part_of(begins + w.units - 1);
+            const int p0 = begins / step, p1 = (begins + w.units - 1) / step;
             int *counter = a.counters + (size_t)w.i * items + w.item;
             __syncthreads();
             if (threadIdx.x == 0) {           // of all the CTA's writes, and before its reads
@@ -719,10 +755,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
             }
         }
         __syncthreads();                      // the join's memory is free again
-        Walk x = w;
-        more = at_next(c, a, x, from, to);
-        __syncwarp();
-        if (lane == 0) w = x;
+        if (lane == 0) w = after;
         __syncwarp();
     }
     zeros();
@@ -793,6 +826,7 @@ extern "C" int cuda_kv4_attention(const holo_kv4 *c, int layer, void *out, const
     if (units * n * c->n_kv_heads * a.chunks > 0x40000000LL) return refuse(HOLO_E_UNSUPPORTED);
     a.page_magic = view.page_blocks == 1 ? 0 : (uint32_t)((((uint64_t)1 << 32) + view.page_blocks - 1) / view.page_blocks);
     a.wide = (uintptr_t)out % 16 == 0 && out_row * size % 16 == 0;
+    a.q_wide = (uintptr_t)q % 16 == 0 && q_row * size % 16 == 0;
     a.counters = work.counters, a.partial = work.partial;
     // where there may be fewer items than CTAs, each CTA has one at most and its cost is the same for all
     a.item_cost = (long long)n * c->n_kv_heads * a.chunks >= holo_dev()->sms * 2 ? AT_ITEM : 0;
