@@ -25,13 +25,22 @@
 //            instruction more an operand but no MMA for the signs; and as its sums are
 //            cut towards 0, a block's sum of values is added to the others outside of it.
 //
-// The units of work, 32 positions of 8 heads of one KV head, of all sequences form one
+// The units of work, 64 positions of 8 heads of one KV head, of all sequences form one
 // list that is cut evenly over the CTAs (ragged batches stay balanced).  Each warp
 // streams every fourth unit of its CTA's part through a ring of its own, one
 // bulk copy a block of 16 positions, its table entry loaded a unit ahead, and
 // keeps a running maximum, sum and output; warps join in shared memory.  A
 // list item that is cut leaves partial results, and the CTA that comes last joins them in
-// their order, so the result does not depend on timing.
+// their order, so the result does not depend on timing; items of up to AT_WHOLE
+// units are not cut, so that a short sequence's result does not depend on its batch either.
+//
+// Measured: bound by instruction issue and, in long runs, by the board's power.  A unit takes a
+// warp 3500 cycles with two warps a scheduler (two CTAs an SM at 128 dims;
+// 12 warps an SM in three CTAs of 32-position units: 59.6 us against 61.7 in the batch below, but
+// 14.0 against 11.8 for one sequence and 164 against 157 for the long ones).  64 sequences
+// of up to 4096 (64 heads over 8 of 128, fp16): 54.9 us, 3.0 TB/s; 8 of up to
+// 131072 (bf16): 162 us, 4.1 TB/s; one of 2047 (32 over 32, fp32): 11.5 us, of which launch,
+// cut, tables and joins are 8.
 #include "kv4.cuh"
 
 #include <cuda_fp16.h>
@@ -640,9 +649,13 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
             issue();
         }
 
-        // the next item, and its q under way while the warps join
-        Walk after = w;
-        more = at_next(c, a, after, from, to);
+        // the next item (mostly where the loads are), and its q under way while the warps join
+        Walk after = load;
+        more = true;
+        if (after.take == 0 || after.start != w.start + w.units + a.item_cost) {
+            after = w;
+            more = at_next(c, a, after, from, to);
+        }
         if (EARLY && more) load_q(after);
 
         // ---- join the warps ----
@@ -708,8 +721,8 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
                 __threadfence();
                 last = atomicAdd(counter, 1) == p1 - p0;
                 if (last) {
-                    *counter = 0;
                     __threadfence();
+                    *counter = 0;             // for the next call
                 }
             }
             __syncthreads();
@@ -726,11 +739,14 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
                         float4 v[BATCH];
 #pragma unroll
                         for (int i = 0; i < BATCH; ++i) {
-                            const int k = min(k0 + i, parts - 1);
+                            const int k = k0 + i;
                             const float *p = part + (size_t)(k ? 2 * k - 1 : 0) * G::SLOT;
-                            ml[i] = __ldcg(reinterpret_cast<const float2 *>(p) + h);
-                            v[i] = __ldcg(reinterpret_cast<const float4 *>(p + 2 * KV4_HEADS + d));
-                            if (k0 + i >= parts) ml[i].y = 0.0f;
+                            ml[i] = make_float2(0.0f, 0.0f);
+                            v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            if (k < parts) {
+                                ml[i] = __ldcg(reinterpret_cast<const float2 *>(p) + h);
+                                v[i] = __ldcg(reinterpret_cast<const float4 *>(p + 2 * KV4_HEADS + d));
+                            }
                         }
                         float to = top;
 #pragma unroll
