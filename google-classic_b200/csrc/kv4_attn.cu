@@ -38,8 +38,8 @@
 // warp 3500 cycles with two warps a scheduler (two CTAs an SM at 128 dims;
 // 12 warps an SM in three CTAs of 32-position units: 59.6 us against 61.7 in the batch below, but
 // 14.0 against 11.8 for one sequence and 164 against 157 for the long ones).  64 sequences
-// of up to 4096 (64 heads over 8 of 128, fp16): 54.9 us, 3.0 TB/s; 8 of up to
-// 131072 (bf16): 162 us, 4.1 TB/s; one of 2047 (32 over 32, fp32): 11.5 us, of which launch,
+// of up to 4096 (64 heads over 8 of 128, fp16): 54.5 us, 3.1 TB/s; 8 of up to
+// 131072 (bf16): 158 to 166 us, 4.0 to 4.2 TB/s; one of 2047 (32 over 32, fp32): 11.5 us, of which launch,
 // cut, tables and joins are 8.
 #include "kv4.cuh"
 

@@ -6,8 +6,11 @@
 // a lane writes the word of its eight key codes, or two halfwords of value codes.
 // A CTA takes up to 16 rows, whose places (sequence, page, block) are looked up
 // once; rows that share a block meet in one CTA, so its partly written sectors are
-// completed in L2.  Both kernels move each byte once and are bound by memory
-// traffic where there are many rows, by latency where there are few.
+// completed in L2.  Both kernels move each byte once.  Few rows are bound by
+// latency (of the look-ups, the loads and the call); many, 22,400 of 8 heads of 128
+// in fp16, take 49 us to write (2.4 TB/s), bound by the quantiser's instructions, and
+// 33 us to read (3.6 TB/s), by the look-ups at a CTA's start and the stores.  More rows a CTA
+// (32, 64) or more rows' loads together in the read (2, 4) gained nothing.
 #include "kv4.cuh"
 
 #include <mutex>
@@ -125,8 +128,7 @@ __device__ __forceinline__ void store8(T *p, bool wide, const T (&x)[8]) {
 // Eight codes of a lane and the scale of its group, over the four lanes that
 // hold it: d = fp16(m / -8), code = rint(x / d) + 8 in 0..15 (fp32 arithmetic,
 // each operation rounded once), NaN as the scale where a value is not finite.
-// Bound by instructions (an append of many rows: 0.78 of the issue slots at 2.9
-// TB/s), so the work is put on the FMA pipe, which takes one a cycle:
+// Bound by instructions (an append of many rows: 0.79 of the issue slots), so the work is put on the FMA pipe, which takes one a cycle:
 //   m         from the group's largest and smallest value; where they are equal
 //             in size, or zero, from a second look for the first of them
 //   x / d     the rounded quotient without a division: from the rounded
