@@ -456,3 +456,52 @@ def test_vectors_of_another_device_are_refused(kv4):
             call()
     cache.check()
     assert cache.lens.tolist() == [0, 0]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_attention_rows_at_odd_addresses(kv4, dtype, hd):
+    """Rows that no wide load or store takes give the same bits."""
+    cache, _ = filled(kv4, [70, 1, 0, 600], 2, hd, 32, 21)
+    q = torch.randn(4, 6, hd, generator=torch.Generator().manual_seed(2)).to(DTYPES[dtype]).cuda()
+    want = cache.attention(0, q)
+    wide_q, wide_o = (torch.zeros(4, 6 * hd + 3, dtype=q.dtype, device="cuda") for _ in range(2))
+    wide_q[:, 1:-2] = q.flatten(1)
+    cache.attention(0, wide_q[:, 1:-2].unflatten(1, (6, hd)), wide_o[:, 1:-2].unflatten(1, (6, hd)))
+    cache.check()
+    assert torch.equal(wide_o[:, 1:-2].unflatten(1, (6, hd)), want)
+    assert not wide_o[:, 0].any() and not wide_o[:, -2:].any()
+
+
+def test_attention_of_many_sequences(kv4):
+    """More sequences than a CTA has threads, several a CTA, empty ones among them: each as it comes out alone (none is long
+    enough to be cut)."""
+    lens = np.random.default_rng(4).integers(0, 512, 300)
+    lens[[0, 7, 150, 298, 299]] = 0, 512, 1, 0, 64
+    cache, held = filled(kv4, lens.tolist(), 2, 64, 64, 31)
+    q = torch.randn(300, 6, 64, generator=torch.Generator().manual_seed(9)).cuda()
+    got = cache.attention(0, q).clone()
+    for i in (0, 7, 8, 127, 128, 150, 255, 256, 298, 299):
+        alone = cache.attention(0, q[i:i + 1], seqs=ints(i))
+        assert torch.equal(alone[0], got[i]), i
+    turned = torch.arange(299, -1, -1, dtype=torch.int32, device="cuda")
+    assert torch.equal(cache.attention(0, q.flip(0), seqs=turned).flip(0), got)
+    cache.check()
+    assert torch.equal(got.flatten(1).any(1).cpu(), torch.tensor(lens > 0))
+
+
+@pytest.mark.parametrize("lens,heads,n_kv,hd", [([33], 4, 2, 64), ([2047, 100], 4, 4, 128), ([20000], 8, 1, 128), ([900], 12, 1, 256)])
+def test_attention_of_fp32_rows_keeps_fp32(kv4, lens, heads, n_kv, hd):
+    """The norm of the error against 64 bits.  q and the weights are held to 2^-22, and so is a block's sum in the tensor core (16
+    positions, cut to 24 bits at up to four times the result); scores of size s, here up to about 5, are off by s 2^-22, and a
+    weight by as much; fp32's own roundings are half of each.  Each enters once a position, independently: no more than the sum
+    of their sizes relative to the result, (1 + 1 + 1 + 5 / 2) 2^-22 = 1.3e-6.  (fp16 weights would leave 1e-4.)"""
+    cache, held = filled(kv4, lens, n_kv, hd, 64, 41)
+    q = torch.randn(len(lens), heads, hd, generator=torch.Generator().manual_seed(43)).cuda()
+    y, qs, first = cache.attention(0, q).double().cpu().numpy(), q.double().cpu().numpy(), 0
+    cache.check()
+    for i, n in enumerate(lens):
+        want = np.stack([ref.attend(qs[i, h:h + 1], *(x[first:first + n, h * n_kv // heads] for x in held[0]), hd ** -0.5)[0][0]
+                         for h in range(heads)])
+        assert np.linalg.norm(y[i] - want) <= 1.3e-6 * np.linalg.norm(want), i
+        first += n
