@@ -437,7 +437,8 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
             // 2^(11 - exponent) brings the largest to [2^11, 2^12)
             const int e0 = max(12, (int)(__float_as_uint(top) >> 23));
             const float up = __uint_as_float((uint32_t)(265 - e0) << 23);
-            const float down = __uint_as_float((uint32_t)(e0 - 11) << 23) * a.scale * 1.4426950408889634f * UNIT;
+            // (never 0, which would make NaN of a masked score)
+            const float down = fmaxf(__uint_as_float((uint32_t)(e0 - 11) << 23) * a.scale * 1.4426950408889634f * UNIT, 1.17549435e-38f);
             float sum[NB];
 #pragma unroll
             for (int b = 0; b < NB; ++b) {

@@ -505,3 +505,17 @@ def test_attention_of_fp32_rows_keeps_fp32(kv4, lens, heads, n_kv, hd):
                          for h in range(heads)])
         assert np.linalg.norm(y[i] - want) <= 1.3e-6 * np.linalg.norm(want), i
         first += n
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_of_zero_queries_and_a_small_scale(kv4, dtype):
+    """Scores of 0, whatever the scale: the mean of the values, also where a unit's last positions are masked."""
+    cache, held = filled(kv4, [37, 1], 2, 64, 64, 51)
+    q = torch.zeros(2, 4, 64, dtype=DTYPES[dtype], device="cuda")
+    for scale in (0.0, 1e-10, 1e-30):
+        y = cache.attention(0, q, scale=scale).double().cpu().numpy()
+        for i, (a, n) in enumerate(((0, 37), (37, 1))):
+            v = held[0][1][a:a + n]
+            tol = ref.bound(np.zeros((1, 64)), held[0][0][a:a + n, 0], v, 1.0, dtype)
+            assert np.abs(y[i] - v.mean(0).repeat(2, 0)).max() <= tol
+    cache.check()
