@@ -142,6 +142,28 @@ def test_strides(packed):
     assert (got.double() - want.double()).abs().max() <= 2 * tol
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("hd", [128, 256])
+def test_rows_at_odd_addresses(packed, dtype, hd):
+    """Rows that no wide load takes, each of q, k and v and out, and their log-sum-exp: within both kernels' bounds of each other."""
+    lens, heads, n_kv = [66, 0, 1, 130], 4, 2
+    q, k, v = rows(lens, heads, n_kv, hd, dtype, 12)
+    cu, total = cu_of(lens), sum(lens)
+    lse = [torch.zeros(heads, total, device="cuda") for _ in range(2)]
+    want = packed(q, k, v, cu, lse=lse[0])
+
+    def odd(x):
+        wide = torch.zeros(total, x.shape[1] * hd + 3, dtype=x.dtype, device="cuda")
+        wide[:, 1:-2] = x.flatten(1)
+        return wide[:, 1:-2].unflatten(1, (-1, hd))
+
+    tol = 2 * ref.bound(*(x.double().cpu().numpy().reshape(-1, hd) for x in (q, k, v)), hd ** -0.5, dtype)
+    for case in ((odd(q), k, v, None), (q, odd(k), odd(v), None), (q, k, v, odd(torch.zeros_like(q)))):
+        got = packed(*case[:3], cu, out=case[3], lse=lse[1])
+        assert (got.double() - want.double()).abs().max() <= tol
+        assert (lse[0] - lse[1]).abs().max() <= 1e-4   # scores of up to about 6, sums of hd products rounded at random: 6 sqrt(hd) 2^-22 on both sides, and twice that
+
+
 def test_rows_outside_the_sequences_keep_their_memory(packed):
     """cu_seqlens that does not reach the last rows: no more than those rows' results may change."""
     q, k, v = rows([200], 2, 1, 64, "f16", 9)
