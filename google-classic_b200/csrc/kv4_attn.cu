@@ -38,8 +38,8 @@
 // warp 3500 cycles with two warps a scheduler (two CTAs an SM at 128 dims;
 // 12 warps an SM in three CTAs of 32-position units: 59.6 us against 61.7 in the batch below, but
 // 14.0 against 11.8 for one sequence and 164 against 157 for the long ones).  64 sequences
-// of up to 4096 (64 heads over 8 of 128, fp16): 54.5 us, 3.1 TB/s; 8 of up to
-// 131072 (bf16): 158 to 166 us, 4.0 to 4.2 TB/s; one of 2047 (32 over 32, fp32): 11.5 us, of which launch,
+// of up to 4096 (64 heads over 8 of 128, fp16): 55.0 us, 3.0 TB/s; 8 of up to
+// 131072 (bf16): 158 to 166 us, 4.0 to 4.2 TB/s; one of 2047 (32 over 32, fp32): 11.6 us, of which launch,
 // cut, tables and joins are 8.
 #include "kv4.cuh"
 
@@ -324,7 +324,17 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
         }
         __syncthreads();
     }
-    const int from = part_start, to = part_end;
+    int from = part_start, to = part_end;
+    // Where every item is one unit and the part has several, each warp takes a quarter of them
+    // for itself, and nothing is joined (the join of one warp's result leaves it as it is): 96
+    // sequences of up to 60, 32 heads of 128 over 32, in 20.8 us and not 47.2; a single item is no sooner done.
+    const int unit_items = units == held * items ? (to - from) / (1 + a.item_cost) : 0;
+    const bool solo = unit_items > 1;
+    if (solo) {
+        to = from + unit_items * (warp + 1) / AT_WARPS * (1 + a.item_cost);
+        from += unit_items * warp / AT_WARPS * (1 + a.item_cost);
+    }
+    const int unit0 = solo ? 0 : warp, unit_step = solo ? 1 : AT_WARPS;
     Walk head = begin;
     bool any = from < to;
     if (any) {
@@ -355,7 +365,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
     Walk &load = walk_load[warp], &w = walk_use[warp];
     if (lane == 0) load = head, w = head;
     __syncwarp();
-    int unit = head.first + warp, unit_end, load_len;   // unit_end 0: no more
+    int unit = head.first + unit0, unit_end, load_len;   // unit_end 0: no more
     const uint8_t *load_base;                 // of the KV head
     const int *load_table;
     const uint32_t page_bytes = (uint32_t)c.n_kv * c.page_blocks * G::BLOCK_BYTES;
@@ -364,7 +374,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
         bool more = true;
         while (more && unit >= x.first + x.take) {
             more = at_next(c, a, x, from, to);
-            unit = x.first + warp;
+            unit = x.first + unit0;
         }
         __syncwarp();
         if (lane == 0) load = x;
@@ -405,7 +415,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
         }
         ++ahead;
         fill = fill + 1 == STAGES ? 0 : fill + 1;
-        unit += AT_WARPS;
+        unit += unit_step;
         if (unit >= unit_end) settle();
         look_up();
     };
@@ -482,7 +492,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
 
         if (!begun)
             for (int k = 1; k < STAGES; ++k) issue();
-        for (int u = w.first + warp; u < u_end; u += AT_WARPS) {
+        for (int u = w.first + unit0; u < u_end; u += unit_step) {
             ok = ok && mbar_wait_bounded(&full[warp][slot], phase, c.status, HOLO_E_TIMEOUT);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
@@ -658,6 +668,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
             more = at_next(c, a, after, from, to);
         }
         if (EARLY && more) load_q(after);
+        T *out = (T *)a.out + w.i * a.out_row + (long long)head0 * HD;
 
         // ---- join the warps ----
 #pragma unroll
@@ -665,6 +676,20 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
 #pragma unroll
             for (int i = 4; i < 32; i <<= 1) l[x] += __shfl_xor_sync(0xffffffffu, l[x], i);
         // l and o hold 2^(AT_SHIFT - power) too; o's codes 1 / UNIT, odd ones 16 times as large
+        if (solo) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    if (2 * t + e < heads)
+                        at_store4<T>(out + (2 * t + e) * HD + 32 * b + 4 * g, a.wide, o[b][0][e] * UNIT / l[e],
+                                     o[b][0][e + 2] * (UNIT / 16) / l[e], o[b][1][e] * UNIT / l[e],
+                                     o[b][1][e + 2] * (UNIT / 16) / l[e]);
+            __syncwarp();
+            if (lane == 0) w = after;
+            __syncwarp();
+            continue;
+        }
         const float scaled = (float)(AT_SHIFT - power);
         if (g == 0) {
             join_m[warp][2 * t] = m[0] - scaled, join_m[warp][2 * t + 1] = m[1] - scaled;
@@ -695,7 +720,6 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
             if (!whole) mine[2 * h] = top, mine[2 * h + 1] = den;
         }
         __syncthreads();
-        T *out = (T *)a.out + w.i * a.out_row + (long long)head0 * HD;
         for (int d = 4 * threadIdx.x; d < heads * HD; d += 4 * AT_THREADS) {
             const int h = d / HD;
             float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);

@@ -519,3 +519,25 @@ def test_attention_of_zero_queries_and_a_small_scale(kv4, dtype):
             tol = ref.bound(np.zeros((1, 64)), held[0][0][a:a + n, 0], v, 1.0, dtype)
             assert np.abs(y[i] - v.mean(0).repeat(2, 0)).max() <= tol
     cache.check()
+
+
+@pytest.mark.parametrize("dtype,hd", [("f32", 64), ("f16", 128), ("bf16", 256)])
+def test_attention_of_many_short_sequences(kv4, dtype, hd):
+    """All of one unit of work or empty: several items a CTA, a warp each, as an item comes out that a CTA has to itself, and as the
+    formula has it."""
+    lens = np.random.default_rng(6).integers(0, 65, 300)
+    lens[[0, 7, 150, 298, 299]] = 0, 64, 1, 0, 64
+    cache, held = filled(kv4, lens.tolist(), 4, hd, 16, 61)
+    q = torch.randn(300, 12, hd, generator=torch.Generator().manual_seed(8)).to(DTYPES[dtype]).cuda()
+    got = cache.attention(0, q).clone()
+    ends = np.cumsum(lens)
+    for i in (0, 7, 8, 127, 128, 150, 255, 256, 298, 299):
+        assert torch.equal(cache.attention(0, q[i:i + 1], seqs=ints(i))[0], got[i]), i
+        k, v = (x[ends[i] - lens[i]:ends[i]] for x in held[0])
+        for h in range(12):
+            qh = q[i, h:h + 1].double().cpu().numpy()
+            want, _ = ref.attend(qh, k[:, h // 3], v[:, h // 3], hd ** -0.5)
+            tol = ref.bound(qh, k[:, h // 3], v[:, h // 3], hd ** -0.5, dtype)
+            assert np.abs(got[i, h].double().cpu().numpy() - want[0]).max() <= tol, (i, h)
+    cache.check()
+    assert torch.equal(got.flatten(1).any(1).cpu(), torch.tensor(lens > 0))
