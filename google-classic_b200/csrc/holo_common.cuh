@@ -141,8 +141,10 @@ struct HoloDevice {
     void *pinned = nullptr;              // 64 KB pinned host buffer
     void *tmp = nullptr;                 // growable scratch of the ABI helpers
     size_t tmp_bytes = 0;
-    void *kv4_work = nullptr;            // workspace of the paged 4-bit cache where the caller gives none
-    size_t kv4_work_bytes = 0;
+    // workspace of the paged 4-bit cache where the caller gives none; its counters apart, which are zero between calls
+    // whatever shapes of cache the calls are for
+    void *kv4_work = nullptr, *kv4_counters = nullptr;
+    size_t kv4_work_bytes = 0, kv4_counter_bytes = 0;
 };
 constexpr int MV_MAX_CTAS = 1024;
 constexpr int MV_MAX_ROWBLOCKS = 1 << 16;

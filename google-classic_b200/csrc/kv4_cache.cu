@@ -31,25 +31,34 @@ size_t partial_bytes(const holo_kv4 *c) {
 
 std::mutex g_work_mu;
 
-// the library's own workspace on the current device, zero when it is made
-void *own_work(size_t bytes) {
-    HoloDevice *D = holo_dev();
-    if (!D) return nullptr;
-    std::lock_guard<std::mutex> lk(g_work_mu);
-    if (D->kv4_work_bytes < bytes) {
-        cudaDeviceSynchronize();   // calls that use the old one
-        if (D->kv4_work) cudaFree(D->kv4_work);
-        D->kv4_work = nullptr;
-        D->kv4_work_bytes = 0;
-        if (cudaMalloc(&D->kv4_work, bytes) != cudaSuccess || cudaMemset(D->kv4_work, 0, bytes) != cudaSuccess ||
-            cudaDeviceSynchronize() != cudaSuccess) {
-            cudaGetLastError();
-            holo_set_status(HOLO_E_NOMEM, "kv4 workspace");
-            return nullptr;
-        }
-        D->kv4_work_bytes = bytes;
+// a buffer of the library's own on the current device, zero when it is made
+bool own_buffer(void *&buf, size_t &have, size_t bytes) {
+    if (have >= bytes) return true;
+    cudaDeviceSynchronize();   // calls that use the old one
+    if (buf) cudaFree(buf);
+    buf = nullptr;
+    have = 0;
+    if (cudaMalloc(&buf, bytes) != cudaSuccess || cudaMemset(buf, 0, bytes) != cudaSuccess ||
+        cudaDeviceSynchronize() != cudaSuccess) {
+        cudaGetLastError();
+        holo_set_status(HOLO_E_NOMEM, "kv4 workspace");
+        return false;
     }
-    return D->kv4_work;
+    have = bytes;
+    return true;
+}
+
+// The library's own workspace.  Caches of all shapes use it in turn, so the counters, which have to be zero before a
+// call, have a buffer that nothing else is written to; no call reads what another left in the other sections.
+bool own_work(HoloDevice *D, const holo_kv4 *c, Kv4Work *work) {
+    std::lock_guard<std::mutex> lk(g_work_mu);
+    if (!own_buffer(D->kv4_counters, D->kv4_counter_bytes, counter_bytes(c)) ||
+        !own_buffer(D->kv4_work, D->kv4_work_bytes, plan_bytes(c) + partial_bytes(c)))
+        return false;
+    work->counters = (int *)D->kv4_counters;
+    work->plan = (int *)D->kv4_work;
+    work->partial = (float *)((uint8_t *)D->kv4_work + plan_bytes(c));
+    return true;
 }
 
 // the sequence i with cu[i] <= row < cu[i + 1]: the last i with cu[i] <= row
@@ -370,9 +379,9 @@ bool kv4_begin(const holo_kv4 *c, int layer, const char *what, Kv4View &view, cu
     view.max_seqs = c->max_seqs;
     view.max_pages = c->max_pages;
     view.status = D->status;
+    if (work && !c->work) return own_work(D, c, work);
     if (work) {
-        uint8_t *w = (uint8_t *)(c->work ? c->work : own_work(cuda_kv4_work_bytes(c)));
-        if (!w) return false;
+        uint8_t *w = (uint8_t *)c->work;
         if ((uintptr_t)w % 16) {
             holo_set_status(HOLO_E_ARG, what);
             return false;

@@ -204,7 +204,7 @@ void cuda_clear_status(void) {
         cudaMemset(g_dev[id].status, 0, sizeof(int));
         cudaMemset(g_dev[id].mv_counters, 0, sizeof(int) * MV_MAX_ROWBLOCKS);
         cudaMemset(g_dev[id].mvb_counters, 0, sizeof(int) * MVB_MAX_GROUPS);
-        if (g_dev[id].kv4_work) cudaMemset(g_dev[id].kv4_work, 0, g_dev[id].kv4_work_bytes);
+        if (g_dev[id].kv4_counters) cudaMemset(g_dev[id].kv4_counters, 0, g_dev[id].kv4_counter_bytes);
         cudaDeviceSynchronize();
     }
     int n = 0;
@@ -284,6 +284,7 @@ void cuda_cleanup(void) {
     cudaFreeHost(D.pinned);
     if (D.tmp) cudaFree(D.tmp);
     if (D.kv4_work) cudaFree(D.kv4_work);
+    if (D.kv4_counters) cudaFree(D.kv4_counters);
     D = HoloDevice();
     std::lock_guard<std::mutex> lk(g_reg_mu);
     g_registry.clear();

@@ -379,7 +379,8 @@ typedef struct {
     void *pool;                             /* cuda_kv4_pool_bytes, 16-byte aligned */
     int *tables, *lens, *refs;
     void *work;                             /* cuda_kv4_work_bytes, zero-filled before the first call and kept by
-                                             * the calls; NULL: the library's own.  Calls that may overlap (other
+                                             * the calls, for caches of one shape; NULL: the library's own, which
+                                             * caches of any shape may share.  Calls that may overlap (other
                                              * streams) need work of their own */
     void *stream;                           /* cudaStream_t; NULL: the library's (cuda_set_stream) */
 } holo_kv4;

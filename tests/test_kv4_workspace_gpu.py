@@ -1,0 +1,67 @@
+"""The workspace of the paged 4-bit cache's calls (include/holo_b200.h,
+holo_kv4.work): the library's own, that of a Kv4Cache, and what else may run
+beside or between the calls that use it."""
+import ctypes as C
+
+import pytest
+import torch
+
+import holo_b200 as hb
+from test_kv4_gpu import filled, ints
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def kv4(dev):
+    from holo_b200 import kv4
+    return kv4
+
+
+class Bare:
+    """Calls of the C ABI on a cache without a workspace: the library's own is taken."""
+
+    def __init__(self, kv4, cache):
+        self.cache, self.lib = cache, hb.load()
+        self.desc = kv4.Kv4Desc.from_buffer_copy(cache.desc)
+        self.desc.work = None
+        self.at = C.addressof(self.desc)
+
+    def _stream(self):
+        self.desc.stream = torch.cuda.current_stream().cuda_stream or 1   # 1: cudaStreamLegacy
+
+    def attention(self, layer, q, out):
+        self._stream()
+        return self.lib.cuda_kv4_attention(self.at, layer, out.data_ptr(), q.data_ptr(), hb.DT_F32, 0, 0, q.shape[1], 0.0,
+                                           None, q.shape[0])
+
+    def extend(self, counts, start):
+        self._stream()
+        return self.lib.cuda_kv4_extend(self.at, None, counts.data_ptr(), start.data_ptr(), counts.numel())
+
+
+def queries(n, heads, hd, seed):
+    return torch.randn(n, heads, hd, generator=torch.Generator().manual_seed(seed)).cuda()
+
+
+def test_caches_of_different_shapes_share_the_librarys_workspace(kv4):
+    """Caches of 672 counters and of a few, call after call on one stream: an extend and a split attention of small ones between the
+    split attentions of the large one.  Each result is the one with a workspace of the cache's own."""
+    big, _ = filled(kv4, [700 + 11 * i for i in range(40)], 8, 64, 16, 1, spare=0)
+    small, _ = filled(kv4, [9000, 20], 1, 64, 16, 2)
+    qb, qs = queries(40, 8, 64, 3), queries(2, 4, 64, 4)
+    want_big, want_small = big.attention(0, qb), small.attention(0, qs)
+    big_bare, small_bare = Bare(kv4, big), Bare(kv4, small)
+    for rc in (small_bare.attention(0, qs, torch.empty_like(qs)), big_bare.attention(0, qb, torch.empty_like(qb))):
+        assert rc == hb.HOLO_OK   # whatever the buffer has to grow by is there
+    grown = kv4.Kv4Cache(1, 1, 64, 16, n_pages=1200, max_seqs=2, max_pages=1200)   # its extend lists 1000 pages in the plan
+    grown_bare, counts, start = Bare(kv4, grown), ints(16000, 0), ints(0, 0)
+    for i in range(3):
+        out_s, out_b = torch.full_like(qs, 7.0), torch.full_like(qb, 7.0)
+        assert small_bare.attention(0, qs, out_s) == hb.HOLO_OK
+        assert grown_bare.extend(counts, start) == hb.HOLO_OK
+        assert big_bare.attention(0, qb, out_b) == hb.HOLO_OK
+        grown.release(ints(0))
+        big.check()
+        assert torch.equal(out_s, want_small), i
+        assert torch.equal(out_b, want_big), i
