@@ -139,6 +139,7 @@ struct Walk {
     int i, s, len, units;      // sequence: its place in the list, number, positions, units an item
     int item;                  // KV head * chunks + chunk
     int start;                 // of the item in the list
+    uint32_t number;           // counts the items in which the warp has units
     int first, take;           // its units in the part
 };
 
@@ -157,8 +158,8 @@ __device__ __forceinline__ void at_clip(const AtArgs &a, Walk &w, int from, int 
     w.first = max(0, from - w.start - a.item_cost);
     w.take = max(0, min(w.units, to - w.start - a.item_cost) - w.first);
 }
-// the next item of the part [from, to) that has units in it; false: none
-__device__ __forceinline__ bool at_next(const Kv4View &c, const AtArgs &a, Walk &w, int from, int to) {
+// the next item of the part [from, to) that has units in it; false: none.  unit0: the warp's first one of an item's
+__device__ __forceinline__ bool at_next(const Kv4View &c, const AtArgs &a, Walk &w, int from, int to, int unit0) {
     do {
         w.start += w.units + a.item_cost;
         w.first = w.take = 0;
@@ -172,6 +173,7 @@ __device__ __forceinline__ bool at_next(const Kv4View &c, const AtArgs &a, Walk 
         }
         at_clip(a, w, from, to);
     } while (w.take == 0);
+    w.number += w.take > unit0;
     return true;
 }
 
@@ -245,11 +247,16 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
     __shared__ float join_m[AT_WARPS][KV4_HEADS], join_l[AT_WARPS][KV4_HEADS], join_w[AT_WARPS][KV4_HEADS];
     __shared__ float join_den[KV4_HEADS];
     __shared__ int last;
+    // Items (a bit each, by their number: no more than the ring's slots are under way) of which the warp met a table entry that
+    // names no page.  Such an item comes out as zeros: its share's sum of weights is given as -1, which no sum of
+    // exponentials is, up to the last join.
+    __shared__ uint32_t bad_items[AT_WARPS];
     float *join = reinterpret_cast<float *>(at_smem + G::RING);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     uint8_t *ring = at_smem + (size_t)warp * STAGES * AT_UNIT * G::BLOCK_BYTES;
 
     if (lane < STAGES) mbar_init(&full[warp][lane], 1);
+    if (lane == 0) bad_items[warp] = 0;
     fence_barrier_init();
     early_wait();
     early_next();
@@ -316,6 +323,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
                 w.i = i0 + threadIdx.x, w.s = s0, w.len = len0, w.units = u0;
                 w.item = (cut0 - start) / item_places;
                 w.start = start + w.item * item_places;
+                w.number = 0;
                 begin = w;
                 part_start = u0 > AT_WHOLE ? cut0 : w.start;
             }
@@ -339,7 +347,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
     bool any = from < to;
     if (any) {
         at_clip(a, head, from, to);
-        if (head.take == 0) any = at_next(c, a, head, from, to);
+        if (head.take == 0) any = at_next(c, a, head, from, to, unit0);
     }
     if (!any) {
         zeros();
@@ -373,7 +381,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
         Walk x = load;
         bool more = true;
         while (more && unit >= x.first + x.take) {
-            more = at_next(c, a, x, from, to);
+            more = at_next(c, a, x, from, to, unit0);
             unit = x.first + unit0;
         }
         __syncwarp();
@@ -403,8 +411,9 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
         if (lane == 0) mbar_arrive_expect_tx(&full[warp][fill], blocks * G::BLOCK_BYTES);
         __syncwarp();
         if (lane < blocks) {
-            if ((uint32_t)entry >= (uint32_t)c.n_pages) {
+            if ((uint32_t)entry >= (uint32_t)c.n_pages) {   // any page, so that the ring goes on: the item's result is dropped
                 kv4_report(c.status, HOLO_E_ARG);
+                atomicOr(&bad_items[warp], 1u << (load.number & 31));
                 entry = 0;
             }
             asm volatile(
@@ -665,7 +674,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
         more = true;
         if (after.take == 0 || after.start != w.start + w.units + a.item_cost) {
             after = w;
-            more = at_next(c, a, after, from, to);
+            more = at_next(c, a, after, from, to, unit0);
         }
         if (EARLY && more) load_q(after);
         T *out = (T *)a.out + w.i * a.out_row + (long long)head0 * HD;
@@ -675,6 +684,19 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
         for (int x = 0; x < 2; ++x)
 #pragma unroll
             for (int i = 4; i < 32; i <<= 1) l[x] += __shfl_xor_sync(0xffffffffu, l[x], i);
+        if (bad_items[warp] >> (w.number & 31) & 1) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[b][x][e] = 0.0f;
+            m[0] = m[1] = 0.0f;
+            l[0] = l[1] = solo ? 1.0f : -1.0f;
+            __syncwarp();
+            if (lane == 0) bad_items[warp] &= ~(1u << (w.number & 31));
+            __syncwarp();
+        }
         // l and o hold 2^(AT_SHIFT - power) too; o's codes 1 / UNIT, odd ones 16 times as large
         if (solo) {
 #pragma unroll
@@ -707,15 +729,19 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
         if (threadIdx.x < KV4_HEADS) {
             const int h = threadIdx.x;
             float top = -INFINITY, den = 0.0f;
+            bool bad = false;
 #pragma unroll
-            for (int i = 0; i < AT_WARPS; ++i)
+            for (int i = 0; i < AT_WARPS; ++i) {
                 if (join_l[i][h] != 0.0f) top = fmaxf(top, join_m[i][h]);
+                bad |= join_l[i][h] < 0.0f;
+            }
 #pragma unroll
             for (int i = 0; i < AT_WARPS; ++i) {
                 const float f = join_l[i][h] != 0.0f ? at_ex2(join_m[i][h] - top) : 0.0f;
                 join_w[i][h] = f;
                 den = fmaf(join_l[i][h], f, den);
             }
+            if (bad) den = -1.0f;
             join_den[h] = den;
             if (!whole) mine[2 * h] = top, mine[2 * h + 1] = den;
         }
@@ -731,7 +757,8 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
             }
             if (whole) {
                 const float den = join_den[h];
-                at_store4<T>(out + d, a.wide, sum.x / den, sum.y / den, sum.z / den, sum.w / den);
+                if (den < 0.0f) at_store4<T>(out + d, a.wide, 0.0f, 0.0f, 0.0f, 0.0f);
+                else at_store4<T>(out + d, a.wide, sum.x / den, sum.y / den, sum.z / den, sum.w / den);
             } else {
                 *reinterpret_cast<float4 *>(mine + 2 * KV4_HEADS + d) = sum;
             }
@@ -758,6 +785,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
                 for (int d = 4 * threadIdx.x; d < heads * HD; d += 4 * AT_THREADS) {
                     const int h = d / HD;
                     float top = -INFINITY, den = 0.0f;
+                    bool bad = false;
                     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     for (int k0 = 0; k0 < parts; k0 += BATCH) {
                         float2 ml[BATCH];
@@ -775,8 +803,10 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
                         }
                         float to = top;
 #pragma unroll
-                        for (int i = 0; i < BATCH; ++i)
+                        for (int i = 0; i < BATCH; ++i) {
                             if (ml[i].y != 0.0f) to = fmaxf(to, ml[i].x);
+                            bad |= ml[i].y < 0.0f;
+                        }
                         const float fix = den != 0.0f ? at_ex2(top - to) : 0.0f;
                         top = to;
                         den *= fix;
@@ -791,7 +821,8 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
                             }
                         }
                     }
-                    at_store4<T>(out + d, a.wide, sum.x / den, sum.y / den, sum.z / den, sum.w / den);
+                    if (bad) at_store4<T>(out + d, a.wide, 0.0f, 0.0f, 0.0f, 0.0f);
+                    else at_store4<T>(out + d, a.wide, sum.x / den, sum.y / den, sum.z / den, sum.w / den);
                 }
             }
         }

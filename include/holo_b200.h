@@ -408,7 +408,8 @@ int cuda_kv4_read(const holo_kv4 *c, int layer, void *k, void *v, int type, long
                   int rows, const int *cu_rows, const int *start, const int *seqs, int n);
 /* One query a sequence over all the positions that it holds:
  *   out[i][h] = sum_j softmax_j(scale * q[i][h] . k[j][h / group]) * v[j][h / group],
- * j < lens[seqs[i]]; zeros for an empty sequence.  q and out [n][n_heads]
+ * j < lens[seqs[i]]; zeros for an empty sequence, and for one whose table lacks
+ * a page of it (which is recorded).  q and out [n][n_heads]
  * [head_dim] of `type` (fp32, fp16 or bf16), *_row elements from row to row
  * (0: dense), n_heads / n_kv_heads <= 16; scale 0: 1 / sqrt(head_dim); n *
  * max_pages * page_tokens * n_kv_heads up to 2^34.  fp32

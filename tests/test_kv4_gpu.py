@@ -541,3 +541,47 @@ def test_attention_of_many_short_sequences(kv4, dtype, hd):
             assert np.abs(got[i, h].double().cpu().numpy() - want[0]).max() <= tol, (i, h)
     cache.check()
     assert torch.equal(got.flatten(1).any(1).cpu(), torch.tensor(lens > 0))
+
+
+# ---- entries of a table that name no page ----
+
+@pytest.mark.parametrize("entry", [-1, 10 ** 6, -2 ** 31])
+@pytest.mark.parametrize("lens,heads,n_kv,hd,dtype", [
+    ([40, 64, 3, 0], 4, 2, 64, "f32"),               # an item each
+    ([30] * 500, 4, 2, 64, "f16"),                   # a warp takes several items
+    ([900, 5000, 200, 7], 16, 1, 128, "bf16"),       # split over CTAs
+    ([300, 1200, 40], 3, 3, 256, "f32")])
+def test_attention_over_an_entry_that_names_no_page(kv4, lens, heads, n_kv, hd, dtype, entry):
+    """The sequence is left out: zeros, and not the values of another page.  The others are as they were, and so is the next call."""
+    cache, _ = filled(kv4, lens, n_kv, hd, 32, 71)
+    q = torch.randn(len(lens), heads, hd, generator=torch.Generator().manual_seed(72)).to(DTYPES[dtype]).cuda()
+    want = cache.attention(0, q).clone()
+    held = cache.tables[1].clone()
+    for col in {0, (lens[1] - 1) // 32}:
+        cache.tables[1, col] = entry
+        out = cache.attention(0, q, torch.full_like(q, 7.0))
+        with pytest.raises(RuntimeError, match=str(hb.HOLO_E_ARG)):
+            cache.check()
+        assert not out[1].any()
+        rest = torch.arange(len(lens)) != 1
+        assert torch.equal(out[rest], want[rest])
+        cache.tables[1] = held
+    cache.tables[1, -1] = entry                      # past the sequence's pages: nobody's concern
+    assert torch.equal(cache.attention(0, q), want)
+    cache.check()
+
+
+def test_attention_over_missing_pages_among_short_and_long_sequences(kv4):
+    """Runs of one-unit items, of which only one warp has anything, before long ones whose first loads are under way meanwhile:
+    every second long sequence lacks its last page, and no other one comes out otherwise for it."""
+    lens = ([20] * 40 + [450]) * 16
+    cache, _ = filled(kv4, lens, 2, 64, 32, 73)
+    q = torch.randn(len(lens), 4, 64, generator=torch.Generator().manual_seed(74)).cuda()
+    want = cache.attention(0, q).clone()
+    gone = torch.arange(40, len(lens), 82)
+    cache.tables[gone.cuda(), 449 // 32] = -1
+    out = cache.attention(0, q)
+    with pytest.raises(RuntimeError, match=str(hb.HOLO_E_ARG)):
+        cache.check()
+    want[gone.cuda()] = 0
+    assert torch.equal(out, want)
