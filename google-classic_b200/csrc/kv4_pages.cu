@@ -184,7 +184,7 @@ copy_kernel(const __grid_constant__ Kv4View c, size_t page_bytes, size_t layer_b
 }
 
 // ---- fork ------------------------------------------------------------------------
-// the children's rows, the pages' counts and the copies
+// the children's rows, the pages' counts and the copies; the plan has looked at the parents' entries
 __device__ __forceinline__ void fork_apply(const Kv4View &c, size_t page_bytes, size_t layer_bytes, int layers,
                                            const int *parents, const int *children, int n, const int *page, const Team &t) {
     const long long total = (long long)n * layers;
@@ -200,8 +200,7 @@ __device__ __forceinline__ void fork_apply(const Kv4View &c, size_t page_bytes, 
                 int e = -1;
                 if (j < full) {
                     e = from[j];
-                    if (e >= 0 && e < c.n_pages) atomicAdd(c.refs + e, 1);
-                    else kv4_report(c.status, HOLO_E_ARG);
+                    atomicAdd(c.refs + e, 1);
                 } else if (j == full) {
                     e = fresh;   // -1: the parent ends with a full page
                     if (e >= 0) c.refs[e] = 1;
@@ -210,11 +209,7 @@ __device__ __forceinline__ void fork_apply(const Kv4View &c, size_t page_bytes, 
             }
             if (t.thread == 0) c.lens[k] = len;
         }
-        if (fresh >= 0) {
-            const int s = from[full];
-            if (s >= 0 && s < c.n_pages) copy_page(t, c.pool + layer * layer_bytes, page_bytes, s, fresh);
-            else if (t.thread == 0) kv4_report(c.status, HOLO_E_ARG);
-        }
+        if (fresh >= 0) copy_page(t, c.pool + layer * layer_bytes, page_bytes, from[full], fresh);
     }
 }
 
@@ -227,21 +222,26 @@ fork_plan_kernel(const __grid_constant__ Kv4View c, size_t page_bytes, size_t la
     early_wait();
     early_next();
     __shared__ int sh[32];
+    // which children there can be: a warp each looks at the parent's pages
+    for (int i = threadIdx.x / 32; i < n; i += PLAN_THREADS / 32) {
+        const int p = parents[i], k = children[i];
+        bool good = p >= 0 && p < c.max_seqs && k >= 0 && k < c.max_seqs && p != k && c.lens[k] == 0;
+        if (good) {
+            const int *from = c.tables + (size_t)p * c.max_pages;
+            const int held = min(pages_of(c, c.lens[p]), c.max_pages);
+            for (int j = threadIdx.x % 32; j < held; j += 32) good &= (unsigned)from[j] < (unsigned)c.n_pages;
+        }
+        good = __all_sync(0xffffffffu, good);
+        if (threadIdx.x % 32 == 0) {
+            page[i] = good ? -1 : -2;
+            if (!good) kv4_report(c.status, HOLO_E_ARG);
+        }
+    }
+    __syncthreads();
     int need_all = 0;
     for (int i0 = 0; i0 < n; i0 += PLAN_THREADS) {
         const int i = i0 + threadIdx.x;
-        int need = 0;
-        if (i < n) {
-            const int p = parents[i], k = children[i];
-            int got = -2;
-            if (p >= 0 && p < c.max_seqs && k >= 0 && k < c.max_seqs && p != k && c.lens[k] == 0) {
-                need = c.lens[p] % c.page_tokens != 0;
-                got = -1;
-            } else {
-                kv4_report(c.status, HOLO_E_ARG);
-            }
-            page[i] = got;
-        }
+        const int need = i < n && page[i] == -1 ? c.lens[parents[i]] % c.page_tokens != 0 : 0;
         int total;
         block_inclusive(need, sh, total);
         need_all += total;

@@ -418,7 +418,8 @@ int cuda_kv4_attention(const holo_kv4 *c, int layer, void *out, const void *q, i
                        long long out_row, int n_heads, float scale, const int *seqs, int n);
 /* children[i] (an empty sequence) becomes a copy of parents[i]: the full pages are
  * shared, a last page with room left is copied, in every layer, to the lowest
- * free page.  Parents may repeat; no parent is a child of the same call. */
+ * free page.  Parents may repeat; no parent is a child of the same call.  A child
+ * whose parent's table lacks a page stays empty (which is recorded). */
 int cuda_kv4_fork(const holo_kv4 *c, const int *parents, const int *children, int n);
 /* Empties sequences; pages that no other one holds become free. */
 int cuda_kv4_release(const holo_kv4 *c, const int *seqs, int n);

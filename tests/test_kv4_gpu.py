@@ -585,3 +585,50 @@ def test_attention_over_missing_pages_among_short_and_long_sequences(kv4):
         cache.check()
     want[gone.cuda()] = 0
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("layers", [2, 600])   # one launch; a plan and a grid
+@pytest.mark.parametrize("entry", [-1, 10 ** 6])
+def test_fork_of_a_parent_that_lacks_a_page(kv4, layers, entry):
+    """Its child stays empty and no page is taken for it; the other children are forked."""
+    cache, _ = filled(kv4, [100, 70, 33, 0, 0, 0], 1, 64, 32, 81, layers=1)
+    cache = kv4.Kv4Cache(layers, 1, 64, 32, pool=cache.pool.expand(layers, -1, -1, -1, -1).contiguous(), tables=cache.tables,
+                         lens=cache.lens, refs=cache.refs)
+    for col in (0, 2):                            # a whole page of the second parent, its last one
+        held = cache.tables[1].clone()
+        cache.tables[1, col] = entry
+        model = Model(cache)
+        cache.fork(ints(0, 1, 2), ints(3, 4, 5))
+        with pytest.raises(RuntimeError, match=str(hb.HOLO_E_ARG)):
+            cache.check()
+        model.fork([0, 2], [3, 5])
+        model.same(cache)
+        cache.tables[1] = held
+        cache.release(ints(3, 4, 5))
+
+
+def test_extend_and_fork_of_more_sequences_than_a_step_of_the_plan(kv4):
+    """2500 sequences: the sums over the list go on from step to step, up to the last free page."""
+    rng = np.random.default_rng(7)
+    counts = rng.integers(0, 70, 2500)
+    need = int((-(-counts // 16)).sum())
+    cache = kv4.Kv4Cache(1, 1, 64, 16, need + 900, 5000, 6)
+    cache.pool.random_(0, 256)
+    model = Model(cache)
+    seqs = rng.permutation(5000)[:2500]
+    start = cache.extend(ints(*counts), ints(*seqs))
+    assert start.tolist() == model.extend(counts, seqs)
+    model.same(cache)
+    empty = np.flatnonzero(model.lens == 0)
+    parents = rng.choice(np.flatnonzero(model.lens), 2400)   # (no parent is a child)
+    cache.fork(ints(*parents), ints(*empty[:2400]))
+    model.fork(parents, empty[:2400])
+    with pytest.raises(RuntimeError, match=str(hb.HOLO_E_NOMEM)):   # more last pages than are free
+        cache.check()
+    model.same(cache)
+    more = rng.integers(0, 30, 3000)
+    cache.release(ints(*range(0, 2000)))
+    model.release(range(0, 2000))
+    assert cache.extend(ints(*more), ints(*range(1000, 4000))).tolist() == model.extend(more, range(1000, 4000))
+    cache.lib.cuda_clear_status()
+    model.same(cache)
