@@ -74,6 +74,10 @@ __device__ int find_free(const Kv4View &c, int want, int *list, int *sh) {
 }
 
 __device__ __forceinline__ int pages_of(const Kv4View &c, int len) { return len / c.page_tokens + (len % c.page_tokens != 0); }
+// whether a length is one that a row of the tables can hold: no other is followed into them
+__device__ __forceinline__ bool len_ok(const Kv4View &c, int len) {
+    return len >= 0 && len <= (long long)c.max_pages * c.page_tokens;
+}
 
 // ---- extend -----------------------------------------------------------------
 // A sequence's need is at most n_pages + 1 (<= 2^20 + 1) in the sums, and the
@@ -95,7 +99,7 @@ extend_kernel(const __grid_constant__ Kv4View c, const int *seqs, const int *cou
             const int s = seqs ? seqs[i] : i, add = counts[i];
             if (s >= 0 && s < c.max_seqs && add > 0) {
                 const long long len = c.lens[s], after = len + add;
-                if (after <= (long long)c.max_pages * c.page_tokens)
+                if (len >= 0 && after <= (long long)c.max_pages * c.page_tokens)
                     need = min(pages_of(c, (int)after) - pages_of(c, (int)len), c.n_pages + 1);
             }
         }
@@ -115,7 +119,8 @@ extend_kernel(const __grid_constant__ Kv4View c, const int *seqs, const int *cou
                 err = HOLO_E_ARG;
             } else {
                 len = c.lens[s];
-                if ((long long)len + add > (long long)c.max_pages * c.page_tokens) err = HOLO_E_NOMEM;
+                if (!len_ok(c, len)) err = HOLO_E_ARG;
+                else if ((long long)len + add > (long long)c.max_pages * c.page_tokens) err = HOLO_E_NOMEM;
                 else need = min(pages_of(c, len + add) - pages_of(c, len), c.n_pages + 1);
             }
         }
@@ -225,10 +230,10 @@ fork_plan_kernel(const __grid_constant__ Kv4View c, size_t page_bytes, size_t la
     // which children there can be: a warp each looks at the parent's pages
     for (int i = threadIdx.x / 32; i < n; i += PLAN_THREADS / 32) {
         const int p = parents[i], k = children[i];
-        bool good = p >= 0 && p < c.max_seqs && k >= 0 && k < c.max_seqs && p != k && c.lens[k] == 0;
+        bool good = p >= 0 && p < c.max_seqs && k >= 0 && k < c.max_seqs && p != k && c.lens[k] == 0 && len_ok(c, c.lens[p]);
         if (good) {
             const int *from = c.tables + (size_t)p * c.max_pages;
-            const int held = min(pages_of(c, c.lens[p]), c.max_pages);
+            const int held = pages_of(c, c.lens[p]);
             for (int j = threadIdx.x % 32; j < held; j += 32) good &= (unsigned)from[j] < (unsigned)c.n_pages;
         }
         good = __all_sync(0xffffffffu, good);
@@ -290,8 +295,15 @@ release_kernel(const __grid_constant__ Kv4View c, const int *seqs, int n) {
             continue;
         }
         __syncthreads();
-        if (threadIdx.x == 0) len_s = atomicExch(c.lens + s, 0);
+        if (threadIdx.x == 0) {
+            len_s = atomicExch(c.lens + s, 0);
+            if (!len_ok(c, len_s)) {          // left as it was
+                c.lens[s] = len_s;
+                kv4_report(c.status, HOLO_E_ARG);
+            }
+        }
         __syncthreads();
+        if (!len_ok(c, len_s)) continue;
         const int held = pages_of(c, len_s);
         int *row = c.tables + (size_t)s * c.max_pages;
         for (int j = threadIdx.x; j < c.max_pages; j += COPY_THREADS) {

@@ -632,3 +632,32 @@ def test_extend_and_fork_of_more_sequences_than_a_step_of_the_plan(kv4):
     assert cache.extend(ints(*more), ints(*range(1000, 4000))).tolist() == model.extend(more, range(1000, 4000))
     cache.lib.cuda_clear_status()
     model.same(cache)
+
+
+@pytest.mark.parametrize("length", [-1, -2 ** 31, 3 * 16 + 1, 2 ** 31 - 1])
+def test_lengths_that_the_tables_cannot_hold(kv4, length):
+    """A length that is negative or past the table's columns is recorded and followed nowhere: the sequence is left as it is, and the
+    others in the call are served."""
+    cache = kv4.Kv4Cache(2, 1, 64, 16, 40, 6, 3)
+    cache.extend(ints(20, 20, 20))
+    cache.check()
+    cache.lens[1] = length
+    before = [x.clone() for x in (cache.tables, cache.refs, cache.lens, cache.pool)]
+    start = cache.extend(ints(1, 1), ints(1, 2))
+    with pytest.raises(RuntimeError, match=str(hb.HOLO_E_ARG)):
+        cache.check()
+    assert start.tolist() == [-1, 20]
+    before[2][2] = 21
+    model = Model(cache)
+    cache.fork(ints(1, 0), ints(3, 4))
+    with pytest.raises(RuntimeError, match=str(hb.HOLO_E_ARG)):
+        cache.check()
+    model.fork([0], [4])
+    model.same(cache)
+    cache.release(ints(1, 4))
+    with pytest.raises(RuntimeError, match=str(hb.HOLO_E_ARG)):
+        cache.check()
+    model.release([4])
+    model.same(cache)
+    for x, y in zip((cache.tables, cache.refs, cache.lens), before):
+        assert torch.equal(x, y)
