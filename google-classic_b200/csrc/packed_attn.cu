@@ -39,9 +39,14 @@
 // A masked place never counts.  Its P is an exact 0, which an infinite or NaN
 // value of V would still make NaN: where a row's result is not finite, the CTA
 // goes through its items a second time with care.  Then warp 11 sets the values
-// that are not finite in a diagonal tile of V, the only ones with masked places,
-// to 0 before the tensor core reads the tile, and the rows that do see such a
-// value, and any whose result is not finite still, are taken alone over their own keys.
+// of V that are not finite to 0 before the tensor core reads a tile, and keeps, for each
+// dim, the first key with a NaN, an infinity and a negative one; the rows from that key
+// on have that as their result (a weight is never 0 in the formula).
+// A NaN score needs none of this: it makes its row NaN by itself.  Where the
+// cleaned sums still overflow fp32 (bf16 values near the largest, times weights before the
+// division), a third pass takes V by 2^-32 and the sums by 2^32.
+// A sequence of 4096 (2 heads over 1 of 128, f16): 60 to 67 us, 270 with two such values, 1,700 with all of V
+// NaN; of 16,383 (64 heads over 8, bf16): 3.5, 15.7 and 101 ms.
 #include "holo_common.cuh"
 #include "mv_unit.cuh"
 #include "tc_util.cuh"
@@ -50,6 +55,7 @@
 #include <cuda_bf16.h>
 
 #include <mutex>
+#include <type_traits>
 
 namespace {
 
@@ -141,11 +147,13 @@ void launch_simple(const PackedArgs &a, int hd, cudaStream_t st) {
 constexpr int PK_ROWS = 128;           // query rows a tile (MMA M)
 constexpr int PK_STEP = 64;            // keys a step (MMA N of S, K of P V)
 constexpr int PK_THREADS = 384;        // three warpgroups
-// registers a thread, of 384 * 168 at launch: 2 * 208 + 80 <= 3 * 168
-constexpr int PK_SOFTMAX_REGS = 208, PK_OTHER_REGS = 80;
+// registers a thread, of 384 * 168 at launch: 2 * 208 + 88 = 3 * 168
+constexpr int PK_SOFTMAX_REGS = 208, PK_OTHER_REGS = 88;
+static_assert(2 * PK_SOFTMAX_REGS + PK_OTHER_REGS <= 3 * 168, "a split above the launch's registers would wait for ever");
 constexpr uint32_t PK_TMEM_COLS = 512; // two S_0, two S_1 (64 columns each), O_0, O_1 (128; O_0 256): all, so they begin at 0
 constexpr float PK_GROWTH = 8.0f;      // log2 of what a row's maximum may grow by before its O is rescaled
 constexpr int PK_STAGES = 5;           // ring of K and V tiles
+constexpr float PK_DOWN = 1.0f / 4294967296.0f;   // 2^-32: of V in the third pass
 
 template <int HD> struct PkGeom {
     static constexpr int TILES = HD == 256 ? 1 : 2;   // query tiles an item: a second O of 256 columns has no room
@@ -170,15 +178,14 @@ template <int STEPS> __device__ __forceinline__ bool pk_is_value(int i, int n, i
 
 struct PkWork {
     int first, len, row0, head;        // the sequence's first row and length; the item's first row in it; len 0: no more
-    int careful;
+    int careful;                       // 1: V is cleaned; 2: and scaled down
 };
 
 struct PkBars {
     uint64_t work_full[2], work_empty[2], q_full[2], q_empty[2], s_full[2][2], p_full[2][2], o_done[2][2];
     uint64_t kv_full[PK_STAGES], kv_empty[PK_STAGES], kv_checked[PK_STAGES], bad_known[2], drain[2];
     PkWork work[2];
-    int bad_from[2];                   // of an item: first key of the diagonal tiles with a value that is not finite
-    int again;                         // a row's result was not finite
+    int again;                         // the `careful` that a row's result asks for
     uint32_t tmem;
 };
 
@@ -249,28 +256,74 @@ __device__ __forceinline__ uint64_t pk_add2(uint64_t a, uint64_t b) {
     return r;
 }
 
-// Row `row` of head h over its own keys first .. row, by one thread: for rows
-// whose tiles hold values that are not finite.
-template <typename T, int HD>
-__device__ __noinline__ void pk_row_alone(const PackedArgs &a, int row, int first, int h) {
-    const T *q = (const T *)a.q + row * a.q_row + h * a.q_head;
-    float acc[HD], m = -INFINITY, l = 0.0f;
-    for (int d = 0; d < HD; ++d) acc[d] = 0.0f;
-    for (int j = first; j <= row; ++j) {
-        const T *k = (const T *)a.k + j * a.k_row + h / a.group * a.k_head;
-        const T *v = (const T *)a.v + j * a.v_row + h / a.group * a.v_head;
-        float dot = 0.0f;
-        for (int d = 0; d < HD; ++d) dot = fmaf(to_float(q[d]), to_float(k[d]), dot);
-        dot *= a.scale;
-        if (dot == -INFINITY) continue;   // weight 0
-        const float mn = fmaxf(m, dot), fix = expf(m - mn), e = expf(dot - mn);
-        l = l * fix + e;
-        m = mn;
-        for (int d = 0; d < HD; ++d) acc[d] = fmaf(e, to_float(v[d]), acc[d] * fix);
+// *p = min(*p, v), in shared memory
+__device__ __forceinline__ void pk_min16(unsigned short *p, unsigned short v) {
+    for (unsigned short old = *(volatile unsigned short *)p; v < old;) {
+        const unsigned short got = atomicCAS(p, old, v);
+        if (got == old) break;
+        old = got;
     }
-    T *o = (T *)a.out + row * a.out_row + h * a.out_head;
-    for (int d = 0; d < HD; ++d) from_float(acc[d] / l, o[d]);
-    if (a.lse) a.lse[(size_t)h * a.total + row] = m + logf(l);
+}
+
+// What is not finite in a row: kinds of values, and row (of the item) from which
+// on the item's rows see one; PK_NEVER: none do
+enum { PK_NAN, PK_INF, PK_MINUS_INF, PK_KINDS };
+constexpr unsigned short PK_NEVER = 0xffff;
+
+// A tile of V in shared memory, its keys from `key0` (of the item's rows) on, as TMA
+// has laid it: boxes of 64 dims, rows of 128 bytes, whose 16-byte pieces are exchanged by
+// the row's last three bits.  Its values that are not finite become 0 and are
+// noted in `seen`; one warp.  scale (bf16): all values by 2^-32.
+template <typename T, int HD, int KEYS>
+__device__ __forceinline__ void pk_clean_tile(uint8_t *tile, int key0, int len, bool scale,
+                                              unsigned short (*seen)[HD]) {
+    constexpr uint32_t X = PkType<T>::EXPONENT;
+    const int lane = threadIdx.x & 31, piece = lane & 7;
+#pragma unroll 1
+    for (int box = 0; box < HD / 64; ++box) {
+        uint4 *rows = reinterpret_cast<uint4 *>(tile + box * KEYS * 128);
+#pragma unroll 4
+        for (int r = lane >> 3; r < KEYS; r += 4) {
+            uint4 *at = rows + r * 8 + (piece ^ (r & 7));
+            const uint4 v = *at;
+            uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            const uint32_t b[4] = {__vcmpeq2(v.x & X, X), __vcmpeq2(v.y & X, X), __vcmpeq2(v.z & X, X), __vcmpeq2(v.w & X, X)};
+            const bool any = (b[0] | b[1] | b[2] | b[3]) != 0;
+            if (any && key0 + r < len) {
+                for (int d = 0; d < 8; ++d) {
+                    const uint32_t pair = d < 4 ? (d < 2 ? w[0] : w[1]) : (d < 6 ? w[2] : w[3]);
+                    const uint32_t x = d & 1 ? pair >> 16 : pair & 0xffffu;
+                    if ((x & X & 0xffffu) != (X & 0xffffu)) continue;
+                    const int kind = x & ~X & 0x7fffu ? PK_NAN : x & 0x8000u ? PK_MINUS_INF : PK_INF;
+                    pk_min16(&seen[kind][box * 64 + piece * 8 + d], (unsigned short)max(0, key0 + r));
+                }
+            }
+            if (any || scale) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    w[i] &= ~b[i];
+                    if (std::is_same<T, __nv_bfloat16>::value && scale) {
+                        const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162 *>(&w[i]),
+                                                         __float2bfloat162_rn(PK_DOWN));
+                        w[i] = *reinterpret_cast<const uint32_t *>(&y);
+                    }
+                }
+                *at = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+    }
+}
+
+// what row r of an item sees that is not finite becomes its result
+template <typename T, int HD>
+__device__ __noinline__ void pk_mark_row(T *row, int r, const unsigned short (*seen)[HD]) {
+    for (int d = 0; d < HD; ++d) {
+        float x = 0.0f;
+        if (r >= seen[PK_NAN][d]) x += NAN;
+        if (r >= seen[PK_INF][d]) x += INFINITY;
+        if (r >= seen[PK_MINUS_INF][d]) x -= INFINITY;
+        if (x != 0.0f) from_float(x, row[d]);
+    }
 }
 
 // Item r of all, heads apart, longest first: the tiles of item_rows rows of all
@@ -348,6 +401,8 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
     using G = PkGeom<HD>;
     extern __shared__ uint8_t pk_smem_raw[];
     __shared__ PkBars B;
+    __shared__ unsigned short seen[PK_KINDS][HD];   // of an item with care
+    static_assert(sizeof(PkBars) + sizeof(seen) + G::SMEM <= 227 * 1024, "shared memory");
     uint8_t *sq = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(pk_smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t *skv = sq + G::TILES * G::Q_TILE;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -513,7 +568,7 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
                     if (h == 0) {
                         v_slot = slot;
                         if (!wait_all(&B.kv_full[v_slot], phase)) break;
-                        if (w.careful && x / 2 >= n0 - 1 && !wait_all(&B.kv_checked[v_slot], phase)) break;
+                        if (w.careful && !wait_all(&B.kv_checked[v_slot], phase)) break;
                         advance();
                     }
                     if (!wait_all(&B.p_full[t][it & 1], it >> 1)) break;
@@ -561,7 +616,8 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
 #pragma unroll
             for (int i = 1; i < PK_KEPT; ++i) kept[i] = pk_len(a, 32 * i + lane);
             int published = 0, base = 0;           // items so far, and of them before this pass
-            bool more = true, careful = false;
+            bool more = true;
+            int careful = 0;
             auto publish = [&](PkWork &mine) {
                 if (published >= 2) wait(&B.work_empty[published & 1], (published >> 1) + 1);
                 ok = __all_sync(0xffffffffu, ok);
@@ -569,7 +625,6 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
                 mine.careful = careful;
                 if (lane == 0) {
                     B.work[published & 1] = mine;
-                    B.bad_from[published & 1] = 0x7fffffff;
                     mbar_arrive(&B.work_full[published & 1]);
                 }
                 __syncwarp();
@@ -590,12 +645,14 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
             int slot = 0, phase = 0;
             for (int k = 0; ok; ++k) {
                 if (k == published) {
-                    // The end of a pass.  Once the last item is through: is one with care wanted?
-                    if (k > 0 && !careful) {
+                    // The end of a pass.  Once the last item is through: is one with more care wanted?
+                    if (k > 0 && careful < 2) {
                         wait(&B.work_empty[(k - 1) & 1], (k - 1) >> 1);
                         ok = __all_sync(0xffffffffu, ok);
-                        if (ok && *(volatile int *)&B.again) {
-                            careful = more = true;
+                        const int again = *(volatile int *)&B.again;
+                        if (ok && again > careful) {
+                            careful = again;
+                            more = true;
                             base = published;
                             find();
                             find();
@@ -608,26 +665,21 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
                     }
                 }
                 if (!next(k)) break;
+                if (w.careful) {                // the rows of the item before have been written
+                    wait(&B.work_empty[(k - 1) & 1], (k - 1) >> 1);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    for (int i = lane; i < PK_KINDS * HD; i += 32) (&seen[0][0])[i] = PK_NEVER;
+                    __syncwarp();
+                }
                 for (int i = 0; i < 2 * n; ++i) {   // every tile of the ring, so that no phase is missed
                     wait(&B.kv_full[slot], phase);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     int j;
-                    if (pk_is_value<G::STEPS>(i, n, j) && careful && j * G::KEYS >= w.row0) {
-                        // a diagonal tile of V: no value that is not finite in a masked place
-                        uint4 *tile = reinterpret_cast<uint4 *>(skv + slot * G::KV_TILE);
-                        constexpr uint32_t X = PkType<T>::EXPONENT;
-#pragma unroll 4
-                        for (int e = lane; e < G::KV_TILE / 16; e += 32) {
-                            const uint4 v = tile[e];
-                            const uint32_t b[4] = {__vcmpeq2(v.x & X, X), __vcmpeq2(v.y & X, X), __vcmpeq2(v.z & X, X),
-                                                   __vcmpeq2(v.w & X, X)};
-                            if (b[0] | b[1] | b[2] | b[3]) {
-                                tile[e] = make_uint4(v.x & ~b[0], v.y & ~b[1], v.z & ~b[2], v.w & ~b[3]);
-                                const int key = j * G::KEYS + (e & (G::KEYS * 8 - 1)) / 8;   // 8 pieces of 16 bytes a key
-                                if (key < w.len) atomicMin(&B.bad_from[k & 1], key);
-                            }
-                        }
+                    if (pk_is_value<G::STEPS>(i, n, j) && w.careful) {
+                        uint8_t *tile = skv + slot * G::KV_TILE;
+                        pk_clean_tile<T, HD, G::KEYS>(tile, j * G::KEYS - w.row0, w.len - w.row0, w.careful == 2, seen);
                         holo_mv::fence_proxy_async_smem();
                         __syncwarp();
                     }
@@ -723,8 +775,8 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
                 if (w.careful) wait(&B.bad_known[k & 1], k >> 1);
                 if (!wait_warp(&B.o_done[t][(it + 1) & 1], (it - 1) >> 1)) break;
                 const int i = w.row0 + t * PK_ROWS + r;   // of the sequence
-                const float inv = 1.0f / l;
-                bool finite = !w.careful || i < B.bad_from[k & 1];
+                const float inv = w.careful == 2 ? 1.0f / PK_DOWN / l : 1.0f / l;
+                bool finite = true;            // all of the sums
                 // 32 values a lane at a time; four lanes turn their 16-byte pieces round, so that they store 64 bytes of a row
                 const int part = lane & 3, i4 = i - part, n4 = w.len - i4;   // the first row of the four, rows from it on
                 T *o = (T *)a.out + (size_t)(w.first + min(i4, w.len - 1)) * a.out_row + (size_t)w.head * a.out_head + 8 * part;
@@ -758,9 +810,15 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
                 }
                 __syncwarp();              // a row is written by four lanes
                 if (i < w.len) {
-                    if (!finite && !w.careful) B.again = 1;
-                    else if (!finite) pk_row_alone<T, HD>(a, w.first + i, w.first, w.head);
-                    if (finite && a.lse) a.lse[(size_t)w.head * a.total + w.first + i] = (m + log2f(l)) * 0.6931471805599453f;
+                    if (!w.careful) {
+                        if (!finite) atomicMax(&B.again, 1);
+                    } else if (l > 0.0f && l < INFINITY) {   // else its scores have made the row NaN
+                        // finite weights and values whose sums are not have overflowed (fp16's cannot)
+                        if (std::is_same<T, __nv_bfloat16>::value && !finite) atomicMax(&B.again, 2);
+                        pk_mark_row<T, HD>((T *)a.out + (size_t)(w.first + i) * a.out_row + (size_t)w.head * a.out_head,
+                                           t * PK_ROWS + r, seen);
+                    }
+                    if (a.lse) a.lse[(size_t)w.head * a.total + w.first + i] = (m + log2f(l)) * 0.6931471805599453f;
                 }
                 __syncwarp();
             }

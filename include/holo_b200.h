@@ -328,7 +328,9 @@ int cuda_matmul_quant_batched(float *Y, const void *W, const float *X, int M, in
  * q and out: [total][n_heads][head_dim], k and v: [total][n_kv_heads]
  * [head_dim], with *_row elements from row to row and *_head from head to head
  * (0: dense); head_dim 64, 128 or 256, type HOLO_DT_F16 or HOLO_DT_BF16.
- * Values in masked places, infinities and NaN included, change nothing. */
+ * Values in masked places, infinities and NaN included, change nothing.  A
+ * value of v in a place that a row sees which is not finite is the row's result in
+ * that dim (NaN, the infinity, or NaN for both infinities). */
 typedef struct {
     int type;                       /* HOLO_DT_F16 or HOLO_DT_BF16: q, k, v and out */
     int n_heads, n_kv_heads, head_dim;

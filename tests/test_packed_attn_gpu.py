@@ -216,3 +216,83 @@ def test_refusals(packed):
     with pytest.raises(RuntimeError, match=str(hb.HOLO_E_ARG)):
         packed(q, k, v, cu, scale=-1.0)
     assert packed(q[:0], k[:0], v[:0], cu_of([0])).shape == (0, 4, 64)
+
+
+def microseconds(call):
+    for _ in range(2):
+        call()
+    times = []
+    for _ in range(5):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        call()
+        b.record()
+        b.synchronize()
+        times.append(a.elapsed_time(b) * 1e3)
+    return min(times)
+
+
+@pytest.mark.parametrize("n,heads,n_kv,hd,dtype", [
+    (4096, 2, 1, 128, "f16"), (3000, 2, 2, 64, "bf16"), (2100, 1, 1, 256, "f16"), (40000, 2, 1, 128, "bf16")])
+def test_values_that_rows_see(packed, n, heads, n_kv, hd, dtype):
+    """Values of v that are not finite, in an early token, in a later one and in the last tiles: the rows before them are what they
+    would be without, those from them on have them in the one dim that they are in, and no call is a multiple slower than the
+    walk over V that looks for them and a second pass cost (a few times the call without)."""
+    q, k, v = rows([n, 100], heads, n_kv, hd, dtype, 13)
+    cu = cu_of([n, 100])
+    places = [(5, 3, float("nan")), (17, 10, float("inf")), (n // 2, 10, -float("inf")), (n - 300, 33, -float("inf")),
+              (n - 3, 40, float("inf")), (n - 1, 63, float("nan"))]
+    clean, bad = v.clone(), v.clone()
+    for i, d, x in places:
+        clean[i, 0, d], bad[i, 0, d] = 0, x
+    want, lse = packed(q, k, clean, cu, lse=(a := torch.empty(heads, n + 100, device="cuda"))), a
+    lse2 = torch.empty_like(lse)
+    got = packed(q, k, bad, cu, lse=lse2)
+    assert hb.load().cuda_last_status() == hb.HOLO_OK
+    add = torch.zeros(n + 100, hd, device="cuda")
+    for i, d, x in places:
+        add[i:n, d] += x
+    want = want.float()
+    want[:, :heads // n_kv] += add[:, None]
+    g, finite = got.float(), want.isfinite()
+    assert torch.equal(g.isnan(), want.isnan()) and torch.equal(g[want.isinf()], want[want.isinf()])
+    tol = 2 * ref.bound(*(x.double().cpu().numpy().reshape(-1, hd) for x in (q, k, clean)), hd ** -0.5, dtype)
+    assert (g - want)[finite].abs().max() <= tol
+    assert (lse - lse2).abs().max() <= 1e-4
+    assert microseconds(lambda: packed(q, k, bad, cu)) <= 20 * microseconds(lambda: packed(q, k, clean, cu))
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_large_bfloat16_values_do_not_overflow(packed, hd):
+    """Values near the type's largest: their weighted sums before the division pass fp32's range, the rows do not.  Scores that
+    rise along the keys, so that the weights before the division are large."""
+    lens, heads = [700, 3], 2
+    q, k, v = rows(lens, heads, 1, hd, "bf16", 14)
+    q.fill_(1)
+    k[:] = (torch.arange(703, device="cuda")[:, None, None] / 703 * 6 * hd ** -0.5).to(k.dtype)
+    v = (v.float() * 2.0 ** 120).bfloat16()
+    got = packed(q, k, v, cu_of(lens))
+    small = packed(q, k, (v.float() * 2.0 ** -100).bfloat16(), cu_of(lens))
+    assert hb.load().cuda_last_status() == hb.HOLO_OK and got.isfinite().all()
+    assert torch.equal((got.float() * 2.0 ** -100).bfloat16(), small)
+    v[600, 0, 1] = float("nan")
+    bad = packed(q, k, v, cu_of(lens))
+    assert bad[600:700, :, 1].isnan().all() and bad[:600].isfinite().all() and bad[700:].isfinite().all()
+    got[600:700, :, 1] = bad[600:700, :, 1] = 0
+    assert torch.equal(got, bad)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_rows_outside_the_sequences_are_not_written(packed, hd):
+    """A cu_seqlens that ends before the rows do, at every place in a tile: out and lse past it keep what they hold, of rows that
+    TMA takes and of rows at odd addresses."""
+    q, k, v = rows([300], 2, 1, hd, "f16", 15)
+    want, odd = packed(q, k, v, cu_of([300])), torch.zeros(300, 2 * hd + 1, dtype=q.dtype, device="cuda")
+    odd[:, 1:] = q.flatten(1)
+    tol = 2 * ref.bound(*(x.double().cpu().numpy().reshape(-1, hd) for x in (q, k, v)), hd ** -0.5, "f16")
+    for end in (1, 127, 128, 150, 257, 299):
+        for rows_q in (q, odd[:, 1:].unflatten(1, (2, hd))):
+            out, lse = torch.full_like(q, 9.0), torch.full((2, 300), 9.0, device="cuda")
+            packed(rows_q, k, v, cu_of([end]), out=out, lse=lse)
+            assert (out[end:] == 9).all() and (lse[:, end:] == 9).all()
+            assert (out[:end] - want[:end]).abs().max() <= tol
