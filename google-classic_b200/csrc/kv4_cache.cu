@@ -136,7 +136,8 @@ __device__ __forceinline__ void store8(T *p, bool wide, const T (&x)[8]) {
 
 // Eight codes of a lane and the scale of its group, over the four lanes that
 // hold it: d = fp16(m / -8), code = rint(x / d) + 8 in 0..15 (fp32 arithmetic,
-// each operation rounded once), NaN as the scale where a value is not finite.
+// each operation rounded once), NaN as the scale where a value is not finite or
+// the scale would be infinite (its product with a zero that a sum leaves is not always NaN).
 // Bound by instructions (an append of many rows: 0.79 of the issue slots), so the work is put on the FMA pipe, which takes one a cycle:
 //   m         from the group's largest and smallest value; where they are equal
 //             in size, or zero, from a second look for the first of them
@@ -180,6 +181,7 @@ __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], __half &d) {
     d = finite ? __float2half_rn(m * -0.125f) : __ushort_as_half(0x7e00);
     const float w = __half2float(d);
     const bool usable = w != 0.0f && fabsf(w) <= 65504.0f;   // a scale to divide by: else code 8
+    if (!(fabsf(w) <= 65504.0f)) d = __ushort_as_half(0x7e00);
     const float r = usable ? __frcp_rn(w) : 0.0f;
     const float magic = 12582912.0f;
     uint32_t codes[2];

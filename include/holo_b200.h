@@ -354,7 +354,8 @@ int cuda_attention_packed(const holo_packed_desc *d, void *out, const void *q, c
  * d = m / -8, m the group's value of largest magnitude (the first of them);
  * code = rint(x / d) + 8 clipped to 0..15, and x reads back as
  * d * (code - 8): the arithmetic of GGUF's Q4_0.  A group with a value that is
- * not finite reads back as NaN.
+ * not finite, or is 524,160 or more in size (d would not be), has NaN as d and reads
+ * back as NaN.
  *
  * Layout: pool [n_layers][n_pages][n_kv_heads][page_tokens / 16] blocks of 16
  * positions, 18 * head_dim bytes each (nb = head_dim / 32 groups):

@@ -661,3 +661,27 @@ def test_lengths_that_the_tables_cannot_hold(kv4, length):
     model.same(cache)
     for x, y in zip((cache.tables, cache.refs, cache.lens), before):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("side", [0, 1])
+def test_values_too_large_for_their_scale(kv4, dtype, side):
+    """A group whose largest value is past 8 times fp16's largest has no scale: it reads back as NaN, and a sequence that holds it
+    attends to NaN, whichever way its products would round.  The largest that has one (524,159 rounds to 8 * 65,504) is a value."""
+    cache, held = filled(kv4, [50, 40, 30], 1, 64, 32, 91)
+    g = torch.Generator().manual_seed(92)          # small components among large ones: sums that are not exact
+    q = (torch.randn(3, 16, 64, generator=g) * 10 ** (-4 * torch.rand(3, 16, 64, generator=g))).to(DTYPES[dtype]).cuda()
+    want = cache.attention(0, q).clone()
+    x = [torch.randn(1, 1, 64, generator=torch.Generator().manual_seed(93 + s)).cuda() for s in range(2)]
+    back = [torch.empty_like(y) for y in x]
+    for value, fits in ((524159.0, True), (524160.0, False), (-6e5, False), (3e38, False)):
+        x[side][0, 0, 40] = value
+        cache.append(0, *x, ints(0, 1), ints(49), ints(0))
+        cache.read(0, ints(0, 1), ints(49), *back, ints(0))
+        got = cache.attention(0, q)
+        cache.check()
+        assert back[side][0, 0, 32:].isnan().all() != fits and back[side][0, 0, 32:].isfinite().all() == fits
+        assert back[side][0, 0, :32].isfinite().all() and back[1 - side].isfinite().all()
+        assert torch.equal(got[1:], want[1:])
+        if not fits:
+            assert got[0].isnan().all() if side == 0 else (got[0, :, 32:].isnan().all() and got[0, :, :32].isfinite().all())
