@@ -11,6 +11,8 @@
 #include <stdint.h>
 #include <stddef.h>
 
+#include <vector>
+
 #include "cuda_ops.h"
 #include "holo_b200.h"
 
@@ -145,6 +147,7 @@ struct HoloDevice {
     // whatever shapes of cache the calls are for
     void *kv4_work = nullptr, *kv4_counters = nullptr;
     size_t kv4_work_bytes = 0, kv4_counter_bytes = 0;
+    std::vector<void *> kv4_outgrown;    // smaller ones that came before: captured graphs may hold them
 };
 constexpr int MV_MAX_CTAS = 1024;
 constexpr int MV_MAX_ROWBLOCKS = 1 << 16;

@@ -31,20 +31,23 @@ size_t partial_bytes(const holo_kv4 *c) {
 
 std::mutex g_work_mu;
 
-// a buffer of the library's own on the current device, zero when it is made
-bool own_buffer(void *&buf, size_t &have, size_t bytes) {
+// A buffer of the library's own on the current device, zero when it is made.  One
+// that is too small is kept, since calls under way and captured graphs may hold it; sizes
+// are powers of two, so that all that were outgrown are no larger than the last.
+bool own_buffer(HoloDevice *D, void *&buf, size_t &have, size_t bytes) {
     if (have >= bytes) return true;
-    cudaDeviceSynchronize();   // calls that use the old one
-    if (buf) cudaFree(buf);
-    buf = nullptr;
-    have = 0;
-    if (cudaMalloc(&buf, bytes) != cudaSuccess || cudaMemset(buf, 0, bytes) != cudaSuccess ||
-        cudaDeviceSynchronize() != cudaSuccess) {
+    size_t size = 1 << 16;
+    while (size < bytes) size *= 2;
+    void *p = nullptr;
+    if (cudaMalloc(&p, size) != cudaSuccess || cudaMemset(p, 0, size) != cudaSuccess || cudaDeviceSynchronize() != cudaSuccess) {
         cudaGetLastError();
+        cudaFree(p);
         holo_set_status(HOLO_E_NOMEM, "kv4 workspace");
         return false;
     }
-    have = bytes;
+    if (buf) D->kv4_outgrown.push_back(buf);
+    buf = p;
+    have = size;
     return true;
 }
 
@@ -52,8 +55,8 @@ bool own_buffer(void *&buf, size_t &have, size_t bytes) {
 // call, have a buffer that nothing else is written to; no call reads what another left in the other sections.
 bool own_work(HoloDevice *D, const holo_kv4 *c, Kv4Work *work) {
     std::lock_guard<std::mutex> lk(g_work_mu);
-    if (!own_buffer(D->kv4_counters, D->kv4_counter_bytes, counter_bytes(c)) ||
-        !own_buffer(D->kv4_work, D->kv4_work_bytes, plan_bytes(c) + partial_bytes(c)))
+    if (!own_buffer(D, D->kv4_counters, D->kv4_counter_bytes, counter_bytes(c)) ||
+        !own_buffer(D, D->kv4_work, D->kv4_work_bytes, plan_bytes(c) + partial_bytes(c)))
         return false;
     work->counters = (int *)D->kv4_counters;
     work->plan = (int *)D->kv4_work;

@@ -285,6 +285,7 @@ void cuda_cleanup(void) {
     if (D.tmp) cudaFree(D.tmp);
     if (D.kv4_work) cudaFree(D.kv4_work);
     if (D.kv4_counters) cudaFree(D.kv4_counters);
+    for (void *p : D.kv4_outgrown) cudaFree(p);
     D = HoloDevice();
     std::lock_guard<std::mutex> lk(g_reg_mu);
     g_registry.clear();

@@ -65,3 +65,23 @@ def test_caches_of_different_shapes_share_the_librarys_workspace(kv4):
         big.check()
         assert torch.equal(out_s, want_small), i
         assert torch.equal(out_b, want_big), i
+
+
+def test_a_captured_call_outlives_the_growth_of_the_workspace(kv4):
+    """A graph holds the library's own workspace as it was when it was captured; a later call that needs more leaves that alone."""
+    cache, _ = filled(kv4, [3000, 30], 1, 64, 16, 8)
+    q = queries(2, 4, 64, 9)
+    want, bare, out = cache.attention(0, q), Bare(kv4, cache), torch.zeros_like(q)
+    bare.attention(0, q, out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        bare.attention(0, q, out)
+    many = kv4.Kv4Cache(1, 256, 64, 16, n_pages=40, max_seqs=4000, max_pages=40)   # 2,048,000 counters
+    assert Bare(kv4, many).attention(0, queries(4000, 256, 64, 1), torch.empty(4000, 256, 64, device="cuda")) == hb.HOLO_OK
+    taken = [torch.full((1 << 20,), -1, dtype=torch.int32, device="cuda") for _ in range(40)]
+    for _ in range(3):
+        out.fill_(7)
+        graph.replay()
+        cache.check()
+        assert torch.equal(out, want)
+    assert all(bool((t == -1).all()) for t in taken)
