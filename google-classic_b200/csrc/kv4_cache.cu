@@ -31,6 +31,24 @@ size_t partial_bytes(const holo_kv4 *c) {
 
 std::mutex g_work_mu;
 
+// Device memory, zero, without touching a stream of anyone's: also while one is being captured.
+void *zero_memory(size_t size) {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;   // of this thread, until it is put back
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    void *p = nullptr;
+    cudaStream_t st = nullptr;
+    const bool done = cudaMalloc(&p, size) == cudaSuccess && cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking) == cudaSuccess &&
+                      cudaMemsetAsync(p, 0, size, st) == cudaSuccess && cudaStreamSynchronize(st) == cudaSuccess;
+    if (st) cudaStreamDestroy(st);
+    if (!done) {
+        cudaGetLastError();
+        cudaFree(p);
+        p = nullptr;
+    }
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    return p;
+}
+
 // A buffer of the library's own on the current device, zero when it is made.  One
 // that is too small is kept, since calls under way and captured graphs may hold it; sizes
 // are powers of two, so that all that were outgrown are no larger than the last.
@@ -38,10 +56,8 @@ bool own_buffer(HoloDevice *D, void *&buf, size_t &have, size_t bytes) {
     if (have >= bytes) return true;
     size_t size = 1 << 16;
     while (size < bytes) size *= 2;
-    void *p = nullptr;
-    if (cudaMalloc(&p, size) != cudaSuccess || cudaMemset(p, 0, size) != cudaSuccess || cudaDeviceSynchronize() != cudaSuccess) {
-        cudaGetLastError();
-        cudaFree(p);
+    void *p = zero_memory(size);
+    if (!p) {
         holo_set_status(HOLO_E_NOMEM, "kv4 workspace");
         return false;
     }

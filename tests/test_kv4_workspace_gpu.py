@@ -67,6 +67,25 @@ def test_caches_of_different_shapes_share_the_librarys_workspace(kv4):
         assert torch.equal(out_b, want_big), i
 
 
+def test_a_call_that_needs_more_workspace_inside_a_capture(kv4):
+    """The library's own workspace is made, or grows, while the call's stream is being captured: the capture goes on, and its
+    replays are right."""
+    cache, _ = filled(kv4, [900, 30], 64, 64, 16, 6)
+    wide = kv4.Kv4Cache(1, 64, 64, 16, pool=cache.pool, tables=torch.cat([cache.tables] * 1500).contiguous(),
+                        lens=torch.cat([cache.lens] * 1500).contiguous(), refs=cache.refs)   # 768,000 counters
+    q = queries(2, 64, 64, 7)
+    want, bare, out = cache.attention(0, q), Bare(kv4, wide), torch.zeros_like(q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        rc = bare.attention(0, q, out)
+    assert rc == hb.HOLO_OK
+    for _ in range(3):
+        out.fill_(7)
+        graph.replay()
+        wide.check()
+        assert torch.equal(out, want)
+
+
 def test_a_captured_call_outlives_the_growth_of_the_workspace(kv4):
     """A graph holds the library's own workspace as it was when it was captured; a later call that needs more leaves that alone."""
     cache, _ = filled(kv4, [3000, 30], 1, 64, 16, 8)
