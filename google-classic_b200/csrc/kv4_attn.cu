@@ -764,7 +764,8 @@ kv4_attn_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ AtArg
             }
         }
         if (!whole) {
-            // the item's units lie in parts p0 .. p1; the last part to come joins their results, in order
+            // The item's units lie in parts p0 .. p1; the last part to come joins their results, in order.  (A part that gave up
+            // waiting comes too, so the counter is 0 after every call.)
             const int begins = w.start + a.item_cost;
             const int p0 = begins / step, p1 = (begins + w.units - 1) / step;
             int *counter = a.counters + (size_t)w.i * items + w.item;

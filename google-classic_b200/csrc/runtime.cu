@@ -204,7 +204,6 @@ void cuda_clear_status(void) {
         cudaMemset(g_dev[id].status, 0, sizeof(int));
         cudaMemset(g_dev[id].mv_counters, 0, sizeof(int) * MV_MAX_ROWBLOCKS);
         cudaMemset(g_dev[id].mvb_counters, 0, sizeof(int) * MVB_MAX_GROUPS);
-        if (g_dev[id].kv4_counters) cudaMemset(g_dev[id].kv4_counters, 0, g_dev[id].kv4_counter_bytes);
         cudaDeviceSynchronize();
     }
     int n = 0;

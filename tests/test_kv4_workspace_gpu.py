@@ -104,3 +104,20 @@ def test_a_captured_call_outlives_the_growth_of_the_workspace(kv4):
         cache.check()
         assert torch.equal(out, want)
     assert all(bool((t == -1).all()) for t in taken)
+
+
+def test_clearing_the_status_leaves_calls_under_way_alone(kv4):
+    """cuda_clear_status while split attentions with the library's own workspace run on another stream."""
+    cache, _ = filled(kv4, [60000, 7000], 1, 64, 64, 10)
+    q = queries(2, 8, 64, 11)
+    want, bare, side = cache.attention(0, q), Bare(kv4, cache), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = torch.empty(8, *q.shape, device="cuda")
+        for _ in range(400):
+            out.fill_(7)
+            for o in out:
+                assert bare.attention(0, q, o) == hb.HOLO_OK
+            bare.lib.cuda_clear_status()
+            side.synchronize()
+            assert all(torch.equal(o, want) for o in out)
