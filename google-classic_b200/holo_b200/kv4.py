@@ -14,10 +14,11 @@ import ctypes as C
 import torch
 
 from . import load
-from .attention import DTYPES, check, row_stride, stream_of
+from .attention import DTYPES, LEGACY_STREAM, _device, _raw_stream, check, row_stride, stream_of
 
 BLOCK = 16   # positions a block of a page
 INT = torch.int32
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None)   # absent from builds of torch without CUDA
 
 
 class Kv4Desc(C.Structure):
@@ -45,7 +46,13 @@ class Kv4Cache:
 
     Lists of sequences are int32 vectors on the device; seqs None is the
     first ones in order.  Calls return when they are enqueued.  What a kernel
-    found wrong (no free page, an index out of range) is raised by check()."""
+    found wrong (no free page, an index out of range) is raised by check().
+
+    Each stream that makes calls gets a workspace of its own with its first
+    one, so that calls of several streams and threads may overlap where the
+    cache's contents allow it (attention beside attention; a call that changes
+    what another reads is ordered by the caller).  Calls that a CUDA graph
+    captures share one more: graphs of one cache are replayed one at a time."""
 
     def __init__(self, n_layers: int, n_kv_heads: int, head_dim: int, page_tokens: int = 64, n_pages: int = 0,
                  max_seqs: int = 0, max_pages: int = 0, pool=None, tables=None, lens=None, refs=None, device="cuda"):
@@ -70,19 +77,34 @@ class Kv4Cache:
         self.desc = d = Kv4Desc(n_layers, n_kv_heads, head_dim, page_tokens, pool.shape[1], tables.shape[0],
                                 tables.shape[1], pool.data_ptr(), tables.data_ptr(), lens.data_ptr(),
                                 None if refs is None else refs.data_ptr())
-        self._at = C.addressof(d)
         self._heads = (n_kv_heads, head_dim)
-        size = self.lib.cuda_kv4_work_bytes(self._at)
+        size = self.lib.cuda_kv4_work_bytes(C.addressof(d))
         if size == 0:
             raise ValueError("Kv4Cache: this shape is not supported (head_dim 64/128/256, page_tokens a multiple of 16)")
         self._index = pool.get_device()
         stream_of(self._index)
-        self.work = torch.zeros(size, dtype=torch.uint8, device=pool.device)
+        self.work = torch.zeros(size, dtype=torch.uint8, device=pool.device)   # of captured calls
         d.work = self.work.data_ptr()
+        torch.cuda.current_stream(pool.device).synchronize()   # it is zero before any stream's capture
+        self._of_stream = {}   # stream: (address of its descriptor, the descriptor, its workspace), of calls that none captures
+
+    def _descriptor(self, stream: int):
+        """(address, descriptor, workspace) for calls on `stream`, the current one."""
+        d = Kv4Desc.from_buffer_copy(self.desc)
+        d.stream = stream
+        if stream != LEGACY_STREAM and _capturing():
+            return C.addressof(d), d, self.work
+        work = torch.zeros_like(self.work)   # on this stream, so before its calls
+        d.work = work.data_ptr()
+        return self._of_stream.setdefault(stream, (C.addressof(d), d, work))
 
     def _call(self, what: str, fn, *args):
-        self.desc.stream = stream_of(self._index)
-        rc = fn(self._at, *args)
+        index = self._index
+        stream = (_raw_stream(index) or LEGACY_STREAM) if index == _device() else stream_of(index)   # (which raises)
+        mine = self._of_stream.get(stream)
+        if mine is None or (stream != LEGACY_STREAM and _capturing()):   # (the default stream cannot be captured)
+            mine = self._descriptor(stream)
+        rc = fn(mine[0], *args)
         if rc:
             check(rc, what)
 

@@ -2,6 +2,8 @@
 holo_kv4.work): the library's own, that of a Kv4Cache, and what else may run
 beside or between the calls that use it."""
 import ctypes as C
+import threading
+import time
 
 import pytest
 import torch
@@ -121,3 +123,56 @@ def test_clearing_the_status_leaves_calls_under_way_alone(kv4):
             bare.lib.cuda_clear_status()
             side.synchronize()
             assert all(torch.equal(o, want) for o in out)
+
+
+def test_one_cache_on_several_streams(kv4):
+    """Split attentions of one cache that run beside each other, each stream's with queries of its own, and a captured one among
+    them: none takes another's counts or partial results."""
+    cache, _ = filled(kv4, [60000, 7000], 1, 64, 64, 12)
+    qs = [queries(2, 8, 64, 20 + i) for i in range(4)]
+    want = [cache.attention(0, q) for q in qs]
+    cache.check()
+    outs = [torch.empty(30, *q.shape, device="cuda").fill_(7) for q in qs]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for o in outs[3]:
+            cache.attention(0, qs[3], o)
+    streams = [torch.cuda.Stream() for _ in qs]
+    for _ in range(5):
+        for o in outs:
+            o.fill_(7)
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(streams[3]):
+            graph.replay()
+        for i in range(30):
+            for s, q, o in zip(streams[:3], qs, outs):
+                with torch.cuda.stream(s):
+                    cache.attention(0, q, o[i])
+        torch.cuda.synchronize()
+        cache.check()
+        for o, w in zip(outs, want):
+            assert all(torch.equal(x, w) for x in o)
+
+
+def test_threads_with_streams_of_their_own(kv4):
+    """A call takes the stream that is current in its thread, whatever another thread enters meanwhile."""
+    cache, _ = filled(kv4, [100], 1, 64, 64, 12)
+    meet, seen = threading.Barrier(2), {}
+
+    def call(stream):
+        def entered(at):   # in the library, without the interpreter's lock
+            meet.wait(timeout=20)
+            time.sleep(0.05)
+            seen[stream.cuda_stream] = kv4.Kv4Desc.from_address(at).stream
+            return hb.HOLO_OK
+        with torch.cuda.stream(stream):
+            cache._call("test", entered)
+
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    threads = [threading.Thread(target=call, args=(s,)) for s in streams]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert seen == {s.cuda_stream: s.cuda_stream for s in streams}
