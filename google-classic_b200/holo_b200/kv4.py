@@ -29,9 +29,11 @@ class Kv4Desc(C.Structure):
                 ("stream", C.c_void_p)]
 
 
-def _ints(t, what: str, shape=None):
-    if t.dtype != torch.int32 or not t.is_contiguous() or (shape is not None and tuple(t.shape) != tuple(shape)):
-        raise TypeError(f"{what} is a contiguous int32 tensor{'' if shape is None else ' ' + str(tuple(shape))}")
+def _ints(t, what: str, shape):
+    """t, an int32 tensor of `shape` (-1: any size)."""
+    if (not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or not t.is_contiguous() or t.dim() != len(shape)
+            or any(n not in (-1, m) for n, m in zip(shape, t.shape))):
+        raise TypeError(f"{what} is a contiguous int32 tensor {tuple(shape)}")
     return t
 
 
@@ -59,14 +61,18 @@ class Kv4Cache:
         self.lib = load()
         blocks = page_tokens // BLOCK
         if pool is None:
+            if tables is not None or lens is not None or refs is not None:
+                raise TypeError("Kv4Cache: tables, lens and refs come with a pool")
             pool = torch.zeros(n_layers, n_pages, n_kv_heads, blocks, 18 * head_dim, dtype=torch.uint8, device=device)
             tables = torch.full((max_seqs, max_pages), -1, dtype=torch.int32, device=device)
             lens = torch.zeros(max_seqs, dtype=torch.int32, device=device)
             refs = torch.zeros(n_pages, dtype=torch.int32, device=device)
+        if not isinstance(pool, torch.Tensor):
+            raise TypeError("Kv4Cache: pool is a tensor")
         if pool.dtype != torch.uint8 or not pool.is_contiguous() or pool.dim() != 5 or (
                 tuple(pool.shape[2:]) != (n_kv_heads, blocks, 18 * head_dim)) or pool.shape[0] != n_layers:
             raise TypeError(f"Kv4Cache: pool {tuple(pool.shape)} {pool.dtype}")
-        _ints(tables, "Kv4Cache: tables")
+        _ints(tables, "Kv4Cache: tables", (-1, -1))
         _ints(lens, "Kv4Cache: lens", tables.shape[:1])
         if refs is not None:
             _ints(refs, "Kv4Cache: refs", (pool.shape[1],))

@@ -685,3 +685,19 @@ def test_values_too_large_for_their_scale(kv4, dtype, side):
         assert torch.equal(got[1:], want[1:])
         if not fits:
             assert got[0].isnan().all() if side == 0 else (got[0, :, 32:].isnan().all() and got[0, :, :32].isfinite().all())
+
+
+def test_a_cache_over_tensors_that_do_not_make_one(kv4):
+    """A pool without its tables or lengths, and tensors of other shapes and types, are refused by name."""
+    pool = torch.zeros(1, 4, 2, 1, 18 * 64, dtype=torch.uint8, device="cuda")
+    tables, lens = torch.full((3, 2), -1, dtype=torch.int32, device="cuda"), ints(0, 0, 0)
+    good = dict(pool=pool, tables=tables, lens=lens, refs=ints(0, 0, 0, 0))
+    kv4.Kv4Cache(1, 2, 64, 16, **good)
+    for change in (dict(tables=None), dict(lens=None), dict(tables=tables[0]), dict(tables=tables.long()), dict(tables=tables.t()),
+                   dict(lens=lens[:2]), dict(lens=lens.float()), dict(refs=ints(0, 0)), dict(pool=pool.view(-1)),
+                   dict(pool=pool.view(torch.int8)), dict(tables=[[0, 1]]), dict(pool=None), dict(pool=None, tables=None)):
+        with pytest.raises(TypeError, match="Kv4Cache"):
+            kv4.Kv4Cache(1, 2, 64, 16, **(good | change))
+    for change in (dict(tables=tables.cpu()), dict(lens=lens.cpu()), dict(refs=good["refs"].cpu())):
+        with pytest.raises(ValueError, match="Kv4Cache"):
+            kv4.Kv4Cache(1, 2, 64, 16, **(good | change))
