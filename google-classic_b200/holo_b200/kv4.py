@@ -50,11 +50,11 @@ class Kv4Cache:
     first ones in order.  Calls return when they are enqueued.  What a kernel
     found wrong (no free page, an index out of range) is raised by check().
 
-    Each stream that makes calls gets a workspace of its own with its first
-    one, so that calls of several streams and threads may overlap where the
-    cache's contents allow it (attention beside attention; a call that changes
-    what another reads is ordered by the caller).  Calls that a CUDA graph
-    captures share one more: graphs of one cache are replayed one at a time."""
+    Each stream has a workspace of its own, made with its first call, so that
+    calls of several streams and threads may overlap where the cache's contents
+    allow it (attention beside attention; a call that changes what another
+    reads is ordered by the caller).  Calls that a CUDA graph captures share one
+    more: graphs of one cache are replayed one at a time."""
 
     def __init__(self, n_layers: int, n_kv_heads: int, head_dim: int, page_tokens: int = 64, n_pages: int = 0,
                  max_seqs: int = 0, max_pages: int = 0, pool=None, tables=None, lens=None, refs=None, device="cuda"):
@@ -88,19 +88,20 @@ class Kv4Cache:
         if size == 0:
             raise ValueError("Kv4Cache: this shape is not supported (head_dim 64/128/256, page_tokens a multiple of 16)")
         self._index = pool.get_device()
-        stream_of(self._index)
-        self.work = torch.zeros(size, dtype=torch.uint8, device=pool.device)   # of captured calls
-        d.work = self.work.data_ptr()
-        torch.cuda.current_stream(pool.device).synchronize()   # it is zero before any stream's capture
-        self._of_stream = {}   # stream: (address of its descriptor, the descriptor, its workspace), of calls that none captures
+        stream = stream_of(self._index)
+        self.work = torch.zeros(2 * size, dtype=torch.uint8, device=pool.device)   # this stream's, and that of captured calls
+        d.stream, d.work = stream, self.work.data_ptr()
+        # stream: (address of its descriptor, the descriptor, its workspace), of calls that no graph captures
+        self._of_stream = {stream: (C.addressof(d), d, self.work)}
 
     def _descriptor(self, stream: int):
         """(address, descriptor, workspace) for calls on `stream`, the current one."""
         d = Kv4Desc.from_buffer_copy(self.desc)
-        d.stream = stream
+        d.stream, size = stream, self.work.numel() // 2
         if stream != LEGACY_STREAM and _capturing():
+            d.work = self.work.data_ptr() + size
             return C.addressof(d), d, self.work
-        work = torch.zeros_like(self.work)   # on this stream, so before its calls
+        work = torch.zeros(size, dtype=torch.uint8, device=self.pool.device)   # on this stream, so before its calls
         d.work = work.data_ptr()
         return self._of_stream.setdefault(stream, (C.addressof(d), d, work))
 
