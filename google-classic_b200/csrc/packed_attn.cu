@@ -33,8 +33,9 @@
 // sequences are bound by their items' first and last steps, where only one of
 // softmax and tensor core has work: 29.5 us for four of 1024 (16 heads over 8), 580.
 // O_t is rescaled only when a row's maximum has grown by more than 2^8 since
-// the last time, which after the first key tiles is rare; P <= 256 loses no
-// precision, its rounding being relative.
+// the last time, which after the first key tiles is rare.  In bf16 P's rounding is
+// relative whatever its size.  In fp16 P is taken times 2^7, up to 2^15 then, so that weights
+// down to 2^-32 of the largest count (2^-25 without, and 100,000 such are 0.3 % of a row).
 //
 // A masked place never counts.  Its P is an exact 0, which an infinite or NaN
 // value of V would still make NaN: where a row's result is not finite, the CTA
@@ -213,6 +214,7 @@ __device__ __forceinline__ bool pk_elect() {
 template <typename T> struct PkType;
 template <> struct PkType<__half> {
     static constexpr uint32_t AB = 0;   // fp16 operands
+    static constexpr float LIFT = 7.0f; // log2 of what P is taken times
     static constexpr uint32_t EXPONENT = 0x7c007c00u;
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
         uint32_t r;
@@ -222,6 +224,7 @@ template <> struct PkType<__half> {
 };
 template <> struct PkType<__nv_bfloat16> {
     static constexpr uint32_t AB = (1u << 7) | (1u << 10);   // bf16 operands
+    static constexpr float LIFT = 0.0f;
     static constexpr uint32_t EXPONENT = 0x7f807f80u;
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
         uint32_t r;
@@ -748,7 +751,7 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
                         tc_st32(to + cb, o);
                     }
                 }
-                const float sub = m == -INFINITY ? 0.0f : m;   // nothing but -inf so far: weights 0
+                const float sub = (m == -INFINITY ? 0.0f : m) - PkType<T>::LIFT;   // nothing but -inf so far: weights 0
                 const uint64_t c2 = pk_pair(c, c), sub2 = pk_pair(-sub, -sub);
                 uint64_t sum[2] = {0, 0};
                 uint32_t p[PK_STEP / 2];
@@ -818,7 +821,7 @@ packed_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ C
                         pk_mark_row<T, HD>((T *)a.out + (size_t)(w.first + i) * a.out_row + (size_t)w.head * a.out_head,
                                            t * PK_ROWS + r, seen);
                     }
-                    if (a.lse) a.lse[(size_t)w.head * a.total + w.first + i] = (m + log2f(l)) * 0.6931471805599453f;
+                    if (a.lse) a.lse[(size_t)w.head * a.total + w.first + i] = (m - PkType<T>::LIFT + log2f(l)) * 0.6931471805599453f;
                 }
                 __syncwarp();
             }
