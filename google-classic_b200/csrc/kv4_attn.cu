@@ -38,9 +38,11 @@
 // warp 3500 cycles with two warps a scheduler (two CTAs an SM at 128 dims;
 // 12 warps an SM in three CTAs of 32-position units: 59.6 us against 61.7 in the batch below, but
 // 14.0 against 11.8 for one sequence and 164 against 157 for the long ones).  64 sequences
-// of up to 4096 (64 heads over 8 of 128, fp16): 55.0 us, 3.0 TB/s; 8 of up to
-// 131072 (bf16): 158 to 166 us, 4.0 to 4.2 TB/s; one of 2047 (32 over 32, fp32): 11.6 us, of which launch,
-// cut, tables and joins are 8.
+// of up to 4096 (64 heads over 8 of 128, fp16): 55.7 us, 3.0 TB/s; 8 of up to
+// 131072 (bf16): 154 to 166 us, 4.0 to 4.3 TB/s; one of 2047 (32 over 32, fp32): 11.7 us, of which launch,
+// cut, tables and joins are 8.  9 to 16 heads a KV head are two items, each of which reads and
+// unpacks the cache: 111 us for 64 sequences with 128 heads over 8 (58 with 64 of the same lengths' range).  Head
+// size 256 has room for one CTA an SM: 135 us, and in fp32, where it spills (152 bytes of stores a thread), 275.
 #include "kv4.cuh"
 
 #include <cuda_fp16.h>
@@ -901,7 +903,8 @@ extern "C" int cuda_kv4_attention(const holo_kv4 *c, int layer, void *out, const
     a.wide = (uintptr_t)out % 16 == 0 && out_row * size % 16 == 0;
     a.q_wide = (uintptr_t)q % 16 == 0 && q_row * size % 16 == 0;
     a.counters = work.counters, a.partial = work.partial;
-    // where there may be fewer items than CTAs, each CTA has one at most and its cost is the same for all
+    // Where there may be fewer items than CTAs, each CTA has one at most and its cost is the same for all.  (Two CTAs an SM, as at
+    // 128 dims; the three at 64 and the one at 256 have not been measured apart.)
     a.item_cost = (long long)n * c->n_kv_heads * a.chunks >= holo_dev()->sms * 2 ? AT_ITEM : 0;
     const int sms = holo_dev()->sms;
     bool done;

@@ -7,9 +7,9 @@
 // A CTA takes up to 16 rows, whose places (sequence, page, block) are looked up
 // once; rows that share a block meet in one CTA, so its partly written sectors are
 // completed in L2.  Both kernels move each byte once.  Few rows are bound by
-// latency (of the look-ups, the loads and the call); many, 22,400 of 8 heads of 128
-// in fp16, take 49 us to write (2.4 TB/s), bound by the quantiser's instructions, and
-// 33 us to read (3.6 TB/s), by the look-ups at a CTA's start and the stores.  More rows a CTA
+// latency (of the look-ups, the loads and the call); many, 36,829 of 8 heads of 128
+// in fp16, take 64 us to write (3.0 TB/s), bound by the quantiser's instructions, and
+// 40 us to read (4.8 TB/s), by the look-ups at a CTA's start and the stores.  More rows a CTA
 // (32, 64) or more rows' loads together in the read (2, 4) gained nothing.
 #include "kv4.cuh"
 

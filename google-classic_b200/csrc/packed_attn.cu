@@ -27,11 +27,13 @@
 // K and V into a ring of tiles of 128 keys, warp 11 finds the items and checks V
 // (below).  All of them run on into the next item: its loads and first scores
 // are under way while the softmax warps write the rows of the last.
-// Bound by the tensor core and, in long runs, by the board's power: 1090 TFLOP/s at
-// one sequence of 16383 (64 heads of 128 over 8, bf16; SM clock 1.6 GHz at 1000 W), 890
-// over eight of up to 4096, 1104 at head size 256 (16 heads over 2, 16384).  Short
-// sequences are bound by their items' first and last steps, where only one of
-// softmax and tensor core has work: 29.5 us for four of 1024 (16 heads over 8), 580.
+// One sequence of 16383 (64 heads of 128 over 8, bf16) runs at 1080 TFLOP/s and the
+// board's power (SM clock 1.6 GHz at 1000 W), 16384 at head size 256 (16 heads over 2) at
+// 1104, eight of up to 4096 at 895.  What bounds the last, and all at full clock (zeros in every
+// row), is the two tiles' chains: a step takes 1645 cycles, 1270 of them the softmax's own, where
+// the MMAs of a pair need 1280, so the tensor pipe is busy for half of them; and an item's
+// ends, where only one of softmax and tensor core has work: 5000 to 5800 cycles, 30,000 of a CTA's
+// 150,000 with sequences of up to 2048.  Four of 1024 (16 heads over 8): 29.5 us, 580.
 // O_t is rescaled only when a row's maximum has grown by more than 2^8 since
 // the last time, which after the first key tiles is rare.  In bf16 P's rounding is
 // relative whatever its size.  In fp16 P is taken times 2^7, up to 2^15 then, so that weights

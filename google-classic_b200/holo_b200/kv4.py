@@ -124,7 +124,7 @@ class Kv4Cache:
         return seqs.data_ptr(), seqs.shape[0]
 
     def check(self):
-        """Waits for the work enqueued so far and raises what a kernel found wrong."""
+        """Waits for the current stream's work and raises what a kernel found wrong."""
         torch.cuda.current_stream(self.pool.device).synchronize()
         check(self.lib.cuda_last_status(), "Kv4Cache")
 
