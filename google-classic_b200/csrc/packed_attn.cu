@@ -4,7 +4,7 @@
 // Two kernels.  The tensor-core kernel takes rows that TMA can address (bases
 // and strides of whole 16 bytes); other rows take one warp a row and head, which is
 // about a hundredth as fast (four sequences of 1024, 16 heads of 128 over 8, bf16:
-// 29.5 us and 3.05 ms) but reads any row in place.
+// 29.5 us and 2.9 ms) but reads any row in place.
 //
 // Tensor-core kernel: persistent CTAs, one an SM; an item of work is 256 query
 // rows of one head and sequence, as two tiles of 128, which walk the sequence's
@@ -89,7 +89,7 @@ __device__ __forceinline__ void packed_seq(const PackedArgs &a, int s, int &firs
 
 // ---------------------------------------------------------------------------
 // one warp a row and head: lane l holds dims l, l + 32, ...; online softmax
-// over the row's own keys
+// over the row's own keys; where its sums are not finite, once more with the values that are not apart
 // ---------------------------------------------------------------------------
 template <typename T, int HD>
 __global__ void __launch_bounds__(128)
@@ -107,30 +107,41 @@ packed_simple_kernel(const __grid_constant__ PackedArgs a) {
     packed_seq(a, lo, first, len);
     if (row < first || row >= first + len) return;
     const T *q = (const T *)a.q + row * a.q_row + h * a.q_head;
-    float qv[NB], acc[NB], m = -INFINITY, l = 0.0f;
+    float qv[NB], acc[NB], bad[NB], m, l;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        qv[b] = to_float(q[32 * b + lane]) * a.scale;
-        acc[b] = 0.0f;
-    }
-    for (int j = first; j <= row; ++j) {
-        const T *k = (const T *)a.k + j * a.k_row + h / a.group * a.k_head;
-        const T *v = (const T *)a.v + j * a.v_row + h / a.group * a.v_head;
-        float dot = 0.0f;
+    for (int b = 0; b < NB; ++b) qv[b] = to_float(q[32 * b + lane]) * a.scale;
+    auto walk = [&](auto apart) {   // apart: values that are not finite into `bad`, without weights
+        m = -INFINITY, l = 0.0f;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) dot = fmaf(qv[b], to_float(k[32 * b + lane]), dot);
+        for (int b = 0; b < NB; ++b) acc[b] = bad[b] = 0.0f;
+        for (int j = first; j <= row; ++j) {
+            const T *k = (const T *)a.k + j * a.k_row + h / a.group * a.k_head;
+            const T *v = (const T *)a.v + j * a.v_row + h / a.group * a.v_head;
+            float dot = 0.0f, x[NB];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-        if (dot == -INFINITY) continue;   // weight 0
-        const float mn = fmaxf(m, dot), fix = expf(m - mn), e = expf(dot - mn);
-        l = l * fix + e;
-        m = mn;
+            for (int b = 0; b < NB; ++b) {
+                dot = fmaf(qv[b], to_float(k[32 * b + lane]), dot);
+                x[b] = to_float(v[32 * b + lane]);
+                if (apart && !isfinite(x[b])) bad[b] += x[b], x[b] = 0.0f;
+            }
 #pragma unroll
-        for (int b = 0; b < NB; ++b) acc[b] = fmaf(e, to_float(v[32 * b + lane]), acc[b] * fix);
-    }
+            for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+            if (dot == -INFINITY) continue;   // weight 0
+            const float mn = fmaxf(m, dot), fix = expf(m - mn), e = expf(dot - mn);
+            l = l * fix + e;
+            m = mn;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) acc[b] = fmaf(e, x[b], acc[b] * fix);
+        }
+    };
+    walk(std::false_type());
+    bool finite = true;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) finite = finite && isfinite(acc[b]);
+    if (!__all_sync(0xffffffffu, finite)) walk(std::true_type());
     T *o = (T *)a.out + row * a.out_row + h * a.out_head;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) from_float(acc[b] / l, o[32 * b + lane]);
+    for (int b = 0; b < NB; ++b) from_float(acc[b] / l + bad[b], o[32 * b + lane]);
     if (a.lse && lane == 0) a.lse[(size_t)h * a.total + row] = m + logf(l);
 }
 

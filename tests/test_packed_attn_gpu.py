@@ -314,3 +314,28 @@ def test_many_small_weights_beside_a_large_one(packed, hd, dtype):
     others = torch.arange(n, device="cuda").double() * ratio
     want = (others / (1 + others))[:, None]
     assert ((got - want).abs()[1000:] <= 0.015 * want[1000:]).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_values_of_keys_with_the_smallest_weights(packed, hd, dtype):
+    """An infinite value of a key whose score lies 200 below those after it, and above those before it: a weight is positive in
+    the formula, so the rows from it on are infinite there.  Of rows that TMA takes and of rows at odd addresses."""
+    n, heads = 300, 2
+    q, k, v = rows([n], heads, 1, hd, dtype, 16)
+    q.fill_(1)
+    k.zero_()
+    k[:50] = -400 * hd ** -0.5
+    k[50:200] = -200 * hd ** -0.5
+    v[60, 0, 3], v[10, 0, 5], v[199, 0, 7], v[250, 0, 9] = float("inf"), -float("inf"), float("nan"), float("inf")
+    odd = torch.zeros(n, heads * hd + 1, dtype=q.dtype, device="cuda")
+    odd[:, 1:] = q.flatten(1)
+    for rows_q in (q, odd[:, 1:].unflatten(1, (heads, hd))):
+        lse = torch.empty(heads, n, device="cuda")
+        y = packed(rows_q, k, v, cu_of([n]), lse=lse)
+        assert (y[60:, :, 3] == float("inf")).all() and y[:60, :, 3].isfinite().all()
+        assert (y[10:, :, 5] == -float("inf")).all() and y[:10, :, 5].isfinite().all()
+        assert y[199:, :, 7].isnan().all() and y[:199, :, 7].isfinite().all()
+        assert (y[250:, :, 9] == float("inf")).all() and y[:250, :, 9].isfinite().all()
+        rest = [d for d in range(hd) if d not in (3, 5, 7, 9)]
+        assert y[..., rest].isfinite().all() and lse.isfinite().all()
