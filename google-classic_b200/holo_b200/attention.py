@@ -81,7 +81,7 @@ def attention_packed(q, k, v, cu_seqlens, out=None, lse=None, scale: float = 0.0
     """Causal attention of packed prompts: q [total][n_heads][head_dim], k and
     v [total][n_kv_heads][head_dim] (float16 or bfloat16, any strides between
     rows and heads), cu_seqlens int32 [n_seqs + 1] on the device.  Returns out
-    (made when None); lse, when given, is float32 [n_heads][total] and gets
+    (made when None; it overlaps none of the others); lse, when given, is float32 [n_heads][total] and gets
     each row's log-sum-exp.  scale 0: 1 / sqrt(head_dim)."""
     shape, kv_shape = q.shape, k.shape
     total, n_heads, hd = shape

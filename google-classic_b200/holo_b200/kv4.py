@@ -53,8 +53,9 @@ class Kv4Cache:
     Each stream has a workspace of its own, made with its first call, so that
     calls of several streams and threads may overlap where the cache's contents
     allow it (attention beside attention; a call that changes what another
-    reads is ordered by the caller).  Calls that a CUDA graph captures share one
-    more: graphs of one cache are replayed one at a time."""
+    reads is ordered by the caller).  Calls that CUDA graphs capture share one
+    more: a graph's calls on a cache follow one another, and so do the replays of
+    its graphs."""
 
     def __init__(self, n_layers: int, n_kv_heads: int, head_dim: int, page_tokens: int = 64, n_pages: int = 0,
                  max_seqs: int = 0, max_pages: int = 0, pool=None, tables=None, lens=None, refs=None, device="cuda"):
